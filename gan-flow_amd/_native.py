@@ -60,6 +60,22 @@ class CnfAdamOpts(ctypes.Structure):
                 ("weight_decay", ctypes.c_double)]
 
 
+MAX_MATRICES = 64       # CNF_MAX_MATRICES
+MAX_MATRIX_DIM = 65536  # CNF_MAX_MATRIX_DIM
+NS_MAX_STEPS = 16       # CNF_NS_MAX_STEPS
+DTYPE_IDS = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # CNF_F32, CNF_F16, CNF_BF16
+
+
+class CnfNewtonSchulz(ctypes.Structure):
+    _fields_ = [("steps", ctypes.c_int32), ("reserved", ctypes.c_int32), ("eps", ctypes.c_double),
+                ("a", ctypes.c_double * NS_MAX_STEPS), ("b", ctypes.c_double * NS_MAX_STEPS), ("c", ctypes.c_double * NS_MAX_STEPS)]
+
+
+class CnfMuonOpts(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("momentum", ctypes.c_double), ("weight_decay", ctypes.c_double), ("scale", ctypes.c_double),
+                ("nesterov", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 SOLVER_IDS = {"dopri5": 0, "rk4": 1, "euler": 2, "midpoint": 3}
 DIV_EXACT, DIV_HUTCHINSON = 0, 1
 DIV_RESIDUAL = 256   # CNF_DIV_RESIDUAL, OR-ed into CnfNetDesc.divergence
@@ -74,7 +90,8 @@ EXPORTS = ("cnf_param_count", "cnf_workspace_bytes", "cnf_last_error", "cnf_eval
            "cnf_eval_aug", "cnf_solve_bwd", "cnf_solve_bwd_train", "cnf_nll_loss", "cnf_adam_step", "cnf_debug_fill_lds",
            "cnf_debug_kernel_timing", "cnf_debug_last_kernel_ms", "cnf_activation", "cnf_debug_eval_field_b16",
            "cnf_solve_fwd_static", "cnf_static_scratch_bytes", "cnf_gu_sample", "cnf_gu_sample_rows", "cnf_solve_fwd_times",
-           "cnf_solve_fwd_reg", "cnf_solve_bwd_reg")
+           "cnf_solve_fwd_reg", "cnf_solve_bwd_reg", "cnf_layer_norm_fwd", "cnf_layer_norm_workspace_bytes",
+           "cnf_layer_norm_bwd", "cnf_orthogonalize_workspace_bytes", "cnf_orthogonalize", "cnf_muon_step")
 
 
 def library_path(act="tanh"):
@@ -137,6 +154,20 @@ def load_library(act="tanh"):
     lib.cnf_nll_loss.argtypes = [P, P, I64, ctypes.c_int32, P, P, P, VP]
     lib.cnf_adam_step.restype = ctypes.c_int
     lib.cnf_adam_step.argtypes = [P, P, P, P, P, I64, ctypes.POINTER(CnfAdamOpts), P, VP]
+    I32, D = ctypes.c_int32, ctypes.c_double
+    lib.cnf_layer_norm_fwd.restype = ctypes.c_int
+    lib.cnf_layer_norm_fwd.argtypes = [P, I64, I32, P, P, I32, I64, I64, D, P, P, P, VP]
+    lib.cnf_layer_norm_workspace_bytes.restype = SZ
+    lib.cnf_layer_norm_workspace_bytes.argtypes = [I64, I64]
+    lib.cnf_layer_norm_bwd.restype = ctypes.c_int
+    lib.cnf_layer_norm_bwd.argtypes = [P, I64, P, I64, I32, P, I32, P, P, I64, I64, P, P, P, P, SZ, VP]
+    NS, MO, PP = ctypes.POINTER(CnfNewtonSchulz), ctypes.POINTER(CnfMuonOpts), ctypes.POINTER(ctypes.c_void_p)
+    lib.cnf_orthogonalize_workspace_bytes.restype = SZ
+    lib.cnf_orthogonalize_workspace_bytes.argtypes = [I64, I64, I64]
+    lib.cnf_orthogonalize.restype = ctypes.c_int
+    lib.cnf_orthogonalize.argtypes = [PP, I64, PP, I64, I32, I64, I64, I64, NS, P, SZ, VP]
+    lib.cnf_muon_step.restype = ctypes.c_int
+    lib.cnf_muon_step.argtypes = [PP, I64, PP, I64, PP, I64, I32, I64, I64, I64, MO, NS, P, P, SZ, VP]
     lib.cnf_debug_kernel_timing.restype = ctypes.c_int
     lib.cnf_debug_kernel_timing.argtypes = [ctypes.c_int]
     lib.cnf_debug_last_kernel_ms.restype = ctypes.c_int
@@ -518,6 +549,149 @@ def adam_step(params, grad, exp_avg, exp_avg_sq, state, lr=1e-3, betas=(0.9, 0.9
     with torch.cuda.device(params.device):
         _check(lib.cnf_adam_step(_ptr(params), _ptr(grad), _ptr(exp_avg), _ptr(exp_avg_sq), _ptr(state), n,
                                  ctypes.byref(o), ctypes.c_void_p(_stats_ptr(guard)), _stream()), lib)
+
+
+def _elem(t, name, dtypes=None):
+    """A floating tensor on the HIP device of a type the operators below take (or of one of `dtypes`)."""
+    if not torch.is_tensor(t) or not t.is_cuda:
+        raise CnfError("%s must be a tensor on a HIP device (got %s); there is no CPU fallback" % (name, getattr(t, "device", type(t))))
+    if t.dtype not in (DTYPE_IDS if dtypes is None else dtypes):
+        raise CnfError("%s must be %s (got %s)" % (name, " or ".join(str(d) for d in (DTYPE_IDS if dtypes is None else dtypes)), t.dtype))
+    return t
+
+
+def _rows_of(t):
+    """(tensor, row stride) of a (rows, cols) tensor whose rows are contiguous; a copy where they are not."""
+    if t.stride(1) != 1 and t.shape[1] > 1:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _norm_weight(t, name, x):
+    if t is None:
+        return None
+    _elem(t, name, (torch.float32, x.dtype))
+    if t.shape != (x.shape[1],) or t.device != x.device:
+        raise CnfError("%s must have shape (%d,) on %s (got %s on %s)" % (name, x.shape[1], x.device, tuple(t.shape), t.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _norm_args(x, weight, bias):
+    _elem(x, "x")
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise CnfError("x must be (rows, cols) with cols > 0 (got %s)" % (tuple(x.shape),))
+    weight, bias = _norm_weight(weight, "weight", x), _norm_weight(bias, "bias", x)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise CnfError("weight and bias must have one type (got %s and %s)" % (weight.dtype, bias.dtype))
+    wd = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
+    return weight, bias, wd
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=True):
+    """Layer normalisation of the rows of x (rows, cols).  Returns (y, mean, rstd); the two statistics (rows floats each, what
+    layer_norm_bwd needs) are None where want_stats is false."""
+    lib = load_library()
+    weight, bias, wd = _norm_args(x, weight, bias)
+    x, stride = _rows_of(x)
+    rows, cols = x.shape
+    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
+    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
+    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
+    with torch.cuda.device(x.device):
+        _check(lib.cnf_layer_norm_fwd(_ptr(x), stride, DTYPE_IDS[x.dtype], _ptr(weight), _ptr(bias), DTYPE_IDS[wd], rows, cols, float(eps),
+                                      _ptr(y), _ptr(mean), _ptr(rstd), _stream()), lib)
+    return y, mean, rstd
+
+
+def layer_norm_bwd(dy, x, weight, mean, rstd, want=(True, True, True), wdtype=None):
+    """Gradients of layer_norm_fwd: (dx, dweight, dbias), each None where `want` says so.  wdtype: the type of dweight and
+    dbias where there is no weight to take it from."""
+    lib = load_library()
+    weight, _, wd = _norm_args(x, weight, None)
+    if weight is None and wdtype is not None:
+        wd = wdtype
+    if wd != torch.float32 and wd != x.dtype:
+        raise CnfError("wdtype must be torch.float32 or x's type (got %s)" % (wd,))
+    _elem(dy, "dy", (x.dtype,))
+    if dy.shape != x.shape or dy.device != x.device:
+        raise CnfError("dy must have x's shape %s and device (got %s on %s)" % (tuple(x.shape), tuple(dy.shape), dy.device))
+    x, x_stride = _rows_of(x)
+    dy, dy_stride = _rows_of(dy)
+    rows, cols = x.shape
+    mean, rstd = _dev(mean, "mean", (rows,)), _dev(rstd, "rstd", (rows,))
+    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if want[0] else None
+    dw = torch.empty(cols, dtype=wd, device=x.device) if want[1] else None
+    db = torch.empty(cols, dtype=wd, device=x.device) if want[2] else None
+    if dx is None and dw is None and db is None:
+        return None, None, None
+    with torch.cuda.device(x.device):
+        ws = torch.empty(int(lib.cnf_layer_norm_workspace_bytes(rows, cols)) if want[1] or want[2] else 0, dtype=torch.uint8, device=x.device)
+        _check(lib.cnf_layer_norm_bwd(_ptr(dy), dy_stride, _ptr(x), x_stride, DTYPE_IDS[x.dtype], _ptr(weight), DTYPE_IDS[wd], _ptr(mean),
+                                      _ptr(rstd), rows, cols, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream()), lib)
+    return dx, dw, db
+
+
+def newton_schulz(steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """CnfNewtonSchulz of `steps` steps; coefficients: one (a, b, c), or a sequence of one per step."""
+    steps = int(steps)
+    if not 1 <= steps <= NS_MAX_STEPS:
+        raise CnfError("between 1 and %d Newton-Schulz steps (got %d)" % (NS_MAX_STEPS, steps))
+    coefficients = list(coefficients)
+    if len(coefficients) == 3 and not any(hasattr(c, "__len__") for c in coefficients):
+        coefficients = [coefficients] * steps
+    if len(coefficients) != steps or any(len(t) != 3 for t in coefficients):
+        raise CnfError("coefficients must be (a, b, c), or one (a, b, c) for each of the %d steps" % steps)
+    ns = CnfNewtonSchulz()
+    ns.steps, ns.eps = steps, float(eps)
+    for k, (a, b, c) in enumerate(coefficients):
+        ns.a[k], ns.b[k], ns.c[k] = float(a), float(b), float(c)
+    return ns
+
+
+def _matrices(ts, name, dtype, like=None):
+    """Checks a list of equally shaped and strided matrices with contiguous rows; returns (pointer array, row stride)."""
+    t0 = ts[0]
+    for t in ts:
+        _elem(t, name, (dtype,))
+        if t.dim() != 2 or t.shape != t0.shape or t.device != t0.device or t.stride() != t0.stride() or \
+                (like is not None and (t.shape != like.shape or t.device != like.device)):
+            raise CnfError("%s: matrices of one shape, device and stride are wanted" % name)
+        if t.shape[1] > 1 and t.stride(1) != 1:
+            raise CnfError("%s: rows must be contiguous (strides %s)" % (name, tuple(t.stride())))
+    ld = t0.stride(0) if t0.shape[0] > 1 else t0.shape[1]
+    if t0.shape[0] > 1 and ld < t0.shape[1]:
+        raise CnfError("%s: rows overlap (strides %s)" % (name, tuple(t0.stride())))
+    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]), ld
+
+
+def orthogonalize(gs, outs, ns):
+    """cnf_orthogonalize: writes the orthogonalised matrices of the list `gs` to those of `outs` (one shape, at most MAX_MATRICES)."""
+    lib = load_library()
+    g, ldg = _matrices(gs, "g", _elem(gs[0], "g").dtype)
+    out, ldo = _matrices(outs, "out", gs[0].dtype, gs[0])
+    rows, cols = gs[0].shape
+    dev = gs[0].device
+    with torch.cuda.device(dev):
+        ws = torch.empty(int(lib.cnf_orthogonalize_workspace_bytes(len(gs), rows, cols)), dtype=torch.uint8, device=dev)
+        _check(lib.cnf_orthogonalize(g, ldg, out, ldo, DTYPE_IDS[gs[0].dtype], len(gs), rows, cols, ctypes.byref(ns), _ptr(ws), ws.numel(),
+                                     _stream()), lib)
+    return outs
+
+
+def muon_step(params, grads, momenta, ns, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, guard=None):
+    """cnf_muon_step: one Muon update, in place, of the matrices `params` (a list of one shape, at most MAX_MATRICES) from `grads`
+    (of their type) with the fp32 momenta.  guard: stats words as in adam_step."""
+    lib = load_library()
+    p, ldp = _matrices(params, "params", _elem(params[0], "params").dtype)
+    g, ldg = _matrices(grads, "grads", params[0].dtype, params[0])
+    m, ldm = _matrices(momenta, "momenta", torch.float32, params[0])
+    rows, cols = params[0].shape
+    dev = params[0].device
+    o = CnfMuonOpts(float(lr), float(momentum), float(weight_decay), float(scale), 1 if nesterov else 0, 0)
+    with torch.cuda.device(dev):
+        ws = torch.empty(int(lib.cnf_orthogonalize_workspace_bytes(len(params), rows, cols)), dtype=torch.uint8, device=dev)
+        _check(lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[params[0].dtype], len(params), rows, cols, ctypes.byref(o),
+                                 ctypes.byref(ns), ctypes.c_void_p(_stats_ptr(guard)), _ptr(ws), ws.numel(), _stream()), lib)
 
 
 def gu_desc(mean, sigma, unif_intsect, unif_p, extend_dim):

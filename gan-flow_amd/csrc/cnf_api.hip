@@ -8,6 +8,7 @@
 #include <string>
 
 #include "cnf_launch.h"
+#include "cnf_ops.h"
 #include "cnf_split.h"
 
 namespace cnf {
@@ -757,6 +758,219 @@ int cnf_gu_sample_rows(const CnfGuDesc* gu, uint64_t seed, uint32_t call, int64_
     if (check_gu("cnf_gu_sample_rows", gu)) return 1;
     hipError_t err = cnf::launch_gu_sample_rows(*gu, seed, call, row0, rows, out, (hipStream_t)stream);
     if (err != hipSuccess) return fail("cnf_gu_sample_rows: launch failed: %s", hipGetErrorString(err));
+    return 0;
+}
+
+// ---- operators of a training step outside the solves ------------------------------------------------------------------
+static int elem_bytes(int32_t dtype) { return dtype == CNF_F32 ? 4 : dtype == CNF_F16 || dtype == CNF_BF16 ? 2 : 0; }
+
+static bool misaligned(const void* p, int bytes) { return (uintptr_t)p % (size_t)bytes != 0; }
+
+// rows * cols elements (and the strided extent) must stay far from the end of a 64-bit byte count
+constexpr int64_t kMaxExtent = (int64_t)1 << 46;
+
+static int check_matrix(const char* who, const char* name, int64_t rows, int64_t cols, int64_t stride) {
+    if (stride < 0 || (stride != 0 && rows > kMaxExtent / stride))
+        return fail("%s: %s has an unsupported row stride (%ld)", who, name, (long)stride);
+    return 0;
+}
+
+static int check_norm(const char* who, const void* x, int64_t x_stride, int32_t dtype, const void* weight, const void* bias,
+                      int32_t wdtype, int64_t rows, int64_t cols) {
+    const int e = elem_bytes(dtype), we = elem_bytes(wdtype);
+    if (!e || !we || (wdtype != CNF_F32 && wdtype != dtype))
+        return fail("%s: unsupported types (dtype %d, wdtype %d): fp32, fp16 or bf16, weights fp32 or of x's type", who, dtype, wdtype);
+    if (rows < 0 || cols <= 0 || cols > kMaxExtent || rows > kMaxExtent / cols)
+        return fail("%s: need rows >= 0 and cols > 0 (got %ld, %ld)", who, (long)rows, (long)cols);
+    if (check_matrix(who, "x", rows, cols, x_stride)) return 1;
+    if ((rows > 0 && !x) || misaligned(x, e) || misaligned(weight, we) || misaligned(bias, we))
+        return fail("%s: x must be given, and every pointer aligned to its element type", who);
+    return 0;
+}
+
+int cnf_layer_norm_fwd(const void* x, int64_t x_stride, int32_t dtype, const void* weight, const void* bias, int32_t wdtype,
+                       int64_t rows, int64_t cols, double eps, void* y, float* mean, float* rstd, void* stream) {
+    const char* who = "cnf_layer_norm_fwd";
+    if (check_norm(who, x, x_stride, dtype, weight, bias, wdtype, rows, cols)) return 1;
+    if (!(eps >= 0.) || !std::isfinite(eps)) return fail("%s: eps must be finite and not negative (got %g)", who, eps);
+    if (rows == 0) return 0;
+    if (!y || misaligned(y, elem_bytes(dtype)) || misaligned(mean, 4) || misaligned(rstd, 4))
+        return fail("%s: y must be given, and every pointer aligned to its element type", who);
+    cnf::NormArgs a{};
+    a.x = x;
+    a.x_stride = x_stride;
+    a.weight = weight;
+    a.bias = bias;
+    a.rows = rows;
+    a.cols = cols;
+    a.eps = (float)eps;
+    a.y = y;
+    a.mean = mean;
+    a.rstd = rstd;
+    hipError_t err = cnf::launch_layer_norm_fwd(dtype, wdtype, a, (hipStream_t)stream);
+    if (err != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(err));
+    return 0;
+}
+
+size_t cnf_layer_norm_workspace_bytes(int64_t rows, int64_t cols) {
+    return rows <= 0 || cols <= 0 ? 0 : cnf::layer_norm_workspace_bytes(rows, cols);
+}
+
+int cnf_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int32_t dtype, const void* weight,
+                       int32_t wdtype, const float* mean, const float* rstd, int64_t rows, int64_t cols, void* dx, void* dweight,
+                       void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "cnf_layer_norm_bwd";
+    if (check_norm(who, x, x_stride, dtype, weight, nullptr, wdtype, rows, cols)) return 1;
+    if (check_matrix(who, "dy", rows, cols, dy_stride)) return 1;
+    const int e = elem_bytes(dtype), we = elem_bytes(wdtype);
+    if (rows > 0 && (!dy || !mean || !rstd)) return fail("%s: dy, mean and rstd must be given", who);
+    if (misaligned(dy, e) || misaligned(dx, e) || misaligned(dweight, we) || misaligned(dbias, we) || misaligned(mean, 4) ||
+        misaligned(rstd, 4))
+        return fail("%s: every pointer must be aligned to its element type", who);
+    if (!dx && !dweight && !dbias) return fail("%s: nothing to compute (dx, dweight and dbias are all NULL)", who);
+    if (rows > 0 && (dweight || dbias) &&
+        (!workspace || misaligned(workspace, 16) || workspace_bytes < cnf::layer_norm_workspace_bytes(rows, cols)))
+        return fail("%s: workspace too small or not 16-byte aligned (%zu bytes needed)", who, cnf::layer_norm_workspace_bytes(rows, cols));
+    cnf::NormArgs a{};
+    a.x = x;
+    a.x_stride = x_stride;
+    a.dy = dy;
+    a.dy_stride = dy_stride;
+    a.weight = weight;
+    a.rows = rows;
+    a.cols = cols;
+    a.mean = const_cast<float*>(mean);
+    a.rstd = const_cast<float*>(rstd);
+    a.dx = dx;
+    a.dweight = dweight;
+    a.dbias = dbias;
+    a.part = (float*)workspace;
+    hipError_t err = cnf::launch_layer_norm_bwd(dtype, wdtype, a, (hipStream_t)stream);
+    if (err != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(err));
+    return 0;
+}
+
+// The largest |f| on [0, s] of f(u) = a u + b u^3 + c u^5: at the ends or where f' = a + 3 b u^2 + 5 c u^4 vanishes.
+static double quintic_max(double a, double b, double c, double s) {
+    auto f = [&](double u) { return std::fabs(u * (a + u * u * (b + u * u * c))); };
+    double best = f(s);
+    double roots[2] = {-1., -1.};
+    const double A = 5. * c, B = 3. * b, D = B * B - 4. * A * a;
+    if (A != 0. && D >= 0.) {
+        roots[0] = (-B + std::sqrt(D)) / (2. * A);
+        roots[1] = (-B - std::sqrt(D)) / (2. * A);
+    } else if (A == 0. && B != 0.) {
+        roots[0] = -a / B;
+    }
+    for (double r : roots)
+        if (r > 0. && std::sqrt(r) < s) best = std::fmax(best, f(std::sqrt(r)));
+    return best;
+}
+
+// X (singular values <= s), A = X X^T (<= s^2) and a I + b A + c A^2 (<= its polynomial) must stay within 64, which this bounds
+// before anything is launched.
+static int check_ns(const char* who, const CnfNewtonSchulz* ns) {
+    if (ns->steps < 1 || ns->steps > CNF_NS_MAX_STEPS) return fail("%s: steps must be 1..%d (got %d)", who, CNF_NS_MAX_STEPS, ns->steps);
+    if (ns->reserved != 0) return fail("%s: CnfNewtonSchulz.reserved must be 0", who);
+    if (!(ns->eps > 0.) || !std::isfinite(ns->eps)) return fail("%s: eps must be positive and finite (got %g)", who, ns->eps);
+    double s = 1.;
+    for (int k = 0; k < ns->steps; ++k) {
+        const double a = ns->a[k], b = ns->b[k], c = ns->c[k], t = s * s;
+        double h = std::fmax(std::fabs(a), std::fabs(a + b * t + c * t * t));   // max of |a + b t + c t^2|, t in [0, s^2]
+        if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < t) h = std::fmax(h, std::fabs(a - b * b / (4. * c)));
+        s = quintic_max(a, b, c, s);
+        if (!(h < 60.) || !(s <= 7.5))
+            return fail("%s: the coefficients of step %d (%g, %g, %g) let singular values grow past 7.5: the iteration would diverge",
+                        who, k + 1, a, b, c);
+        s = std::fmax(s * 1.0001, 1e-3);
+    }
+    return 0;
+}
+
+static int check_muon(const char* who, int32_t dtype, int64_t count, int64_t rows, int64_t cols, const CnfNewtonSchulz* ns,
+                      void* workspace, size_t workspace_bytes) {
+    if (!elem_bytes(dtype)) return fail("%s: unsupported type %d: fp32, fp16 or bf16", who, dtype);
+    if (!ns) return fail("%s: NULL pointer", who);
+    if (count < 1 || count > CNF_MAX_MATRICES) return fail("%s: count must be 1..%d (got %ld)", who, CNF_MAX_MATRICES, (long)count);
+    if (rows < 1 || cols < 1 || rows > CNF_MAX_MATRIX_DIM || cols > CNF_MAX_MATRIX_DIM)
+        return fail("%s: rows and cols must be 1..%d (got %ld, %ld)", who, CNF_MAX_MATRIX_DIM, (long)rows, (long)cols);
+    if (check_ns(who, ns)) return 1;
+    if (!workspace || misaligned(workspace, 16) || workspace_bytes < cnf::muon_workspace_bytes(count, rows, cols))
+        return fail("%s: workspace too small or not 16-byte aligned (%zu bytes needed)", who, cnf::muon_workspace_bytes(count, rows, cols));
+    return 0;
+}
+
+static int check_ptrs(const char* who, const char* name, const void* const* p, int64_t count, int64_t rows, int64_t cols, int64_t ld,
+                      int bytes) {
+    if (!p) return fail("%s: NULL pointer (%s)", who, name);
+    if (rows > 1 && (ld < cols || ld > kMaxExtent / rows)) return fail("%s: %s: row stride %ld for %ld columns", who, name, (long)ld, (long)cols);
+    for (int64_t i = 0; i < count; ++i)
+        if (!p[i] || misaligned(p[i], bytes)) return fail("%s: %s[%ld] is NULL or not aligned to its element type", who, name, (long)i);
+    return 0;
+}
+
+size_t cnf_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols) {
+    if (count < 1 || count > CNF_MAX_MATRICES || rows < 1 || cols < 1 || rows > CNF_MAX_MATRIX_DIM || cols > CNF_MAX_MATRIX_DIM) return 0;
+    return cnf::muon_workspace_bytes(count, rows, cols);
+}
+
+int cnf_orthogonalize(const void* const* g, int64_t ldg, void* const* out, int64_t ldo, int32_t dtype, int64_t count, int64_t rows,
+                      int64_t cols, const CnfNewtonSchulz* ns, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "cnf_orthogonalize";
+    if (check_muon(who, dtype, count, rows, cols, ns, workspace, workspace_bytes)) return 1;
+    if (check_ptrs(who, "g", g, count, rows, cols, ldg, elem_bytes(dtype)) ||
+        check_ptrs(who, "out", out, count, rows, cols, ldo, elem_bytes(dtype)))
+        return 1;
+    cnf::MuonArgs a{};
+    a.g = g;
+    a.ldg = ldg;
+    a.out = out;
+    a.ldo = ldo;
+    a.count = (int)count;
+    a.rows = rows;
+    a.cols = cols;
+    a.ns = ns;
+    a.ws = workspace;
+    hipError_t err = cnf::launch_muon(dtype, a, (hipStream_t)stream);
+    if (err != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(err));
+    return 0;
+}
+
+int cnf_muon_step(void* const* params, int64_t ldp, const void* const* grads, int64_t ldg, float* const* momenta, int64_t ldm,
+                  int32_t dtype, int64_t count, int64_t rows, int64_t cols, const CnfMuonOpts* opts, const CnfNewtonSchulz* ns,
+                  const CnfStats* guard, void* workspace, size_t workspace_bytes, void* stream) {
+    const char* who = "cnf_muon_step";
+    if (check_muon(who, dtype, count, rows, cols, ns, workspace, workspace_bytes)) return 1;
+    if (!opts) return fail("%s: NULL pointer", who);
+    if (!(opts->lr >= 0.) || !(opts->momentum >= 0. && opts->momentum < 1.) || !(opts->weight_decay >= 0.) || !(opts->scale >= 0.) ||
+        !std::isfinite(opts->lr * opts->scale) || !std::isfinite(opts->lr * opts->weight_decay) || (opts->nesterov & ~1) ||
+        opts->reserved != 0)
+        return fail("%s: invalid hyper-parameters (lr %g, momentum %g, weight_decay %g, scale %g, nesterov %d)", who, opts->lr,
+                    opts->momentum, opts->weight_decay, opts->scale, opts->nesterov);
+    const int e = elem_bytes(dtype);
+    if (check_ptrs(who, "params", params, count, rows, cols, ldp, e) || check_ptrs(who, "grads", grads, count, rows, cols, ldg, e) ||
+        check_ptrs(who, "momenta", (const void* const*)momenta, count, rows, cols, ldm, 4))
+        return 1;
+    for (int64_t i = 0; i < count; ++i)
+        for (int64_t j = 0; j < i; ++j)
+            if (params[i] == params[j] || momenta[i] == momenta[j])
+                return fail("%s: matrices %ld and %ld are the same parameter or momentum", who, (long)j, (long)i);
+    cnf::MuonArgs a{};
+    a.g = grads;
+    a.ldg = ldg;
+    a.out = params;
+    a.ldo = ldp;
+    a.momenta = momenta;
+    a.ldm = ldm;
+    a.count = (int)count;
+    a.rows = rows;
+    a.cols = cols;
+    a.ns = ns;
+    a.opts = opts;
+    a.guard = guard;
+    a.ws = workspace;
+    hipError_t err = cnf::launch_muon(dtype, a, (hipStream_t)stream);
+    if (err != hipSuccess) return fail("%s: launch failed: %s", who, hipGetErrorString(err));
     return 0;
 }
 

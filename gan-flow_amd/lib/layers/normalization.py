@@ -5,6 +5,9 @@ parity unpinned.  An elementwise map over (rows, d) with d <= 16: ordinary tenso
 integrators; it is a flow layer like CNF (same call signature, contributes its log-determinant)."""
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from ... import _native
 
 
 class MovingBatchNormNd(nn.Module):
@@ -98,3 +101,61 @@ class MovingBatchNorm1d(MovingBatchNormNd):
     @property
     def shape(self):
         return [1, -1]
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _native.layer_norm_fwd(x, weight, bias, eps)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.wdtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        return _native.layer_norm_bwd(dy, x, weight, mean, rstd, ctx.needs_input_grad[:3], ctx.wdtype) + (None,)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """Layer normalisation over the last axis of x: (x - mean) / sqrt(var + eps) * weight + bias, one HIP kernel forward and
+    backward (gan-flow_amd/csrc/cnf_norm.hip).  x: fp32, fp16 or bf16 on a HIP device, any leading axes, weight and bias of
+    x's type or fp32, or None.  Statistics and the sums of the weight gradients are fp32.  Differentiable once."""
+    if not torch.is_tensor(x) or x.dim() == 0:
+        raise _native.CnfError("x must be a tensor with at least one axis (got %s)" % (getattr(x, "shape", type(x)),))
+    x2 = x if x.dim() == 2 else x.reshape(-1 if x.numel() else x[..., 0].numel(), x.shape[-1])
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        y = _LayerNormFn.apply(x2, weight, bias, eps)
+    else:
+        y = _native.layer_norm_fwd(x2, weight, bias, eps, want_stats=False)[0]
+    return y if x.dim() == 2 else y.view(x.shape)
+
+
+class LayerNorm(nn.Module):
+    """Per-row normalisation of the hidden features of a network trained beside a flow (a conditioner, a critic, an encoder):
+    unlike MovingBatchNorm1d it keeps rows apart -- log-likelihoods of single rows, gradient penalties -- and has no running
+    state.  Not a flow layer (it is not invertible): y = layer_norm(x, weight, bias, eps).  The reference has no such layer."""
+
+    def __init__(self, num_features, eps=1e-5, affine=True):
+        super().__init__()
+        self.num_features, self.eps, self.affine = int(num_features), eps, affine
+        if affine:
+            self.weight = nn.Parameter(torch.ones(self.num_features))
+            self.bias = nn.Parameter(torch.zeros(self.num_features))
+        else:
+            self.register_parameter("weight", None)
+            self.register_parameter("bias", None)
+
+    def reset_parameters(self):
+        if self.affine:
+            nn.init.ones_(self.weight)
+            nn.init.zeros_(self.bias)
+
+    def forward(self, x):
+        if x.shape[-1] != self.num_features:
+            raise _native.CnfError("LayerNorm(%d) got %d features" % (self.num_features, x.shape[-1]))
+        return layer_norm(x, self.weight, self.bias, self.eps)
+
+    def extra_repr(self):
+        return "%d, eps=%s, affine=%s" % (self.num_features, self.eps, self.affine)

@@ -1,0 +1,135 @@
+"""The Muon optimiser for the matrices of a network: each update is the momentum with its singular values driven to one
+by Newton-Schulz products (gan-flow_amd/csrc/cnf_muon.hip).  The reference trains with Adam only (the library's
+cnf_adam_step); vectors, and whatever else is not a matrix, stay with it."""
+import math
+
+import torch
+
+from .. import _native
+
+DEFAULT_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at 0 (3.44), hovers around 1: five steps lift 1e-2 .. 1 into 0.7 .. 1.2
+# one call iterates as many matrices side by side as this much workspace holds (at least one): enough to fill the device
+_WORKSPACE_BUDGET = 8 << 30
+
+
+def _chunks(n, rows, cols):
+    lib = _native.load_library()
+    one = int(lib.cnf_orthogonalize_workspace_bytes(1, rows, cols))
+    if not one:
+        raise _native.CnfError("matrices of 1..%d rows and columns (got %d x %d)" % (_native.MAX_MATRIX_DIM, rows, cols))
+    step = max(1, min(_native.MAX_MATRICES, _WORKSPACE_BUDGET // one))
+    return [(i, min(n, i + step)) for i in range(0, n, step)]
+
+
+def orthogonalize(g, steps=5, coefficients=DEFAULT_COEFFICIENTS, eps=1e-7):
+    """X = g / (|g|_F + eps), then `steps` times X <- a X + (b X X^T + c (X X^T)^2) X, for every matrix of g (..., rows, cols);
+    fp32, fp16 or bf16, returned in g's type.  coefficients: (a, b, c), or one such triple per step.  Matrices of zeros
+    stay zero."""
+    _native._elem(g, "g")
+    if g.dim() < 2:
+        raise _native.CnfError("g must be a matrix or a stack of matrices (got shape %s)" % (tuple(g.shape),))
+    ns = _native.newton_schulz(steps, coefficients, eps)
+    out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
+    if g.numel() == 0:
+        return out
+    g3 = g.detach().reshape((-1,) + tuple(g.shape[-2:]))
+    if (g3.shape[2] > 1 and g3.stride(2) != 1) or (g3.shape[1] > 1 and g3.stride(1) < g3.shape[2]):
+        g3 = g3.contiguous()
+    o3 = out.view(g3.shape)
+    for lo, hi in _chunks(len(g3), *g3.shape[1:]):
+        _native.orthogonalize(g3[lo:hi].unbind(0), o3[lo:hi].unbind(0), ns)
+    return out
+
+
+def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, steps=5,
+              coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, guard=None):
+    """One Muon update, in place, of a list of matrices:
+        m <- momentum m + g;   u = g + momentum m (nesterov) or m;   p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)
+    grads: of the parameters' types; momenta: fp32.  Matrices of one shape, type and stride are updated side by side.  The
+    matrices must not overlap.  guard: the stats words of the solve that made the gradients (a failed one changes nothing)."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    if not len(params) == len(grads) == len(momenta):
+        raise _native.CnfError("%d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
+    ns = _native.newton_schulz(steps, coefficients, eps)
+    groups = {}
+    for p, g, m in zip(params, grads, momenta):
+        for name, t in (("params", p), ("grads", g), ("momenta", m)):
+            _native._elem(t, name)
+            if t.dim() != 2:
+                raise _native.CnfError("%s: Muon updates matrices (got shape %s)" % (name, tuple(t.shape)))
+        if p.numel() == 0:
+            continue
+        if g.shape[1] > 1 and g.stride(1) != 1 or g.shape[0] > 1 and g.stride(0) < g.shape[1]:
+            g = g.contiguous()
+        groups.setdefault((p.shape, p.dtype, p.device, p.stride(), g.stride(), m.stride()), []).append((p, g, m))
+    for what in (params, momenta):
+        seen = [t.data_ptr() for t in what if t.numel()]
+        if len(set(seen)) < len(seen):
+            raise _native.CnfError("the same parameter or momentum is given twice")
+    for key, members in groups.items():
+        for lo, hi in _chunks(len(members), *key[0]):
+            ps, gs, ms = zip(*members[lo:hi])
+            _native.muon_step(ps, gs, ms, ns, lr, momentum, nesterov, weight_decay, scale, guard)
+
+
+def adjusted_scale(how, rows, cols):
+    """The factor on the orthogonalised update: 'original' sqrt(max(1, rows / cols)), 'match_rms_adamw' 0.2 sqrt(max(rows, cols)) (the
+    root mean square of an Adam update, so that Adam's learning rate carries over), or a number."""
+    if how == "original":
+        return math.sqrt(max(1.0, rows / cols))
+    if how == "match_rms_adamw":
+        return 0.2 * math.sqrt(max(rows, cols))
+    if isinstance(how, str):
+        raise _native.CnfError("adjust_lr must be 'original', 'match_rms_adamw' or a number (got %r)" % (how,))
+    return float(how)
+
+
+class Muon(torch.optim.Optimizer):
+    """Muon for a model's matrices (2-d parameters on a HIP device); every parameter of one shape is updated in one set of
+    launches.  State per parameter: `momentum_buffer`, fp32.  step() synchronises nothing and can be captured into a graph
+    once the momenta exist (after the first step); a captured step keeps the learning rate it was captured with."""
+
+    def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_steps=5,
+                 ns_coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, adjust_lr="original"):
+        if not (lr >= 0.0 and 0.0 <= momentum < 1.0 and weight_decay >= 0.0 and eps > 0.0):
+            raise ValueError("invalid hyper-parameters (lr %r, momentum %r, weight_decay %r, eps %r)" % (lr, momentum, weight_decay, eps))
+        adjusted_scale(adjust_lr, 1, 1)
+        _native.newton_schulz(ns_steps, ns_coefficients, eps)
+        super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_steps=ns_steps,
+                                      ns_coefficients=ns_coefficients, eps=eps, adjust_lr=adjust_lr))
+        for group in self.param_groups:
+            for p in group["params"]:
+                if p.dim() != 2:
+                    raise ValueError("Muon updates matrices; give parameters of shape %s to another optimizer" % (tuple(p.shape),))
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)   # (casts state to the parameter's type: the momentum is fp32 whatever that is)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(saved, mine):
+            if i in state_dict["state"]:
+                self.state[p]["momentum_buffer"] = state_dict["state"][i]["momentum_buffer"].to(device=p.device, dtype=torch.float32, copy=True)
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_shape = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise _native.CnfError("Muon does not take sparse gradients")
+                state = self.state[p]
+                if not state:
+                    state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+                by_shape.setdefault(p.shape, []).append((p, p.grad, state["momentum_buffer"]))
+            for shape, members in by_shape.items():
+                ps, gs, ms = zip(*members)
+                muon_step(ps, gs, ms, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
+                          weight_decay=group["weight_decay"], scale=adjusted_scale(group["adjust_lr"], *shape), steps=group["ns_steps"],
+                          coefficients=group["ns_coefficients"], eps=group["eps"])
+        return loss

@@ -322,6 +322,67 @@ int cnf_gu_sample(const CnfGuDesc *gu, uint64_t seed, int32_t *state, int64_t ro
  * are N(mean, sigma^2): the prior draws of the sampling protocol and the Gaussian "tail" half of config 3's points.   */
 int cnf_gu_sample_rows(const CnfGuDesc *gu, uint64_t seed, uint32_t call, int64_t row0, int64_t rows, float *out, void *stream);
 
+/* Element types of the operators below: tensors are fp32, fp16 or bf16; every sum, statistic and state is fp32 or wider. */
+enum { CNF_F32 = 0, CNF_F16 = 1, CNF_BF16 = 2 };
+
+/* Layer normalisation of the rows of a (rows x cols) matrix, for the networks trained beside a flow (conditioners, critics,
+ * encoders), whose rows must not mix as they do in a batch norm.  NO COUNTERPART IN THE REFERENCE'S PATH.
+ *     y = (x - mean) * rstd * weight + bias,   mean = sum(x) / cols,   rstd = (sum((x - mean)^2) / cols + eps)^(-1/2)
+ *   x: rows of `cols` contiguous elements, x_stride elements apart (0: one row repeated; rows may overlap);
+ *   weight, bias (cols elements of type wdtype: CNF_F32 or x's type), each nullable (1 and 0);
+ *   y: rows x cols, contiguous, not overlapping x;  mean, rstd: rows floats each, nullable, what the backward pass needs.
+ * rows = 0 enqueues nothing.  A row that holds a NaN or an infinity is NaN throughout; other rows are untouched by it.  */
+int cnf_layer_norm_fwd(const void *x, int64_t x_stride, int32_t dtype, const void *weight, const void *bias, int32_t wdtype,
+                       int64_t rows, int64_t cols, double eps, void *y, float *mean, float *rstd, void *stream);
+
+/* Its gradients: with h = dy * weight and xh = (x - mean) * rstd,
+ *     dx = rstd * (h - mean(h) - xh * mean(h * xh)) per row,   dweight = sum over rows of dy * xh,   dbias = sum of dy.
+ * dx (rows x cols, contiguous, not overlapping x or dy), dweight, dbias (cols elements of type wdtype): each nullable, then not
+ * computed.  rows = 0 writes zeros to dweight and dbias.  workspace: cnf_layer_norm_workspace_bytes() bytes, 16-byte aligned,
+ * any content.  Deterministic: column sums in a fixed order, no atomics.                                                 */
+size_t cnf_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
+int cnf_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, int32_t dtype, const void *weight,
+                       int32_t wdtype, const float *mean, const float *rstd, int64_t rows, int64_t cols, void *dx,
+                       void *dweight, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* Newton-Schulz orthogonalisation, the part of the Muon optimiser that makes an update out of a matrix's gradient.  NO
+ * COUNTERPART IN THE REFERENCE, which trains with Adam.
+ *     X = G / (|G|_F + eps);   for every step k:   A = X X^T,   X <- a[k] X + (b[k] A + c[k] A^2) X        (fewer rows than
+ * columns; a matrix with more rows than columns is iterated transposed), i.e. an odd polynomial of the singular values.
+ * fp32 accuracy whatever the type.  Refused: coefficients whose polynomial leaves [-7.5, 7.5] on the
+ * singular values it is applied to (it would diverge).  */
+#define CNF_NS_MAX_STEPS 16
+#define CNF_MAX_MATRICES 64
+#define CNF_MAX_MATRIX_DIM 65536
+typedef struct CnfNewtonSchulz {
+    int32_t steps;       /* 1 .. CNF_NS_MAX_STEPS */
+    int32_t reserved;    /* 0 */
+    double eps;          /* > 0 */
+    double a[CNF_NS_MAX_STEPS], b[CNF_NS_MAX_STEPS], c[CNF_NS_MAX_STEPS];
+} CnfNewtonSchulz;
+
+/*   g, out: HOST arrays of `count` (1 .. CNF_MAX_MATRICES) device pointers to rows x cols (each 1 .. CNF_MAX_MATRIX_DIM) matrices of type dtype with
+ *   contiguous rows, ldg / ldo elements apart; copied into the kernels' arguments (capturable).  out[i] may be g[i] (with the
+ *   same ld); no other overlap.  workspace: cnf_orthogonalize_workspace_bytes() bytes, 16-byte aligned, any content.     */
+size_t cnf_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols);
+int cnf_orthogonalize(const void *const *g, int64_t ldg, void *const *out, int64_t ldo, int32_t dtype, int64_t count,
+                      int64_t rows, int64_t cols, const CnfNewtonSchulz *ns, void *workspace, size_t workspace_bytes,
+                      void *stream);
+
+/* One Muon update of `count` matrices of one shape, in place:
+ *     M <- momentum M + g;   U = g + momentum M (nesterov) or M;   W <- (1 - lr weight_decay) W - lr scale NS(U)
+ *   params, grads: matrices of type dtype;  momenta: fp32 whatever dtype is (a state: never rounded to fewer bits).
+ *   workspace as above.  guard (nullable): as in cnf_adam_step, a non-zero status there changes nothing.                */
+typedef struct CnfMuonOpts {
+    double lr, momentum, weight_decay, scale;
+    int32_t nesterov;    /* 0 | 1 */
+    int32_t reserved;    /* 0 */
+} CnfMuonOpts;
+int cnf_muon_step(void *const *params, int64_t ldp, const void *const *grads, int64_t ldg, float *const *momenta, int64_t ldm,
+                  int32_t dtype, int64_t count, int64_t rows, int64_t cols, const CnfMuonOpts *opts,
+                  const CnfNewtonSchulz *ns, const struct CnfStats *guard, void *workspace, size_t workspace_bytes,
+                  void *stream);
+
 /* Diagnostics (no counterpart in the reference): fill the LDS of every compute unit with `pattern`.  LDS keeps the
  * previous kernel's content, so the tests poison it (NaN bit patterns) before a solve to prove that no result
  * depends on it.  scratch_word: one uint32 of device memory (never written in practice).                    */
