@@ -850,40 +850,15 @@ int cnf_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t
     return 0;
 }
 
-// The largest |f| on [0, s] of f(u) = a u + b u^3 + c u^5: at the ends or where f' = a + 3 b u^2 + 5 c u^4 vanishes.
-static double quintic_max(double a, double b, double c, double s) {
-    auto f = [&](double u) { return std::fabs(u * (a + u * u * (b + u * u * c))); };
-    double best = f(s);
-    double roots[2] = {-1., -1.};
-    const double A = 5. * c, B = 3. * b, D = B * B - 4. * A * a;
-    if (A != 0. && D >= 0.) {
-        roots[0] = (-B + std::sqrt(D)) / (2. * A);
-        roots[1] = (-B - std::sqrt(D)) / (2. * A);
-    } else if (A == 0. && B != 0.) {
-        roots[0] = -a / B;
-    }
-    for (double r : roots)
-        if (r > 0. && std::sqrt(r) < s) best = std::fmax(best, f(std::sqrt(r)));
-    return best;
-}
-
-// X (singular values <= s), A = X X^T (<= s^2) and a I + b A + c A^2 (<= its polynomial) must stay within 64, which this bounds
-// before anything is launched.
 static int check_ns(const char* who, const CnfNewtonSchulz* ns) {
     if (ns->steps < 1 || ns->steps > CNF_NS_MAX_STEPS) return fail("%s: steps must be 1..%d (got %d)", who, CNF_NS_MAX_STEPS, ns->steps);
     if (ns->reserved != 0) return fail("%s: CnfNewtonSchulz.reserved must be 0", who);
     if (!(ns->eps > 0.) || !std::isfinite(ns->eps)) return fail("%s: eps must be positive and finite (got %g)", who, ns->eps);
-    double s = 1.;
-    for (int k = 0; k < ns->steps; ++k) {
-        const double a = ns->a[k], b = ns->b[k], c = ns->c[k], t = s * s;
-        double h = std::fmax(std::fabs(a), std::fabs(a + b * t + c * t * t));   // max of |a + b t + c t^2|, t in [0, s^2]
-        if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < t) h = std::fmax(h, std::fabs(a - b * b / (4. * c)));
-        s = quintic_max(a, b, c, s);
-        if (!(h < 60.) || !(s <= 7.5))
-            return fail("%s: the coefficients of step %d (%g, %g, %g) let singular values grow past 7.5: the iteration would diverge",
-                        who, k + 1, a, b, c);
-        s = std::fmax(s * 1.0001, 1e-3);
-    }
+    double grow[CNF_NS_MAX_STEPS];
+    const int bad = cnf::ns_bounds(*ns, grow);
+    if (bad)
+        return fail("%s: the coefficients of step %d (%g, %g, %g) let singular values grow past 7.5: the iteration would diverge", who,
+                    bad, ns->a[bad - 1], ns->b[bad - 1], ns->c[bad - 1]);
     return 0;
 }
 

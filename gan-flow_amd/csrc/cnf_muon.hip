@@ -3,7 +3,28 @@
 //   X0 = G / (|G|_F + eps);   A = X X^T;   X <- a X + (b A + c A^2) X     for each step's (a, b, c)
 // on the side that is shorter (m <= n after a transposition), for `count` matrices of one shape at a time.  The Muon update:
 //   M <- mu M + g;   G = g + mu M (Nesterov) or M;   W <- (1 - lr wd) W - lr scale X.
-// The Frobenius norm is summed in double from per-block partial sums added in a fixed order; everything else is fp32.
+//
+// ARITHMETIC.  The steps amplify small singular values (3.4445-fold each with the usual coefficients, 485-fold over five), and
+// a rounding of the operands with them: products of bf16 or fp16 operands leave 2e-2 / 2e-3 of the result wrong, which is not
+// the rounding of any output type here.  An operand is therefore kept as TWO fp16 pieces of its value times 2^10: hi = fp16(v),
+// lo = fp16(v - hi), together 23 bits (|v| < 64, which cnf_api.hip's check of the coefficients guarantees; what lies below
+// 2^-34 is lost, against a norm of at most 1.3).  A product is hi hi + hi lo + lo hi on the fp16 matrix pipe with fp32 sums -- the
+// lo lo term is 2^-22 of it -- at a third of the pipe's 2.5 PFLOP/s instead of the 0.157 of fp32 MFMAs.  The Frobenius norm
+// is summed in double from per-block partial sums added in a fixed order.
+//
+// A gradient far below eps makes X0 = G / eps tiny, below what pieces hold.  X is therefore s Y with a factor s per matrix and
+// step: s = 1 unless |X0|_F < 1/2, then s = |X0|_F, Y = G / |G|_F, and every step takes s to min(1, s max|a + b t + c t^2|), which never lets Y grow
+// before s has reached 1:   A = s^2 Y Y^T,   Y' = (s / s') (a I + b A + c A^2) Y.
+//
+// LAYOUT ("piece matrix").  R x K, padded with zeros to multiples of 64 and stored in blocks of 64 rows x 32 columns, 8 KB
+// each, block (r / 64, k / 32) after block along k.  A row of a block is one 128-byte line: four 16-byte slots of hi, four of lo, slot s
+// at s ^ (row & 7), so that a block copied to LDS as it lies is read by MFMA operands without bank conflicts.
+// Every product is of the form C[r][c] = sum_k P[r][k] Q[c][k] with both operands contiguous along k: A = X X^T, A A (A is
+// symmetric) and X' = (a I + b A + c A^2) X with Q = X^T, which the step that makes X writes beside it.  A and A^2 are symmetric: only
+// tiles on and below the diagonal are computed, and written twice.
+#include <cmath>
+#include <type_traits>
+
 #include "cnf_ops.h"
 
 namespace cnf {
@@ -11,6 +32,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kNormBlocks = 128;
+constexpr float kScale = 1024.f, kInvScale = 1.f / 1024.f;
+constexpr long kBlockBytes = 64 * 128;
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef float float16v __attribute__((ext_vector_type(16)));
 
 struct Ptrs {
     const void* g[CNF_MAX_MATRICES];
@@ -21,18 +48,27 @@ struct Ptrs {
 struct Dims {
     long rows, cols, ldg, ldo, ldm;
     long m, n;      // the shorter and the longer side
+    long mp, np;    // padded
     int tall;       // rows > cols: the iteration runs on the transposed matrix
 };
 
-// the matrix the iteration starts from, before normalisation: X (m x n) and the partial sums of its squares
+// byte offset of element (r, c)'s hi piece in a piece matrix of kc blocks per row panel; its lo piece is at this ^ 64
+__device__ __forceinline__ long piece_at(long r, long c, long kc) {
+    return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ (r & 7)) << 4) + ((c & 7) << 1);
+}
+
+__device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
+    hi = (f16)v;
+    lo = (f16)(v - (float)hi);
+}
+
+// the matrix the iteration starts from, before normalisation: the new momentum, and the partial sums of the matrix's squares
 template <typename T, bool kMuon>
-__global__ __launch_bounds__(kThreads) void begin_kernel(Ptrs p, Dims d, float* x, double* part, float mu, int nesterov,
-                                                         const CnfStats* guard) {
+__global__ __launch_bounds__(kThreads) void begin_kernel(Ptrs p, Dims d, double* part, float mu, int nesterov, const CnfStats* guard) {
     __shared__ double red[kThreads / 64];
     const int mat = blockIdx.y;
     const bool skip = guard && guard->status != 0;
     const T* g = (const T*)p.g[mat];
-    float* xm = x + (long)mat * d.m * d.n;
     double s = 0.;
     for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < d.rows * d.cols; i += (long)gridDim.x * kThreads) {
         const long r = i / d.cols, c = i % d.cols;
@@ -43,7 +79,6 @@ __global__ __launch_bounds__(kThreads) void begin_kernel(Ptrs p, Dims d, float* 
             if (!skip) *pm = mv;
             v = nesterov ? fmaf(mu, mv, v) : mv;
         }
-        xm[d.tall ? c * d.n + r : i] = v;
         s += (double)v * (double)v;
     }
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
@@ -52,67 +87,232 @@ __global__ __launch_bounds__(kThreads) void begin_kernel(Ptrs p, Dims d, float* 
     if (threadIdx.x == 0) part[mat * kNormBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ __launch_bounds__(kThreads) void normalize_kernel(Dims d, float* x, const double* part, double eps) {
-    __shared__ float inv;
-    const int mat = blockIdx.y;
-    if (threadIdx.x == 0) {
-        double s = 0.;
-        for (int k = 0; k < kNormBlocks; ++k) s += part[mat * kNormBlocks + k];
-        inv = (float)(1.0 / (sqrt(s) + eps));
-    }
-    __syncthreads();
-    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < d.m * d.n; i += (long)gridDim.x * kThreads) x[(long)mat * d.m * d.n + i] *= inv;
-}
+struct Grow {
+    float by[CNF_NS_MAX_STEPS];
+};
 
-// C (M x N) = alpha op(P, Q) + beta D;  kNT: sum_k P[i,k] Q[j,k], else sum_k P[i,k] Q[k,j].  64 x 64 tile, 4 x 4 per thread.
-template <bool kNT>
-__global__ __launch_bounds__(kThreads) void gemm_kernel(const float* p, const float* q, const float* dd, float* cc, long M, long N, long K,
-                                                        long bp, long bq, long bd, long bc, float alpha, float beta) {
-    __shared__ float ps[16][65], qs[16][65];
+// X0 = G / (|G| + eps) as the piece matrices X (m x n) and X^T (n x m); one 64 x 64 tile of G per workgroup, through LDS
+template <typename T, bool kMuon>
+__global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* x, char* xt, const double* part, double eps, float mu,
+                                                          int nesterov, Grow grow, float* factors) {
+    __shared__ float tile[64][65];
+    __shared__ double scale;     // (double: the largest and smallest fp32 gradients have a scale outside fp32)
     const int mat = blockIdx.z;
-    p += mat * bp, q += mat * bq, cc += mat * bc;
-    const long i0 = (long)blockIdx.y * 64, j0 = (long)blockIdx.x * 64;
-    const int ti = threadIdx.x >> 4, tj = threadIdx.x & 15;
-    float acc[4][4] = {};
-    for (long k0 = 0; k0 < K; k0 += 16) {
-        for (int e = threadIdx.x; e < 1024; e += kThreads) {
-            const int row = e >> 4, k = e & 15;
-            ps[k][row] = (i0 + row < M && k0 + k < K) ? p[(i0 + row) * K + k0 + k] : 0.f;
-            if (kNT) {
-                qs[k][row] = (j0 + row < N && k0 + k < K) ? q[(j0 + row) * K + k0 + k] : 0.f;
-            } else {
-                const int kk = e >> 6, col = e & 63;
-                qs[kk][col] = (j0 + col < N && k0 + kk < K) ? q[(k0 + kk) * N + j0 + col] : 0.f;
+    if (threadIdx.x < 64) {
+        double s = 0.;
+        for (int k = threadIdx.x; k < kNormBlocks; k += 64) s += part[mat * kNormBlocks + k];
+        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        if (threadIdx.x == 0) {
+            const double norm = sqrt(s);
+            const bool small = norm < eps;                   // |X0| = norm / (norm + eps) < 1/2
+            scale = kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
+            if (blockIdx.x == 0 && blockIdx.y == 0) {
+                float f = small && norm > 0. ? fmaxf((float)(norm / (norm + eps)), 1e-37f) : 1.f;   // (never 0: it divides)
+                for (int k = 0; k < CNF_NS_MAX_STEPS; ++k) {
+                    factors[mat * CNF_NS_MAX_STEPS + k] = f;
+                    f = fminf(1.f, f * grow.by[k]);
+                }
             }
         }
-        __syncthreads();
-        for (int k = 0; k < 16; ++k)
-            for (int u = 0; u < 4; ++u)
-                for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(ps[k][ti + 16 * u], qs[k][tj + 16 * v], acc[u][v]);
-        __syncthreads();
     }
-    for (int u = 0; u < 4; ++u)
-        for (int v = 0; v < 4; ++v) {
-            const long i = i0 + ti + 16 * u, j = j0 + tj + 16 * v;
-            if (i < M && j < N) cc[i * N + j] = alpha * acc[u][v] + (dd ? beta * dd[mat * bd + i * N + j] : 0.f);
+    const T* g = (const T*)p.g[mat];
+    const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 64;
+    __syncthreads();
+    for (int e = threadIdx.x; e < 4096; e += kThreads) {
+        const int i = e >> 6, j = e & 63;
+        const long r = r0 + i, c = c0 + j;
+        float v = 0.f;
+        if (r < d.rows && c < d.cols) {
+            v = to_f32(g[r * d.ldg + c]);
+            if (kMuon) {
+                const float mv = p.m[mat][r * d.ldm + c];     // the new momentum
+                v = nesterov ? fmaf(mu, mv, v) : mv;
+            }
+            v = (float)((double)v * scale);
         }
-}
-
-template <typename T, bool kMuon>
-__global__ __launch_bounds__(kThreads) void end_kernel(Ptrs p, Dims d, const float* x, float decay, float step, const CnfStats* guard) {
-    if (guard && guard->status != 0) return;
-    const int mat = blockIdx.y;
-    T* out = (T*)p.out[mat];
-    const float* xm = x + (long)mat * d.m * d.n;
-    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < d.rows * d.cols; i += (long)gridDim.x * kThreads) {
-        const long r = i / d.cols, c = i % d.cols;
-        const float v = xm[d.tall ? c * d.n + r : i];
-        T* o = out + r * d.ldo + c;
-        *o = from_f32<T>(kMuon ? fmaf(-step, v, decay * to_f32(*o)) : v);
+        tile[i][j] = v;
+    }
+    __syncthreads();
+    // (rows, cols) as they are, then transposed; X gets the one whose rows are the shorter side
+    char* straight = (d.tall ? xt : x) + mat * d.mp * d.np * 4;
+    char* flipped = (d.tall ? x : xt) + mat * d.mp * d.np * 4;
+    const long kc_s = (d.tall ? d.mp : d.np) >> 5, kc_f = (d.tall ? d.np : d.mp) >> 5;
+    for (int e = threadIdx.x; e < 1024; e += kThreads) {
+        const int i = (e & 511) >> 3, q = (e & 7) * 8;
+        half8 hi, lo;
+        for (int k = 0; k < 8; ++k) {
+            f16 h, l;
+            split(e < 512 ? tile[i][q + k] : tile[q + k][i], h, l);
+            hi[k] = h;
+            lo[k] = l;
+        }
+        char* base = e < 512 ? straight : flipped;
+        const long at = e < 512 ? piece_at(r0 + i, c0 + q, kc_s) : piece_at(c0 + i, r0 + q, kc_f);
+        *(half8*)(base + at) = hi;
+        *(half8*)(base + (at ^ 64)) = lo;
     }
 }
 
-template <typename T, bool kMuon>
+constexpr int kGram = 0, kPoly = 1, kApply = 2, kFinal = 3;
+
+struct GemmArgs {
+    const char *p, *q;          // piece matrices; C[r][c] = sum_k P[r][k] Q[c][k]
+    long bp, bq;                // bytes between matrices of the batch
+    int kc;                     // blocks of 32 along k
+    int tiles_r, tiles_c;       // tiles of C (kGram, kPoly: tiles_r x tiles_r symmetric)
+    // kGram, kPoly: C to `c0` (symmetric); kApply: C to c0 and its transpose to c1
+    char *c0, *c1;
+    long b0, b1;
+    int kc0, kc1;
+    float ca, cb, cc;           // kPoly: a I + b P + c C
+    long m;                     // kPoly: rows of the identity
+    const float* factors;       // of this step; the next one's follow
+};
+
+struct FinalArgs : GemmArgs {   // kFinal: the iteration's result to the output matrices, or into the parameters
+    Ptrs ptrs;
+    long rows, cols, ldo;
+    float decay, step;
+    int vec;                    // out's rows can be accessed four elements at a time
+    const CnfStats* guard;
+};
+
+template <int kMode>
+using ArgsOf = std::conditional_t<kMode == kFinal, FinalArgs, GemmArgs>;
+
+using gptr = const __attribute__((address_space(1))) void*;
+using lptr = __attribute__((address_space(3))) void*;
+
+// One T x T tile of C per workgroup of four waves (2 x 2), each a (T/2) x (T/2) square of 32 x 32 MFMA tiles.  A stage is one block column (32 k) of
+// both operands, copied to LDS by global_load_lds one stage ahead of the products.
+template <int T, int kMode, typename O = float, bool kMuon = false>
+__global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
+    constexpr int kStage = 2 * T * 128, kN = T / 64;         // bytes of a stage; 32 x 32 tiles per wave and direction
+    constexpr int kLoads = kStage / 1024 / 4;                // 1 KB copies per wave and stage
+    __shared__ __align__(16) char lds[2][kStage];
+    const int mat = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int ti, tj;
+    if (kMode == kGram || kMode == kPoly) {                  // tile (ti, tj), tj <= ti, of the lower triangle
+        const int id = blockIdx.x;
+        ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+        while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
+        while (ti * (ti + 1) / 2 > id) --ti;
+        tj = id - ti * (ti + 1) / 2;
+    } else {
+        ti = blockIdx.x % a.tiles_r;
+        tj = blockIdx.x / a.tiles_r;
+    }
+    const char* src[kLoads];
+    for (int i = 0; i < kLoads; ++i) {
+        const int kb = wave * kLoads + i;                    // which KB of the stage: T / 8 of them are P's
+        const int row = (kb % (T / 8)) * 8;                  // first of its eight rows
+        const bool is_p = kb < T / 8;
+        const long panel = (long)(is_p ? ti : tj) * (T / 64) + (row >> 6);
+        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + panel * a.kc * kBlockBytes + (row & 63) * 128 + lane * 16;
+    }
+    auto load = [&](int stage, int k) {
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes), (lptr)(&lds[stage][(wave * kLoads + i) * 1024]), 16, 0, 0);
+    };
+    const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
+    const int slot = ((lane >> 5) ^ (lane & 7)) << 4, line = (lane & 31) << 7;
+    float16v acc[kN][kN] = {};
+    load(0, 0);
+    for (int k = 0; k < a.kc; ++k) {
+        __syncthreads();                                     // this stage has landed; the other has been read by every wave
+        if (k + 1 < a.kc) load((k + 1) & 1, k + 1);
+        const char* st = lds[k & 1] + line;
+#pragma unroll
+        for (int kh = 0; kh < 2; ++kh) {
+            half8 ph[kN], pl[kN], qh[kN], ql[kN];
+            for (int u = 0; u < kN; ++u) {
+                const char* pr = st + (wr + u * 32) * 128;
+                const char* qr = st + (T + wc + u * 32) * 128;
+                ph[u] = *(const half8*)(pr + (slot ^ (kh << 5)));
+                pl[u] = *(const half8*)(pr + (slot ^ (kh << 5) ^ 64));
+                qh[u] = *(const half8*)(qr + (slot ^ (kh << 5)));
+                ql[u] = *(const half8*)(qr + (slot ^ (kh << 5) ^ 64));
+            }
+            for (int u = 0; u < kN; ++u)
+                for (int v = 0; v < kN; ++v) {               // operands exchanged: a lane holds four neighbouring columns of a row of C
+                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
+                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
+                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
+                }
+        }
+    }
+    if constexpr (kMode == kFinal) {
+        if (a.guard && a.guard->status != 0) return;
+    }
+    float scale = kInvScale;                                 // from the accumulator to C times 2^10
+    if (kMode != kPoly) {
+        const float f = a.factors[mat * CNF_NS_MAX_STEPS];
+        scale *= kMode == kGram ? f * f : kMode == kApply ? f / a.factors[mat * CNF_NS_MAX_STEPS + 1] : f * kInvScale;
+    }
+    for (int u = 0; u < kN; ++u)
+        for (int v = 0; v < kN; ++v)
+            for (int g = 0; g < 4; ++g) {
+                const long r = (long)ti * T + wr + u * 32 + (lane & 31), c = (long)tj * T + wc + v * 32 + g * 8 + (lane >> 5) * 4;
+                float val[4];
+                for (int e = 0; e < 4; ++e) val[e] = acc[u][v][g * 4 + e] * scale;
+                if constexpr (kMode == kFinal) {
+                    if (r >= a.rows) continue;
+                    O* o = (O*)a.ptrs.out[mat] + r * a.ldo + c;
+                    if (a.vec && c + 4 <= a.cols) {
+                        struct alignas(4 * sizeof(O)) Four { O e[4]; } four;
+                        if (kMuon) four = *(const Four*)o;
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = val[e];
+                            four.e[e] = from_f32<O>(kMuon ? fmaf(-a.step, x, a.decay * to_f32(four.e[e])) : x);
+                        }
+                        *(Four*)o = four;
+                    } else {
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.cols) {
+                                const float x = val[e];
+                                o[e] = from_f32<O>(kMuon ? fmaf(-a.step, x, a.decay * to_f32(o[e])) : x);
+                            }
+                    }
+                } else {
+                const long at = piece_at(r, c, a.kc0);
+                if (kMode == kPoly) {
+                    const char* pm = a.p + mat * a.bp;
+                    const half4 h = *(const half4*)(pm + at), l = *(const half4*)(pm + (at ^ 64));
+                    for (int e = 0; e < 4; ++e) {
+                        val[e] = fmaf(a.cc, val[e], a.cb * ((float)h[e] + (float)l[e]));
+                        if (r == c + e && r < a.m) val[e] += a.ca * kScale;
+                    }
+                }
+                half4 hi, lo;
+                for (int e = 0; e < 4; ++e) {
+                    f16 h, l;
+                    split(val[e], h, l);
+                    hi[e] = h;
+                    lo[e] = l;
+                }
+                char* c0 = a.c0 + mat * a.b0;
+                *(half4*)(c0 + at) = hi;
+                *(half4*)(c0 + (at ^ 64)) = lo;
+                if (kMode == kApply || ti != tj) {
+                    char* ct = kMode == kApply ? a.c1 + mat * a.b1 : c0;
+                    for (int e = 0; e < 4; ++e) {
+                        const long t = piece_at(c + e, r, kMode == kApply ? a.kc1 : a.kc0);
+                        *(f16*)(ct + t) = hi[e];
+                        *(f16*)(ct + (t ^ 64)) = lo[e];
+                    }
+                }
+                }
+            }
+}
+
+long pad_to(long v, long t) { return (v + t - 1) / t * t; }
+
+int tile_of(long count, long m, long n) {
+    const long t = ((m + 127) / 128) * ((n + 127) / 128) * count;
+    return t >= 128 ? 128 : 64;
+}
+
+template <int T, typename O, bool kMuon>
 hipError_t run(const MuonArgs& a, hipStream_t s) {
     Ptrs p{};
     for (int i = 0; i < a.count; ++i) {
@@ -120,39 +320,107 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         p.out[i] = a.out[i];
         p.m[i] = kMuon ? a.momenta[i] : nullptr;
     }
-    Dims d{a.rows, a.cols, a.ldg, a.ldo, a.ldm, a.rows < a.cols ? a.rows : a.cols, a.rows < a.cols ? a.cols : a.rows, a.rows > a.cols};
-    const long mn = d.m * d.n, mm = d.m * d.m;
+    Dims d{};
+    d.rows = a.rows, d.cols = a.cols, d.ldg = a.ldg, d.ldo = a.ldo, d.ldm = a.ldm;
+    d.tall = a.rows > a.cols;
+    d.m = d.tall ? a.cols : a.rows;
+    d.n = d.tall ? a.rows : a.cols;
+    d.mp = pad_to(d.m, T);
+    d.np = pad_to(d.n, T);
+    const long xb = d.mp * d.np * 4, ab = d.mp * d.mp * 4;
     double* part = (double*)a.ws;
-    float *x = (float*)(part + (size_t)a.count * kNormBlocks), *x2 = x + a.count * mn, *A = x2 + a.count * mn, *B = A + a.count * mm;
+    char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *A = xt2 + a.count * xb,
+         *B = A + a.count * ab;
+    float* factors = (float*)(B + a.count * ab);
+    double grow[CNF_NS_MAX_STEPS];
+    if (ns_bounds(*a.ns, grow)) return hipErrorInvalidValue;
+    Grow by{};
+    for (int k = 0; k < a.ns->steps; ++k) by.by[k] = (float)fmax(1., grow[k]);
     const float mu = kMuon ? (float)a.opts->momentum : 0.f;
-    const dim3 elem(kNormBlocks, a.count);
-    begin_kernel<T, kMuon><<<elem, kThreads, 0, s>>>(p, d, x, part, mu, kMuon ? a.opts->nesterov : 0, a.guard);
-    normalize_kernel<<<elem, kThreads, 0, s>>>(d, x, part, a.ns->eps);
-    const unsigned tm = (unsigned)((d.m + 63) / 64), tn = (unsigned)((d.n + 63) / 64);
+    const int nesterov = kMuon ? a.opts->nesterov : 0;
+    begin_kernel<O, kMuon><<<dim3(kNormBlocks, a.count), kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
+    const long rp = d.tall ? d.np : d.mp, cp = d.tall ? d.mp : d.np;
+    pieces_kernel<O, kMuon><<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), a.count), kThreads, 0, s>>>(p, d, x, xt, part, a.ns->eps, mu, nesterov,
+                                                                                                              by, factors);
+    const int tm = (int)(d.mp / T), tn = (int)(d.np / T), km = (int)(d.mp / 32), kn = (int)(d.np / 32);
     for (int k = 0; k < a.ns->steps; ++k) {
-        gemm_kernel<true><<<dim3(tm, tm, a.count), kThreads, 0, s>>>(x, x, nullptr, A, d.m, d.m, d.n, mn, mn, 0, mm, 1.f, 0.f);
-        gemm_kernel<true><<<dim3(tm, tm, a.count), kThreads, 0, s>>>(A, A, A, B, d.m, d.m, d.m, mm, mm, mm, mm, (float)a.ns->c[k], (float)a.ns->b[k]);
-        gemm_kernel<false><<<dim3(tn, tm, a.count), kThreads, 0, s>>>(B, x, x, x2, d.m, d.n, d.m, mm, mn, mn, mn, 1.f, (float)a.ns->a[k]);
-        float* t = x;
-        x = x2;
-        x2 = t;
+        FinalArgs g{};
+        g.p = g.q = x, g.bp = g.bq = xb, g.kc = kn, g.tiles_r = g.tiles_c = tm;
+        g.c0 = A, g.b0 = ab, g.kc0 = km;
+        g.factors = factors + k;
+        const dim3 sym(tm * (tm + 1) / 2, a.count);
+        gemm_kernel<T, kGram><<<sym, kThreads, 0, s>>>(g);
+        g.p = g.q = A, g.bp = g.bq = ab, g.kc = km;
+        g.c0 = B;
+        g.ca = (float)a.ns->a[k], g.cb = (float)a.ns->b[k], g.cc = (float)a.ns->c[k], g.m = d.m;
+        gemm_kernel<T, kPoly><<<sym, kThreads, 0, s>>>(g);
+        const bool last = k + 1 == a.ns->steps;
+        g.p = B, g.bp = ab, g.q = xt, g.bq = xb, g.tiles_r = tm, g.tiles_c = tn;
+        if (!last) {
+            g.c0 = x, g.b0 = xb, g.kc0 = kn;
+            g.c1 = xt2, g.b1 = xb, g.kc1 = km;
+            gemm_kernel<T, kApply><<<dim3(tm * tn, a.count), kThreads, 0, s>>>(g);
+            char* t = xt;
+            xt = xt2;
+            xt2 = t;
+            continue;
+        }
+        if (d.tall) {      // the output's rows are X^T's
+            g.p = xt, g.bp = xb, g.q = B, g.bq = ab, g.tiles_r = tn, g.tiles_c = tm;
+        }
+        g.ptrs = p, g.rows = d.rows, g.cols = d.cols, g.ldo = d.ldo, g.guard = a.guard;
+        g.decay = kMuon ? (float)(1.0 - a.opts->lr * a.opts->weight_decay) : 1.f;
+        g.step = kMuon ? (float)(a.opts->lr * a.opts->scale) : 1.f;
+        g.vec = d.ldo % 4 == 0;
+        for (int i = 0; i < a.count; ++i) g.vec = g.vec && (uintptr_t)p.out[i] % (4 * sizeof(O)) == 0;
+        gemm_kernel<T, kFinal, O, kMuon><<<dim3(tm * tn, a.count), kThreads, 0, s>>>(g);
     }
-    const float decay = kMuon ? (float)(1.0 - a.opts->lr * a.opts->weight_decay) : 1.f;
-    const float step = kMuon ? (float)(a.opts->lr * a.opts->scale) : 1.f;
-    end_kernel<T, kMuon><<<elem, kThreads, 0, s>>>(p, d, x, decay, step, a.guard);
     return hipGetLastError();
 }
 
-template <typename T>
+template <typename O>
 hipError_t run_op(const MuonArgs& a, hipStream_t s) {
-    return a.opts ? run<T, true>(a, s) : run<T, false>(a, s);
+    if (tile_of(a.count, a.rows, a.cols) == 128) return a.opts ? run<128, O, true>(a, s) : run<128, O, false>(a, s);
+    return a.opts ? run<64, O, true>(a, s) : run<64, O, false>(a, s);
 }
 
 }  // namespace
 
+// The largest |f| on [0, s] of f(u) = a u + b u^3 + c u^5: at the ends or where f' = a + 3 b u^2 + 5 c u^4 vanishes.
+static double quintic_max(double a, double b, double c, double s) {
+    auto f = [&](double u) { return std::fabs(u * (a + u * u * (b + u * u * c))); };
+    double best = f(s);
+    double roots[2] = {-1., -1.};
+    const double A = 5. * c, B = 3. * b, D = B * B - 4. * A * a;
+    if (A != 0. && D >= 0.) {
+        roots[0] = (-B + std::sqrt(D)) / (2. * A);
+        roots[1] = (-B - std::sqrt(D)) / (2. * A);
+    } else if (A == 0. && B != 0.) {
+        roots[0] = -a / B;
+    }
+    for (double r : roots)
+        if (r > 0. && std::sqrt(r) < s) best = std::fmax(best, f(std::sqrt(r)));
+    return best;
+}
+
+int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
+    double s = 1.;   // bound of |X|; A = X X^T (<= s^2) and a I + b A + c A^2 have to stay within the pieces' 64
+    for (int k = 0; k < ns.steps; ++k) {
+        const double a = ns.a[k], b = ns.b[k], c = ns.c[k], t = s * s;
+        double h = std::fmax(std::fabs(a), std::fabs(a + b * t + c * t * t));
+        if (c != 0. && -b / (2. * c) > 0. && -b / (2. * c) < t) h = std::fmax(h, std::fabs(a - b * b / (4. * c)));
+        grow[k] = h;
+        s = quintic_max(a, b, c, s);
+        if (!(h < 60.) || !(s <= 7.5)) return k + 1;
+        s = std::fmax(s * 1.0001, 1e-3);
+    }
+    return 0;
+}
+
 size_t muon_workspace_bytes(long count, long rows, long cols) {
-    const size_t m = rows < cols ? rows : cols, n = rows < cols ? cols : rows;
-    return (size_t)count * (kNormBlocks * sizeof(double) + (2 * m * n + 2 * m * m) * sizeof(float));
+    const int t = tile_of(count, rows, cols);
+    const size_t m = pad_to(rows < cols ? rows : cols, t), n = pad_to(rows < cols ? cols : rows, t);
+    return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + 2 * m * m) * 4 + CNF_NS_MAX_STEPS * sizeof(float));
 }
 
 hipError_t launch_muon(int dtype, const MuonArgs& a, hipStream_t s) {

@@ -53,6 +53,9 @@ struct MuonArgs {
     const CnfStats* guard;
     void* ws;
 };
+// bounds the iteration over singular values in [0, 1]: 0, or the number of the first step that lets them leave the range the
+// kernels hold; grow[k]: the largest |a + b t + c t^2| of step k
+int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]);
 size_t muon_workspace_bytes(long count, long rows, long cols);
 hipError_t launch_muon(int dtype, const MuonArgs& a, hipStream_t s);
 
