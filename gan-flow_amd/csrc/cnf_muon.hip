@@ -31,7 +31,7 @@ namespace cnf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kNormBlocks = 128;
+constexpr int kNormBlocks = 512;   // at most, per matrix
 constexpr float kScale = 1024.f, kInvScale = 1.f / 1024.f;
 constexpr long kBlockBytes = 64 * 128;
 
@@ -62,55 +62,91 @@ __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
     lo = (f16)(v - (float)hi);
 }
 
-// the matrix the iteration starts from, before normalisation: the new momentum, and the partial sums of the matrix's squares
-template <typename T, bool kMuon>
+// four neighbouring elements of a row, or the last ones of it
+template <typename T, bool kVec>
+__device__ __forceinline__ void load4(const T* p, long left, float (&v)[4]) {
+    if (kVec) {
+        struct alignas(4 * sizeof(T)) Four { T e[4]; } four = *(const Four*)p;
+        for (int k = 0; k < 4; ++k) v[k] = to_f32(four.e[k]);
+    } else {
+        for (int k = 0; k < 4; ++k) v[k] = k < left ? to_f32(p[k]) : 0.f;
+    }
+}
+
+// The matrix the iteration starts from, before normalisation: the new momentum, and the partial sums of the matrix's squares.  A
+// workgroup takes every gridDim.x-th band of 1024 / cols rows (kVec: cols, strides and pointers allow four elements at a time).
+template <typename T, bool kMuon, bool kVec>
 __global__ __launch_bounds__(kThreads) void begin_kernel(Ptrs p, Dims d, double* part, float mu, int nesterov, const CnfStats* guard) {
     __shared__ double red[kThreads / 64];
     const int mat = blockIdx.y;
     const bool skip = guard && guard->status != 0;
     const T* g = (const T*)p.g[mat];
+    const int quads = (int)((d.cols + 3) / 4);               // groups of four per row
+    const int wide = quads < kThreads ? quads : kThreads;    // threads along a row
+    const int band = kThreads / wide;                        // rows at a time
+    const int tr = threadIdx.x / wide, tc = threadIdx.x % wide;
     double s = 0.;
-    for (long i = (long)blockIdx.x * kThreads + threadIdx.x; i < d.rows * d.cols; i += (long)gridDim.x * kThreads) {
-        const long r = i / d.cols, c = i % d.cols;
-        float v = to_f32(g[r * d.ldg + c]);
-        if (kMuon) {
-            float* pm = p.m[mat] + r * d.ldm + c;
-            const float mv = fmaf(mu, *pm, v);
-            if (!skip) *pm = mv;
-            v = nesterov ? fmaf(mu, mv, v) : mv;
+    for (long r = (long)blockIdx.x * band + tr; tr < band && r < d.rows; r += (long)gridDim.x * band)
+        for (int q = tc; q < quads; q += wide) {
+            const long c = (long)q * 4, left = d.cols - c;
+            float v[4];
+            load4<T, kVec>(g + r * d.ldg + c, left, v);
+            if (kMuon) {
+                float* pm = p.m[mat] + r * d.ldm + c;
+                float m[4];
+                load4<float, kVec>(pm, left, m);
+                for (int k = 0; k < 4; ++k) {
+                    m[k] = fmaf(mu, m[k], v[k]);
+                    v[k] = nesterov ? fmaf(mu, m[k], v[k]) : m[k];
+                }
+                if (!skip) {
+                    if (kVec) {
+                        *(float4*)pm = make_float4(m[0], m[1], m[2], m[3]);
+                    } else {
+                        for (int k = 0; k < 4; ++k)
+                            if (k < left) pm[k] = m[k];
+                    }
+                }
+            }
+            for (int k = 0; k < 4; ++k) s = fma((double)v[k], (double)v[k], s);
         }
-        s += (double)v * (double)v;
-    }
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
     if (threadIdx.x == 0) part[mat * kNormBlocks + blockIdx.x] = (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-struct Grow {
-    float by[CNF_NS_MAX_STEPS];
+struct Steps {
+    int n;
+    float a[CNF_NS_MAX_STEPS], b[CNF_NS_MAX_STEPS], c[CNF_NS_MAX_STEPS];
+    float grow[CNF_NS_MAX_STEPS];   // what s is multiplied by, at most to 1
 };
+
+// what the matrix is multiplied by to become Y times 2^10, and the first factor s
+__device__ __forceinline__ double start_scale(double norm, double eps, float& f) {
+    const bool small = norm < eps;                           // |X0| = norm / (norm + eps) < 1/2
+    f = small && norm > 0. ? fmaxf((float)(norm / (norm + eps)), 1e-37f) : 1.f;   // (never 0: it divides)
+    return (double)kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
+}
 
 // X0 = G / (|G| + eps) as the piece matrices X (m x n) and X^T (n x m); one 64 x 64 tile of G per workgroup, through LDS
 template <typename T, bool kMuon>
-__global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* x, char* xt, const double* part, double eps, float mu,
-                                                          int nesterov, Grow grow, float* factors) {
+__global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* x, char* xt, const double* part, int parts, double eps, float mu,
+                                                          int nesterov, Steps st, float* factors) {
     __shared__ float tile[64][65];
     __shared__ double scale;     // (double: the largest and smallest fp32 gradients have a scale outside fp32)
     const int mat = blockIdx.z;
     if (threadIdx.x < 64) {
         double s = 0.;
-        for (int k = threadIdx.x; k < kNormBlocks; k += 64) s += part[mat * kNormBlocks + k];
+        for (int k = threadIdx.x; k < parts; k += 64) s += part[mat * kNormBlocks + k];
         for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
         if (threadIdx.x == 0) {
-            const double norm = sqrt(s);
-            const bool small = norm < eps;                   // |X0| = norm / (norm + eps) < 1/2
-            scale = kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
+            float f;
+            scale = start_scale(sqrt(s), eps, f);
             if (blockIdx.x == 0 && blockIdx.y == 0) {
-                float f = small && norm > 0. ? fmaxf((float)(norm / (norm + eps)), 1e-37f) : 1.f;   // (never 0: it divides)
                 for (int k = 0; k < CNF_NS_MAX_STEPS; ++k) {
                     factors[mat * CNF_NS_MAX_STEPS + k] = f;
-                    f = fminf(1.f, f * grow.by[k]);
+                    f = fminf(1.f, f * st.grow[k]);
                 }
             }
         }
@@ -180,16 +216,32 @@ struct FinalArgs : GemmArgs {   // kFinal: the iteration's result to the output 
 template <int kMode>
 using ArgsOf = std::conditional_t<kMode == kFinal, FinalArgs, GemmArgs>;
 
+// four neighbouring elements of a row of the result to the output matrix, or into the parameters
+template <typename O, bool kMuon>
+__device__ __forceinline__ void put4(const FinalArgs& a, int mat, long r, long c, const float (&x)[4]) {
+    O* o = (O*)a.ptrs.out[mat] + r * a.ldo + c;
+    if (a.vec && c + 4 <= a.cols) {
+        struct alignas(4 * sizeof(O)) Four { O e[4]; } four;
+        if (kMuon) four = *(const Four*)o;
+        for (int e = 0; e < 4; ++e) four.e[e] = from_f32<O>(kMuon ? fmaf(-a.step, x[e], a.decay * to_f32(four.e[e])) : x[e]);
+        *(Four*)o = four;
+    } else {
+        for (int e = 0; e < 4; ++e)
+            if (c + e < a.cols) o[e] = from_f32<O>(kMuon ? fmaf(-a.step, x[e], a.decay * to_f32(o[e])) : x[e]);
+    }
+}
+
 using gptr = const __attribute__((address_space(1))) void*;
 using lptr = __attribute__((address_space(3))) void*;
 
 // One T x T tile of C per workgroup of four waves (2 x 2), each a (T/2) x (T/2) square of 32 x 32 MFMA tiles.  A stage is one block column (32 k) of
-// both operands, copied to LDS by global_load_lds one stage ahead of the products.
+// both operands, copied to LDS by global_load_lds kStages - 1 stages ahead of the products.
 template <int T, int kMode, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
     constexpr int kStage = 2 * T * 128, kN = T / 64;         // bytes of a stage; 32 x 32 tiles per wave and direction
     constexpr int kLoads = kStage / 1024 / 4;                // 1 KB copies per wave and stage
-    __shared__ __align__(16) char lds[2][kStage];
+    constexpr int kStages = T == 64 ? 4 : 2;                 // 64 KB either way: two workgroups per CU
+    __shared__ __align__(16) char lds[kStages][kStage];
     const int mat = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int ti, tj;
     if (kMode == kGram || kMode == kPoly) {                  // tile (ti, tj), tj <= ti, of the lower triangle
@@ -217,11 +269,17 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
     const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
     const int slot = ((lane >> 5) ^ (lane & 7)) << 4, line = (lane & 31) << 7;
     float16v acc[kN][kN] = {};
-    load(0, 0);
+    for (int k = 0; k < kStages - 1 && k < a.kc; ++k) load(k, k);
     for (int k = 0; k < a.kc; ++k) {
-        __syncthreads();                                     // this stage has landed; the other has been read by every wave
-        if (k + 1 < a.kc) load((k + 1) & 1, k + 1);
-        const char* st = lds[k & 1] + line;
+        // this stage has landed (the kStages - 2 after it may be on their way), and every wave's reads of the one before are done
+        if (k + kStages - 1 <= a.kc)
+            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (k + kStages - 1 < a.kc) load((k + kStages - 1) % kStages, k + kStages - 1);
+        const char* st = lds[k % kStages] + line;
 #pragma unroll
         for (int kh = 0; kh < 2; ++kh) {
             half8 ph[kN], pl[kN], qh[kN], ql[kN];
@@ -256,23 +314,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
                 float val[4];
                 for (int e = 0; e < 4; ++e) val[e] = acc[u][v][g * 4 + e] * scale;
                 if constexpr (kMode == kFinal) {
-                    if (r >= a.rows) continue;
-                    O* o = (O*)a.ptrs.out[mat] + r * a.ldo + c;
-                    if (a.vec && c + 4 <= a.cols) {
-                        struct alignas(4 * sizeof(O)) Four { O e[4]; } four;
-                        if (kMuon) four = *(const Four*)o;
-                        for (int e = 0; e < 4; ++e) {
-                            const float x = val[e];
-                            four.e[e] = from_f32<O>(kMuon ? fmaf(-a.step, x, a.decay * to_f32(four.e[e])) : x);
-                        }
-                        *(Four*)o = four;
-                    } else {
-                        for (int e = 0; e < 4; ++e)
-                            if (c + e < a.cols) {
-                                const float x = val[e];
-                                o[e] = from_f32<O>(kMuon ? fmaf(-a.step, x, a.decay * to_f32(o[e])) : x);
-                            }
-                    }
+                    if (r < a.rows) put4<O, kMuon>(a, mat, r, c, val);
                 } else {
                 const long at = piece_at(r, c, a.kc0);
                 if (kMode == kPoly) {
@@ -305,83 +347,252 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
             }
 }
 
-long pad_to(long v, long t) { return (v + t - 1) / t * t; }
-
-int tile_of(long count, long m, long n) {
-    const long t = ((m + 127) / 128) * ((n + 127) / 128) * count;
-    return t >= 128 ? 128 : 64;
+// Matrices of at most 64 x 64: one workgroup per matrix does the whole update, with X, X^T, A and a I + b A + c A^2 as piece matrices in LDS
+// (two blocks of 8 KB each).  A wave computes one 32 x 32 quadrant of every product.  What bounds it is the chain: 3 products per
+// step, each a barrier, its operands' LDS reads, 12 dependent MFMAs and the split of its result.
+template <typename O, bool kMuon>
+__global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, Steps st, double eps, float mu, int nesterov) {
+    __shared__ __align__(16) char xs[2 * kBlockBytes], xts[2 * kBlockBytes], as[2 * kBlockBytes], bs[2 * kBlockBytes];
+    __shared__ double red[kThreads / 64];
+    const int mat = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const bool skip = a.guard && a.guard->status != 0;
+    const O* g = (const O*)a.ptrs.g[mat];
+    // the matrix: thread (tr, tc) holds four rows of four columns
+    const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
+    float v[4][4];
+    double s = 0.;
+    for (int i = 0; i < 4; ++i) {
+        const int r = tr * 4 + i;
+        for (int k = 0; k < 4; ++k) {
+            const int c = tc + k;
+            float u = 0.f;
+            if (r < a.rows && c < a.cols) {
+                u = to_f32(g[r * d.ldg + c]);
+                if (kMuon) {
+                    float* pm = a.ptrs.m[mat] + r * d.ldm + c;
+                    const float mv = fmaf(mu, *pm, u);
+                    if (!skip) *pm = mv;
+                    u = nesterov ? fmaf(mu, mv, u) : mv;
+                }
+            }
+            v[i][k] = u;
+            s = fma((double)u, (double)u, s);
+        }
+    }
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    float f;
+    const double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
+    char *straight = d.tall ? xts : xs, *flipped = d.tall ? xs : xts;
+    for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < 4; ++k) v[i][k] = (float)((double)v[i][k] * scale);
+    for (int i = 0; i < 4; ++i) {
+        half4 h, l, ht, lt;
+        for (int k = 0; k < 4; ++k) {
+            f16 hi, lo;
+            split(v[i][k], hi, lo);
+            h[k] = hi, l[k] = lo;
+            split(v[k][i], hi, lo);
+            ht[k] = hi, lt[k] = lo;
+        }
+        const long at = piece_at(tr * 4 + i, tc, 2), att = piece_at(tc + i, tr * 4, 2);
+        *(half4*)(straight + at) = h;
+        *(half4*)(straight + (at ^ 64)) = l;
+        *(half4*)(flipped + att) = ht;
+        *(half4*)(flipped + (att ^ 64)) = lt;
+    }
+    const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
+    const int slot = ((lane >> 5) ^ (lane & 7)) << 4, line = (lane & 31) << 7;
+    // quadrant (pr, qr) of sum_k P[r][k] Q[c][k]: a lane holds columns 8 g + 4 (lane / 32) + e of row lane % 32
+    auto multiply = [&](const char* p, int pr, const char* q, int qr) {
+        float16v acc = {};
+#pragma unroll
+        for (int kb = 0; kb < 4; ++kb) {
+            const char *pp = p + (kb >> 1) * kBlockBytes + pr * 128 + line, *qq = q + (kb >> 1) * kBlockBytes + qr * 128 + line;
+            const int so = slot ^ ((kb & 1) << 5);
+            const half8 ph = *(const half8*)(pp + so), pl = *(const half8*)(pp + (so ^ 64));
+            const half8 qh = *(const half8*)(qq + so), ql = *(const half8*)(qq + (so ^ 64));
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+        }
+        return acc;
+    };
+    const int row = wr + (lane & 31), col = wc + (lane >> 5) * 4;
+    auto store = [&](char* to, char* flip, const float16v& x) {      // pieces of the quadrant, and of its transpose where flip is given
+        for (int q = 0; q < 4; ++q) {
+            half4 h, l;
+            for (int e = 0; e < 4; ++e) {
+                f16 hi, lo;
+                split(x[q * 4 + e], hi, lo);
+                h[e] = hi, l[e] = lo;
+            }
+            const long at = piece_at(row, col + q * 8, 2);
+            *(half4*)(to + at) = h;
+            *(half4*)(to + (at ^ 64)) = l;
+            if (flip)
+                for (int e = 0; e < 4; ++e) {
+                    const long t = piece_at(col + q * 8 + e, row, 2);
+                    *(f16*)(flip + t) = h[e];
+                    *(f16*)(flip + (t ^ 64)) = l[e];
+                }
+        }
+    };
+    for (int k = 0; k < st.n; ++k) {
+        __syncthreads();
+        float16v A = multiply(xs, wr, xs, wc);
+        for (int i = 0; i < 16; ++i) A[i] *= kInvScale * f * f;
+        store(as, nullptr, A);
+        __syncthreads();
+        float16v B = multiply(as, wr, as, wc);
+        for (int i = 0; i < 16; ++i) {
+            B[i] = fmaf(st.c[k] * kInvScale, B[i], st.b[k] * A[i]);
+            if (row == col + (i >> 2) * 8 + (i & 3) && row < d.m) B[i] += st.a[k] * kScale;
+        }
+        store(bs, nullptr, B);
+        __syncthreads();
+        if (k + 1 < st.n) {
+            float16v X = multiply(bs, wr, xts, wc);
+            const float f1 = fminf(1.f, f * st.grow[k]);
+            for (int i = 0; i < 16; ++i) X[i] *= kInvScale * (f / f1);
+            f = f1;
+            __syncthreads();                                 // everybody has read X^T
+            store(xs, xts, X);
+        }
+    }
+    if (skip) return;
+    const float16v X = d.tall ? multiply(xts, wr, bs, wc) : multiply(bs, wr, xts, wc);
+    if (row >= a.rows) return;
+    for (int q = 0; q < 4; ++q) {
+        float val[4];
+        for (int e = 0; e < 4; ++e) val[e] = X[q * 4 + e] * (kInvScale * kInvScale * f);
+        if (col + q * 8 < a.cols) put4<O, kMuon>(a, mat, row, col + q * 8, val);
+    }
 }
 
-template <int T, typename O, bool kMuon>
+long pad_to(long v, long t) { return (v + t - 1) / t * t; }
+
+// The tile of a product of `tiles` 128 x 128 tiles: 128 reads its operands half as often, 64 has four times the workgroups.
+bool wide_tiles(long tiles) { return tiles >= 160; }
+
+struct Plan {
+    long m, n, mp, np;
+    bool wide_sym, wide_full;
+    bool small;     // one workgroup per matrix does everything in LDS
+};
+
+Plan plan_of(long count, long rows, long cols) {
+    Plan p{};
+    p.m = rows < cols ? rows : cols;
+    p.n = rows < cols ? cols : rows;
+    p.small = p.n <= 64;
+    const long t = pad_to(p.m, 128) / 128, u = pad_to(p.n, 128) / 128;
+    p.wide_sym = wide_tiles(t * (t + 1) / 2 * count);
+    p.wide_full = wide_tiles(t * u * count);
+    const long to = p.wide_sym || p.wide_full ? 128 : 64;
+    p.mp = pad_to(p.m, to);
+    p.np = pad_to(p.n, to);
+    return p;
+}
+
+template <int kMode, typename O = float, bool kMuon = false>
+void product(bool wide, const FinalArgs& args, const Plan& p, bool transposed, int count, hipStream_t s) {
+    FinalArgs g = args;
+    const int t = wide ? 128 : 64, tm = (int)(p.mp / t), tn = (int)(p.np / t);
+    const bool sym = kMode == kGram || kMode == kPoly;
+    g.tiles_r = transposed ? tn : tm;
+    g.tiles_c = sym ? tm : transposed ? tm : tn;
+    const dim3 grid(sym ? tm * (tm + 1) / 2 : tm * tn, count);
+    if (wide)
+        gemm_kernel<128, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+    else
+        gemm_kernel<64, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+}
+
+template <typename O, bool kMuon>
 hipError_t run(const MuonArgs& a, hipStream_t s) {
+    double grow[CNF_NS_MAX_STEPS];
+    if (ns_bounds(*a.ns, grow)) return hipErrorInvalidValue;
+    Steps st{};
+    st.n = a.ns->steps;
+    for (int k = 0; k < st.n; ++k) {
+        st.a[k] = (float)a.ns->a[k];
+        st.b[k] = (float)a.ns->b[k];
+        st.c[k] = (float)a.ns->c[k];
+        st.grow[k] = (float)fmax(1., grow[k]);
+    }
+    const Plan pl = plan_of(a.count, a.rows, a.cols);
     Ptrs p{};
+    bool vec_in = a.cols % 4 == 0 && a.ldg % 4 == 0 && (!kMuon || a.ldm % 4 == 0), vec_out = a.ldo % 4 == 0;
     for (int i = 0; i < a.count; ++i) {
         p.g[i] = a.g[i];
         p.out[i] = a.out[i];
         p.m[i] = kMuon ? a.momenta[i] : nullptr;
+        vec_in = vec_in && (uintptr_t)p.g[i] % (4 * sizeof(O)) == 0 && (uintptr_t)p.m[i] % 16 == 0;
+        vec_out = vec_out && (uintptr_t)p.out[i] % (4 * sizeof(O)) == 0;
     }
     Dims d{};
     d.rows = a.rows, d.cols = a.cols, d.ldg = a.ldg, d.ldo = a.ldo, d.ldm = a.ldm;
     d.tall = a.rows > a.cols;
-    d.m = d.tall ? a.cols : a.rows;
-    d.n = d.tall ? a.rows : a.cols;
-    d.mp = pad_to(d.m, T);
-    d.np = pad_to(d.n, T);
+    d.m = pl.m, d.n = pl.n, d.mp = pl.mp, d.np = pl.np;
+    const float mu = kMuon ? (float)a.opts->momentum : 0.f;
+    const int nesterov = kMuon ? a.opts->nesterov : 0;
+    FinalArgs g{};
+    g.ptrs = p, g.rows = d.rows, g.cols = d.cols, g.ldo = d.ldo, g.guard = a.guard;
+    g.decay = kMuon ? (float)(1.0 - a.opts->lr * a.opts->weight_decay) : 1.f;
+    g.step = kMuon ? (float)(a.opts->lr * a.opts->scale) : 1.f;
+    g.vec = vec_out;
+    if (pl.small) {
+        small_kernel<O, kMuon><<<dim3(a.count), kThreads, 0, s>>>(g, d, st, a.ns->eps, mu, nesterov);
+        return hipGetLastError();
+    }
     const long xb = d.mp * d.np * 4, ab = d.mp * d.mp * 4;
     double* part = (double*)a.ws;
     char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *A = xt2 + a.count * xb,
          *B = A + a.count * ab;
     float* factors = (float*)(B + a.count * ab);
-    double grow[CNF_NS_MAX_STEPS];
-    if (ns_bounds(*a.ns, grow)) return hipErrorInvalidValue;
-    Grow by{};
-    for (int k = 0; k < a.ns->steps; ++k) by.by[k] = (float)fmax(1., grow[k]);
-    const float mu = kMuon ? (float)a.opts->momentum : 0.f;
-    const int nesterov = kMuon ? a.opts->nesterov : 0;
-    begin_kernel<O, kMuon><<<dim3(kNormBlocks, a.count), kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
+    // partial sums: enough workgroups for the device, at least 8 K elements each
+    long parts = (d.rows * d.cols + 8191) / 8192, most = (2048 + a.count - 1) / a.count;
+    most = most < kNormBlocks ? most : kNormBlocks;
+    parts = parts < most ? parts : most;
+    const dim3 grid_in((unsigned)parts, a.count);
+    if (vec_in)
+        begin_kernel<O, kMuon, true><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
+    else
+        begin_kernel<O, kMuon, false><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
     const long rp = d.tall ? d.np : d.mp, cp = d.tall ? d.mp : d.np;
-    pieces_kernel<O, kMuon><<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), a.count), kThreads, 0, s>>>(p, d, x, xt, part, a.ns->eps, mu, nesterov,
-                                                                                                              by, factors);
-    const int tm = (int)(d.mp / T), tn = (int)(d.np / T), km = (int)(d.mp / 32), kn = (int)(d.np / 32);
-    for (int k = 0; k < a.ns->steps; ++k) {
-        FinalArgs g{};
-        g.p = g.q = x, g.bp = g.bq = xb, g.kc = kn, g.tiles_r = g.tiles_c = tm;
-        g.c0 = A, g.b0 = ab, g.kc0 = km;
+    pieces_kernel<O, kMuon><<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), a.count), kThreads, 0, s>>>(p, d, x, xt, part, (int)parts, a.ns->eps,
+                                                                                                         mu, nesterov, st, factors);
+    const int km = (int)(d.mp / 32), kn = (int)(d.np / 32);
+    for (int k = 0; k < st.n; ++k) {
         g.factors = factors + k;
-        const dim3 sym(tm * (tm + 1) / 2, a.count);
-        gemm_kernel<T, kGram><<<sym, kThreads, 0, s>>>(g);
+        g.p = g.q = x, g.bp = g.bq = xb, g.kc = kn;
+        g.c0 = A, g.b0 = ab, g.kc0 = km;
+        product<kGram>(pl.wide_sym, g, pl, false, a.count, s);
         g.p = g.q = A, g.bp = g.bq = ab, g.kc = km;
         g.c0 = B;
-        g.ca = (float)a.ns->a[k], g.cb = (float)a.ns->b[k], g.cc = (float)a.ns->c[k], g.m = d.m;
-        gemm_kernel<T, kPoly><<<sym, kThreads, 0, s>>>(g);
-        const bool last = k + 1 == a.ns->steps;
-        g.p = B, g.bp = ab, g.q = xt, g.bq = xb, g.tiles_r = tm, g.tiles_c = tn;
-        if (!last) {
+        g.ca = st.a[k], g.cb = st.b[k], g.cc = st.c[k], g.m = d.m;
+        product<kPoly>(pl.wide_sym, g, pl, false, a.count, s);
+        g.p = B, g.bp = ab, g.q = xt, g.bq = xb;
+        if (k + 1 < st.n) {
             g.c0 = x, g.b0 = xb, g.kc0 = kn;
             g.c1 = xt2, g.b1 = xb, g.kc1 = km;
-            gemm_kernel<T, kApply><<<dim3(tm * tn, a.count), kThreads, 0, s>>>(g);
+            product<kApply>(pl.wide_full, g, pl, false, a.count, s);
             char* t = xt;
             xt = xt2;
             xt2 = t;
             continue;
         }
-        if (d.tall) {      // the output's rows are X^T's
-            g.p = xt, g.bp = xb, g.q = B, g.bq = ab, g.tiles_r = tn, g.tiles_c = tm;
-        }
-        g.ptrs = p, g.rows = d.rows, g.cols = d.cols, g.ldo = d.ldo, g.guard = a.guard;
-        g.decay = kMuon ? (float)(1.0 - a.opts->lr * a.opts->weight_decay) : 1.f;
-        g.step = kMuon ? (float)(a.opts->lr * a.opts->scale) : 1.f;
-        g.vec = d.ldo % 4 == 0;
-        for (int i = 0; i < a.count; ++i) g.vec = g.vec && (uintptr_t)p.out[i] % (4 * sizeof(O)) == 0;
-        gemm_kernel<T, kFinal, O, kMuon><<<dim3(tm * tn, a.count), kThreads, 0, s>>>(g);
+        if (d.tall) g.p = xt, g.bp = xb, g.q = B, g.bq = ab;   // the output's rows are X^T's
+        product<kFinal, O, kMuon>(pl.wide_full, g, pl, d.tall, a.count, s);
     }
     return hipGetLastError();
 }
 
 template <typename O>
 hipError_t run_op(const MuonArgs& a, hipStream_t s) {
-    if (tile_of(a.count, a.rows, a.cols) == 128) return a.opts ? run<128, O, true>(a, s) : run<128, O, false>(a, s);
-    return a.opts ? run<64, O, true>(a, s) : run<64, O, false>(a, s);
+    return a.opts ? run<O, true>(a, s) : run<O, false>(a, s);
 }
 
 }  // namespace
@@ -418,8 +629,9 @@ int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
 }
 
 size_t muon_workspace_bytes(long count, long rows, long cols) {
-    const int t = tile_of(count, rows, cols);
-    const size_t m = pad_to(rows < cols ? rows : cols, t), n = pad_to(rows < cols ? cols : rows, t);
+    const Plan p = plan_of(count, rows, cols);
+    const size_t m = p.mp, n = p.np;
+    if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)
     return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + 2 * m * m) * 4 + CNF_NS_MAX_STEPS * sizeof(float));
 }
 
