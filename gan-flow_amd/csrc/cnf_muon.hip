@@ -18,7 +18,8 @@
 //
 // LAYOUT ("piece matrix").  R x K, padded with zeros to multiples of 64 and stored in blocks of 64 rows x 32 columns, 8 KB
 // each, block (r / 64, k / 32) after block along k.  A row of a block is one 128-byte line: four 16-byte slots of hi, four of lo, slot s
-// at s ^ (row & 7), so that a block copied to LDS as it lies is read by MFMA operands without bank conflicts.
+// at s ^ (row / 2 & 7): a block copied to LDS as it lies is read as MFMA operands (a 16-byte slot of 16 rows per cycle, two rows
+// to a line of the 64 banks) without bank conflicts.
 // Every product is of the form C[r][c] = sum_k P[r][k] Q[c][k] with both operands contiguous along k: A = X X^T, A A (A is
 // symmetric) and X' = (a I + b A + c A^2) X with Q = X^T, which the step that makes X writes beside it.  A and A^2 are symmetric: only
 // tiles on and below the diagonal are computed, and written twice.
@@ -54,7 +55,7 @@ struct Dims {
 
 // byte offset of element (r, c)'s hi piece in a piece matrix of kc blocks per row panel; its lo piece is at this ^ 64
 __device__ __forceinline__ long piece_at(long r, long c, long kc) {
-    return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ (r & 7)) << 4) + ((c & 7) << 1);
+    return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ ((r >> 1) & 7)) << 4) + ((c & 7) << 1);
 }
 
 __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
@@ -236,11 +237,10 @@ using lptr = __attribute__((address_space(3))) void*;
 
 // One T x T tile of C per workgroup of four waves (2 x 2), each a (T/2) x (T/2) square of 32 x 32 MFMA tiles.  A stage is one block column (32 k) of
 // both operands, copied to LDS by global_load_lds kStages - 1 stages ahead of the products.
-template <int T, int kMode, typename O = float, bool kMuon = false>
+template <int T, int kStages, int kMode, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
     constexpr int kStage = 2 * T * 128, kN = T / 64;         // bytes of a stage; 32 x 32 tiles per wave and direction
     constexpr int kLoads = kStage / 1024 / 4;                // 1 KB copies per wave and stage
-    constexpr int kStages = T == 64 ? 4 : 2;                 // 64 KB either way: two workgroups per CU
     __shared__ __align__(16) char lds[kStages][kStage];
     const int mat = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     int ti, tj;
@@ -267,7 +267,7 @@ __global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
             __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes), (lptr)(&lds[stage][(wave * kLoads + i) * 1024]), 16, 0, 0);
     };
     const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
-    const int slot = ((lane >> 5) ^ (lane & 7)) << 4, line = (lane & 31) << 7;
+    const int slot = ((lane >> 5) ^ ((lane >> 1) & 7)) << 4, line = (lane & 31) << 7;
     float16v acc[kN][kN] = {};
     for (int k = 0; k < kStages - 1 && k < a.kc; ++k) load(k, k);
     for (int k = 0; k < a.kc; ++k) {
@@ -357,28 +357,28 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
     const int mat = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const bool skip = a.guard && a.guard->status != 0;
     const O* g = (const O*)a.ptrs.g[mat];
-    // the matrix: thread (tr, tc) holds four rows of four columns
+    // the matrix: thread (tr, tc) holds four rows of four columns (what lies outside is read at the last element and not used)
     const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
-    float v[4][4];
-    double s = 0.;
-    for (int i = 0; i < 4; ++i) {
-        const int r = tr * 4 + i;
+    float v[4][4], old[4][4];
+    for (int i = 0; i < 4; ++i)
         for (int k = 0; k < 4; ++k) {
-            const int c = tc + k;
-            float u = 0.f;
-            if (r < a.rows && c < a.cols) {
-                u = to_f32(g[r * d.ldg + c]);
-                if (kMuon) {
-                    float* pm = a.ptrs.m[mat] + r * d.ldm + c;
-                    const float mv = fmaf(mu, *pm, u);
-                    if (!skip) *pm = mv;
-                    u = nesterov ? fmaf(mu, mv, u) : mv;
-                }
-            }
-            v[i][k] = u;
-            s = fma((double)u, (double)u, s);
+            const int r = min(tr * 4 + i, (int)a.rows - 1), c = min(tc + k, (int)a.cols - 1);
+            v[i][k] = to_f32(g[r * d.ldg + c]);
+            if (kMuon) old[i][k] = a.ptrs.m[mat][r * d.ldm + c];
         }
-    }
+    double s = 0.;
+    for (int i = 0; i < 4; ++i)
+        for (int k = 0; k < 4; ++k) {
+            const int r = tr * 4 + i, c = tc + k;
+            const bool in = r < a.rows && c < a.cols;
+            if (kMuon) {
+                const float mv = fmaf(mu, old[i][k], v[i][k]);
+                if (in && !skip) a.ptrs.m[mat][r * d.ldm + c] = mv;
+                v[i][k] = nesterov ? fmaf(mu, mv, v[i][k]) : mv;
+            }
+            if (!in) v[i][k] = 0.f;
+            s = fma((double)v[i][k], (double)v[i][k], s);
+        }
     for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
     if (lane == 0) red[wave] = s;
     __syncthreads();
@@ -403,7 +403,7 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
         *(half4*)(flipped + (att ^ 64)) = lt;
     }
     const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-    const int slot = ((lane >> 5) ^ (lane & 7)) << 4, line = (lane & 31) << 7;
+    const int slot = ((lane >> 5) ^ ((lane >> 1) & 7)) << 4, line = (lane & 31) << 7;
     // quadrant (pr, qr) of sum_k P[r][k] Q[c][k]: a lane holds columns 8 g + 4 (lane / 32) + e of row lane % 32
     auto multiply = [&](const char* p, int pr, const char* q, int qr) {
         float16v acc = {};
@@ -446,9 +446,10 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
         store(as, nullptr, A);
         __syncthreads();
         float16v B = multiply(as, wr, as, wc);
+        const float diag = row < d.m ? st.a[k] * kScale : 0.f;
         for (int i = 0; i < 16; ++i) {
             B[i] = fmaf(st.c[k] * kInvScale, B[i], st.b[k] * A[i]);
-            if (row == col + (i >> 2) * 8 + (i & 3) && row < d.m) B[i] += st.a[k] * kScale;
+            B[i] += row == col + (i >> 2) * 8 + (i & 3) ? diag : 0.f;
         }
         store(bs, nullptr, B);
         __syncthreads();
@@ -474,7 +475,7 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
 long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 
 // The tile of a product of `tiles` 128 x 128 tiles: 128 reads its operands half as often, 64 has four times the workgroups.
-bool wide_tiles(long tiles) { return tiles >= 160; }
+bool wide_tiles(long tiles) { return tiles >= 128; }
 
 struct Plan {
     long m, n, mp, np;
@@ -504,10 +505,16 @@ void product(bool wide, const FinalArgs& args, const Plan& p, bool transposed, i
     g.tiles_r = transposed ? tn : tm;
     g.tiles_c = sym ? tm : transposed ? tm : tn;
     const dim3 grid(sym ? tm * (tm + 1) / 2 : tm * tn, count);
-    if (wide)
-        gemm_kernel<128, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+    // at most one workgroup per CU: 128 KB of stages in flight each, else 64 KB and two workgroups
+    const bool deep = (long)grid.x * grid.y <= 256;
+    if (wide && deep)
+        gemm_kernel<128, 4, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+    else if (wide)
+        gemm_kernel<128, 2, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+    else if (deep)
+        gemm_kernel<64, 8, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
     else
-        gemm_kernel<64, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+        gemm_kernel<64, 4, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
 }
 
 template <typename O, bool kMuon>
@@ -552,8 +559,8 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *A = xt2 + a.count * xb,
          *B = A + a.count * ab;
     float* factors = (float*)(B + a.count * ab);
-    // partial sums: enough workgroups for the device, at least 8 K elements each
-    long parts = (d.rows * d.cols + 8191) / 8192, most = (2048 + a.count - 1) / a.count;
+    // partial sums: enough workgroups for the device, at least 2 K elements each
+    long parts = (d.rows * d.cols + 2047) / 2048, most = (2048 + a.count - 1) / a.count;
     most = most < kNormBlocks ? most : kNormBlocks;
     parts = parts < most ? parts : most;
     const dim3 grid_in((unsigned)parts, a.count);
