@@ -25,6 +25,7 @@
 // tiles on and below the diagonal are computed, and written twice.
 #include <cmath>
 #include <type_traits>
+#include <utility>
 
 #include "cnf_ops.h"
 
@@ -58,7 +59,11 @@ __device__ __forceinline__ long piece_at(long r, long c, long kc) {
     return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ ((r >> 1) & 7)) << 4) + ((c & 7) << 1);
 }
 
+// The value is settled before it is split: the compiler otherwise folds the operation that makes v into one of the two conversions
+// (fp32 arithmetic with an fp16 result, rounded once), and a hi from the unrounded value beside a lo from the rounded one is a
+// whole fp16 step off where the two round differently.
 __device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
+    asm("" : "+v"(v));
     hi = (f16)v;
     lo = (f16)(v - (float)hi);
 }
@@ -145,9 +150,9 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
             float f;
             scale = start_scale(sqrt(s), eps, f);
             if (blockIdx.x == 0 && blockIdx.y == 0) {
-                for (int k = 0; k < CNF_NS_MAX_STEPS; ++k) {
-                    factors[mat * CNF_NS_MAX_STEPS + k] = f;
-                    f = fminf(1.f, f * st.grow[k]);
+                for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
+                    factors[mat * (CNF_NS_MAX_STEPS + 1) + k] = f;
+                    if (k < st.n) f = fminf(1.f, f * st.grow[k]);
                 }
             }
         }
@@ -190,20 +195,20 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
     }
 }
 
-constexpr int kGram = 0, kPoly = 1, kApply = 2, kFinal = 3;
+constexpr int kGram = 0, kPoly = 1, kSym = 2, kApply = 3, kFinal = 4;
 
 struct GemmArgs {
     const char *p, *q;          // piece matrices; C[r][c] = sum_k P[r][k] Q[c][k]
     long bp, bq;                // bytes between matrices of the batch
-    int kc;                     // blocks of 32 along k
-    int tiles_r, tiles_c;       // tiles of C (kGram, kPoly: tiles_r x tiles_r symmetric)
-    // kGram, kPoly: C to `c0` (symmetric); kApply: C to c0 and its transpose to c1
+    int kc;                     // blocks of 32 along k (even)
+    int panels_p, panels_q;     // panels of 64 rows of P and Q
+    // kGram, kPoly, kSym: C to `c0` (symmetric); kApply: C to c0 and its transpose to c1
     char *c0, *c1;
     long b0, b1;
-    int kc0, kc1;
     float ca, cb, cc;           // kPoly: a I + b P + c C
     long m;                     // kPoly: rows of the identity
-    const float* factors;       // of this step; the next one's follow
+    const float* factors;       // kGram, kApply, kFinal: s at this step; `ahead` further on: after the steps the product stands for
+    int ahead;
 };
 
 struct FinalArgs : GemmArgs {   // kFinal: the iteration's result to the output matrices, or into the parameters
@@ -216,6 +221,8 @@ struct FinalArgs : GemmArgs {   // kFinal: the iteration's result to the output 
 
 template <int kMode>
 using ArgsOf = std::conditional_t<kMode == kFinal, FinalArgs, GemmArgs>;
+template <int kMode>
+constexpr bool kSymmetric = kMode == kGram || kMode == kPoly || kMode == kSym;
 
 // four neighbouring elements of a row of the result to the output matrix, or into the parameters
 template <typename O, bool kMuon>
@@ -235,116 +242,288 @@ __device__ __forceinline__ void put4(const FinalArgs& a, int mat, long r, long c
 using gptr = const __attribute__((address_space(1))) void*;
 using lptr = __attribute__((address_space(3))) void*;
 
-// One T x T tile of C per workgroup of four waves (2 x 2), each a (T/2) x (T/2) square of 32 x 32 MFMA tiles.  A stage is one block column (32 k) of
-// both operands, copied to LDS by global_load_lds kStages - 1 stages ahead of the products.
-template <int T, int kStages, int kMode, typename O = float, bool kMuon = false>
-__global__ __launch_bounds__(kThreads) void gemm_kernel(ArgsOf<kMode> a) {
-    constexpr int kStage = 2 * T * 128, kN = T / 64;         // bytes of a stage; 32 x 32 tiles per wave and direction
-    constexpr int kLoads = kStage / 1024 / 4;                // 1 KB copies per wave and stage
-    __shared__ __align__(16) char lds[kStages][kStage];
-    const int mat = blockIdx.y, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    int ti, tj;
-    if (kMode == kGram || kMode == kPoly) {                  // tile (ti, tj), tj <= ti, of the lower triangle
-        const int id = blockIdx.x;
-        ti = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
-        while ((ti + 1) * (ti + 2) / 2 <= id) ++ti;
-        while (ti * (ti + 1) / 2 > id) --ti;
-        tj = id - ti * (ti + 1) / 2;
+// Which tile a workgroup computes.  Consecutive workgroups go to the eight XCDs in turn, each with an L2 of its own: an XCD gets
+// a contiguous run of the tiles -- matrix after matrix, each in bands of eight tile rows, a band column after column -- so that the
+// workgroups that share an L2 share operand panels.  With tiles dealt out in turn instead every L2 streams nearly all of X, and the fabric
+// behind the L2s bounds the products (Muon 8 x (1024 x 512): 26 against 19 us a Gram product); so it does where the lower triangle is
+// taken row after row (4096 x 4096: 345 against 235 us).
+__device__ __forceinline__ int triangle_row(int id) {        // the row of element `id` of a lower triangle stored row after row
+    int r = (int)((sqrtf(8.f * (float)id + 1.f) - 1.f) * 0.5f);
+    while ((r + 1) * (r + 2) / 2 <= id) ++r;
+    while (r * (r + 1) / 2 > id) --r;
+    return r;
+}
+
+__device__ __forceinline__ void my_tile(int tiles_r, int tiles_c, bool sym, int& mat, int& ti, int& tj) {
+    constexpr int kBand = 8;
+    const int total = gridDim.x, q = total >> 3, rem = total & 7, xcd = blockIdx.x & 7, nth = blockIdx.x >> 3;
+    int id = xcd * q + (xcd < rem ? xcd : rem) + nth;
+    const int per = sym ? tiles_r * (tiles_r + 1) / 2 : tiles_r * tiles_c;
+    mat = id / per;
+    id -= mat * per;
+    if (sym) {                                               // tj <= ti: a band's columns before its diagonal, then the triangle on it
+        const int first = triangle_row(id) / kBand * kBand, high = min(kBand, tiles_r - first);
+        id -= first * (first + 1) / 2;
+        if (id < first * high) {
+            ti = first + id % high;
+            tj = id / high;
+        } else {
+            id -= first * high;
+            ti = triangle_row(id);
+            tj = first + id - ti * (ti + 1) / 2;
+            ti += first;
+        }
     } else {
-        ti = blockIdx.x % a.tiles_r;
-        tj = blockIdx.x / a.tiles_r;
+        const int band = id / (kBand * tiles_c), first = band * kBand, high = min(kBand, tiles_r - first);
+        id -= first * tiles_c;
+        ti = first + id % high;
+        tj = id / high;
     }
+}
+
+// Operands of the products of 16 k: kNu x kNv tiles of 32 x 32 from a block column of P and of Q in LDS
+template <int kNu, int kNv>
+struct Frag {
+    half8 ph[kNu], pl[kNu], qh[kNv], ql[kNv];
+    // p, q: the wave's first rows of the two blocks; h: which 16 of the 32 k
+    __device__ __forceinline__ void read(const char* p, const char* q, int lane, int h) {
+        const int at = ((lane & 31) << 7) + ((((lane >> 5) ^ ((lane >> 1) & 7)) << 4) ^ (h << 5));
+        for (int v = 0; v < kNv; ++v) {
+            ql[v] = *(const half8*)(q + v * 32 * 128 + (at ^ 64));
+            qh[v] = *(const half8*)(q + v * 32 * 128 + at);
+        }
+        for (int u = 0; u < kNu; ++u) {
+            ph[u] = *(const half8*)(p + u * 32 * 128 + at);
+            pl[u] = *(const half8*)(p + u * 32 * 128 + (at ^ 64));
+        }
+    }
+    // operands exchanged: a lane gets four neighbouring columns of a row of C
+    __device__ __forceinline__ void multiply(float16v (&acc)[kNu][kNv]) const {
+        for (int u = 0; u < kNu; ++u)
+            for (int v = 0; v < kNv; ++v) {
+                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
+                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
+                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
+            }
+    }
+};
+
+// What happens to a 32 x 32 tile of C whose first element is (r0, c0): lane l holds columns 8 g + 4 (l / 32) + e (register 4 g + e) of
+// row l % 32.  A row of the tile is one line of a piece matrix; the two lanes of a row exchange halves (hi of both to the first,
+// lo of both to the second) and store whole 16-byte slots.  A transposed copy goes through LDS (4.6 KB a wave, (hi, lo) as a word).
+constexpr int kFlipBytes = 32 * 36 * 4;
+
+template <int kMode, typename O, bool kMuon>
+__device__ __forceinline__ void finish(const ArgsOf<kMode>& a, int mat, float scale, const float16v& acc, long r0, long c0, bool flip, int lane,
+                                       char* lds) {
+    if (r0 >= (long)a.panels_p * 64 || c0 >= (long)a.panels_q * 64) return;     // (a tile larger than 64 can reach past the end)
+    const int row = lane & 31, half = lane >> 5;
+    const long r = r0 + row;
+    const long kc0 = a.panels_q * 2;
+    const long line = piece_at(r, c0, kc0) & ~127l, sw = ((r >> 1) & 7) << 4;
+    if constexpr (kMode == kFinal) {
+        if (r < a.rows)
+            for (int g = 0; g < 4; ++g) {
+                float val[4];
+                for (int e = 0; e < 4; ++e) val[e] = acc[g * 4 + e] * scale;
+                const long c = c0 + g * 8 + half * 4;
+                if (c < a.cols) put4<O, kMuon>(a, mat, r, c, val);
+            }
+    } else {
+        char* to = a.c0 + mat * a.b0 + line;
+        unsigned word[16];                                   // (hi, lo)
+        for (int g = 0; g < 4; ++g) {
+            float val[4];
+            for (int e = 0; e < 4; ++e) val[e] = acc[g * 4 + e] * scale;
+            if (kMode == kPoly) {
+                const char* pm = a.p + mat * a.bp + line + half * 8;
+                const half4 h = *(const half4*)(pm + ((g << 4) ^ sw)), l = *(const half4*)(pm + ((g << 4) ^ sw ^ 64));
+                const int on = (int)(r - (c0 + g * 8 + half * 4));              // which of the four is on the diagonal
+                for (int e = 0; e < 4; ++e) {
+                    val[e] = fmaf(a.cc, val[e], a.cb * ((float)h[e] + (float)l[e]));
+                    val[e] += e == on && r < a.m ? a.ca * kScale : 0.f;
+                }
+            }
+            union { f16 e[4]; unsigned w[2]; } hi, lo;
+            for (int e = 0; e < 4; ++e) {
+                split(val[e], hi.e[e], lo.e[e]);
+                union { f16 e[2]; unsigned w; } both;
+                both.e[0] = hi.e[e], both.e[1] = lo.e[e];
+                word[g * 4 + e] = both.w;
+            }
+            uint4 slot;                                      // the first lane of a row: hi of both halves; the second: lo
+            const auto x = __builtin_amdgcn_permlane32_swap(hi.w[0], lo.w[0], false, false);
+            const auto y = __builtin_amdgcn_permlane32_swap(hi.w[1], lo.w[1], false, false);
+            slot.x = x[0], slot.y = y[0], slot.z = x[1], slot.w = y[1];
+            *(uint4*)(to + ((g << 4) ^ sw ^ (half << 6))) = slot;
+        }
+        if (flip) {
+            unsigned* t = (unsigned*)lds;
+            for (int g = 0; g < 4; ++g) *(uint4*)(t + row * 36 + g * 8 + half * 4) = make_uint4(word[g * 4], word[g * 4 + 1], word[g * 4 + 2], word[g * 4 + 3]);
+            // (a wave's LDS operations are executed in order: the reads see the writes)
+            const long c = c0 + row;                         // this lane's row of the transpose, k = 16 half ..
+            const long kc1 = a.panels_p * 2;
+            char* tc = (kMode == kApply ? a.c1 + mat * a.b1 : a.c0 + mat * a.b0) + (piece_at(c, r0, kMode == kApply ? kc1 : kc0) & ~127l);
+            const long tw = ((c >> 1) & 7) << 4;
+            for (int g = 0; g < 2; ++g) {
+                unsigned w[8];
+                for (int i = 0; i < 8; ++i) w[i] = t[(half * 16 + g * 8 + i) * 36 + row];
+                uint4 h, l;
+                h.x = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u), l.x = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
+                h.y = __builtin_amdgcn_perm(w[3], w[2], 0x05040100u), l.y = __builtin_amdgcn_perm(w[3], w[2], 0x07060302u);
+                h.z = __builtin_amdgcn_perm(w[5], w[4], 0x05040100u), l.z = __builtin_amdgcn_perm(w[5], w[4], 0x07060302u);
+                h.w = __builtin_amdgcn_perm(w[7], w[6], 0x05040100u), l.w = __builtin_amdgcn_perm(w[7], w[6], 0x07060302u);
+                const long at = ((half * 2 + g) << 4) ^ tw;
+                *(uint4*)(tc + at) = h;
+                *(uint4*)(tc + (at ^ 64)) = l;
+            }
+        }
+    }
+}
+
+// from the accumulator to C times 2^10 (kFinal: to C)
+template <int kMode>
+__device__ __forceinline__ float scale_of(const ArgsOf<kMode>& a, int mat) {
+    if (kMode == kPoly || kMode == kSym) return kInvScale;
+    const float* f = a.factors + mat * (CNF_NS_MAX_STEPS + 1);
+    return kInvScale * (kMode == kGram ? f[0] * f[0] : kMode == kApply ? f[0] / f[a.ahead] : f[0] * kInvScale);
+}
+
+// 64 x 64 tiles.  Each of kW waves computes the whole tile over every kW-th block of k -- a wave copies its own operands to its own part of
+// LDS, so nothing but its own counters holds it up -- and the partial sums are added at the end, in a fixed order.
+template <int kW, int kMode, typename O = float, bool kMuon = false>
+__global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
+    constexpr int kStages = 2, kStage = 2 * 64 * 128, kLoads = kStage / 1024;
+    __shared__ __align__(16) char lds[kW][kStages][kStage];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int mat, ti, tj;
+    my_tile(a.panels_p, a.panels_q, kSymmetric<kMode>, mat, ti, tj);
+    const char* ps = a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes + lane * 16;
+    const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes + lane * 16;
+    const int stages = (a.kc - wave + kW - 1) / kW;          // of this wave: blocks wave, wave + kW, ..
+    auto load = [&](int s) {
+        const long off = (long)(s * kW + wave) * kBlockBytes;
+        for (int i = 0; i < kLoads / 2; ++i) {
+            __builtin_amdgcn_global_load_lds((gptr)(ps + off + i * 1024), (lptr)(&lds[wave][s % kStages][i * 1024]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)(qs + off + i * 1024), (lptr)(&lds[wave][s % kStages][8192 + i * 1024]), 16, 0, 0);
+        }
+    };
+    float16v acc[2][2] = {};
+    for (int s = 0; s < kStages && s < stages; ++s) load(s);
+    for (int s = 0; s < stages; ++s) {
+        if (s + kStages <= stages)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+        else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const char* st = lds[wave][s % kStages];
+        Frag<2, 2> f0, f1;
+        f0.read(st, st + 8192, lane, 0);
+        f1.read(st, st + 8192, lane, 1);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read: the next copy may take its place
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + kStages < stages) load(s + kStages);
+        f0.multiply(acc);
+        f1.multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if constexpr (kMode == kFinal) {
+        if (a.guard && a.guard->status != 0) return;
+    }
+    const float scale = scale_of<kMode>(a, mat);
+    const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
+    if constexpr (kW == 1) {
+        for (int u = 0; u < 2; ++u)
+            for (int v = 0; v < 2; ++v) finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], ti * 64l + u * 32, tj * 64l + v * 32, flip, lane, lds[0][0]);
+    } else if constexpr (kW == 2) {                          // a wave finishes a row of quadrants
+        __syncthreads();
+        float* sums = (float*)&lds[0][0][0];                 // [register][wave][lane], 16 KB
+        for (int i = 0; i < 32; ++i) sums[(i * 2 + wave) * 64 + lane] = wave == 0 ? acc[1][i >> 4][i & 15] : acc[0][i >> 4][i & 15];
+        __syncthreads();
+        for (int v = 0; v < 2; ++v) {
+            float16v mine = wave == 0 ? acc[0][v] : acc[1][v];
+            for (int i = 0; i < 16; ++i) mine[i] += sums[((v * 16 + i) * 2 + (wave ^ 1)) * 64 + lane];
+            finish<kMode, O, kMuon>(a, mat, scale, mine, ti * 64l + wave * 32, tj * 64l + v * 32, flip, lane, &lds[1][0][0] + wave * kFlipBytes);
+        }
+    } else {
+        static_assert(kW == 4, "a wave per quadrant");
+        __syncthreads();
+        float* sums = (float*)&lds[0][0][0];                 // [quadrant][register][wave][lane]
+        for (int t = 0; t < 4; ++t)
+            if (t != wave)
+                for (int i = 0; i < 16; ++i) sums[((t * 16 + i) * 4 + wave) * 64 + lane] = acc[t >> 1][t & 1][i];
+        __syncthreads();
+        float16v mine = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1];
+        for (int w = 0; w < 4; ++w)
+            if (w != wave)
+                for (int i = 0; i < 16; ++i) mine[i] += sums[((wave * 16 + i) * 4 + w) * 64 + lane];
+        // (the transposition's LDS lies behind the sums' 64 KB, which other waves may still read)
+        finish<kMode, O, kMuon>(a, mat, scale, mine, ti * 64l + (wave >> 1) * 32, tj * 64l + (wave & 1) * 32, flip, lane, &lds[2][0][0] + wave * kFlipBytes);
+    }
+}
+
+// T x T tiles for larger products: waves of kNu x kNv MFMA tiles share kStages stages of one block column each.  The operands of each 16 k are
+// read while the products of the 16 before are computed, and the stage's one barrier falls between the two halves, with products on
+// either side.  4096 x 4096 x 4096 with T = 256: 336 us (1.23 PFLOP/s of piece products), against 374 with reads and products in turn; the
+// products alone, on operands that stay in registers, take 252 us: the device's power limit (177 with zeros for operands).
+template <int T, int kNu, int kNv, int kStages, int kMode, typename O = float, bool kMuon = false>
+__global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_kernel(ArgsOf<kMode> a) {
+    constexpr int kAcross = T / 32 / kNv, kW = T / 32 / kNu * kAcross, kStage = 2 * T * 128, kLoads = kStage / 1024 / kW;
+    static_assert(kW * kFlipBytes <= kStage && kLoads * kW * 1024 == kStage, "");
+    __shared__ __align__(16) char lds[kStages][kStage];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    int mat, ti, tj;
+    my_tile((a.panels_p + T / 64 - 1) / (T / 64), (a.panels_q + T / 64 - 1) / (T / 64), kSymmetric<kMode>, mat, ti, tj);
     const char* src[kLoads];
     for (int i = 0; i < kLoads; ++i) {
-        const int kb = wave * kLoads + i;                    // which KB of the stage: T / 8 of them are P's
-        const int row = (kb % (T / 8)) * 8;                  // first of its eight rows
+        const int kb = wave * kLoads + i, row = (kb % (T / 8)) * 8;             // KB of the stage: P's rows by eight, then Q's
         const bool is_p = kb < T / 8;
-        const long panel = (long)(is_p ? ti : tj) * (T / 64) + (row >> 6);
-        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + panel * a.kc * kBlockBytes + (row & 63) * 128 + lane * 16;
+        const int panel = min((is_p ? ti : tj) * (T / 64) + (row >> 6), (is_p ? a.panels_p : a.panels_q) - 1);   // (past the end: the last one again)
+        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + (long)panel * a.kc * kBlockBytes + (row & 63) * 128 + lane * 16;
     }
-    auto load = [&](int stage, int k) {
+    auto load = [&](int k) {
         for (int i = 0; i < kLoads; ++i)
-            __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes), (lptr)(&lds[stage][(wave * kLoads + i) * 1024]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes), (lptr)(&lds[k % kStages][(wave * kLoads + i) * 1024]), 16, 0, 0);
     };
-    const int wr = (wave >> 1) * (T / 2), wc = (wave & 1) * (T / 2);
-    const int slot = ((lane >> 5) ^ ((lane >> 1) & 7)) << 4, line = (lane & 31) << 7;
-    float16v acc[kN][kN] = {};
-    for (int k = 0; k < kStages - 1 && k < a.kc; ++k) load(k, k);
+    const int wr = (wave / kAcross) * kNu * 32, wc = (wave % kAcross) * kNv * 32;
+    float16v acc[kNu][kNv] = {};
+    Frag<kNu, kNv> f0, f1;
+    for (int k = 0; k < kStages && k < a.kc; ++k) load(k);
+    if (kStages <= a.kc)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    f0.read(lds[0] + wr * 128, lds[0] + (T + wc) * 128, lane, 0);
     for (int k = 0; k < a.kc; ++k) {
-        // this stage has landed (the kStages - 2 after it may be on their way), and every wave's reads of the one before are done
-        if (k + kStages - 1 <= a.kc)
+        f1.read(lds[k % kStages] + wr * 128, lds[k % kStages] + (T + wc) * 128, lane, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        f0.multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
+        // the next stage has landed (the kStages - 2 after it may be on their way), and every wave has read this one
+        if (k + kStages <= a.kc)
             asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + kStages - 1 < a.kc) load((k + kStages - 1) % kStages, k + kStages - 1);
-        const char* st = lds[k % kStages] + line;
-#pragma unroll
-        for (int kh = 0; kh < 2; ++kh) {
-            half8 ph[kN], pl[kN], qh[kN], ql[kN];
-            for (int u = 0; u < kN; ++u) {
-                const char* pr = st + (wr + u * 32) * 128;
-                const char* qr = st + (T + wc + u * 32) * 128;
-                ph[u] = *(const half8*)(pr + (slot ^ (kh << 5)));
-                pl[u] = *(const half8*)(pr + (slot ^ (kh << 5) ^ 64));
-                qh[u] = *(const half8*)(qr + (slot ^ (kh << 5)));
-                ql[u] = *(const half8*)(qr + (slot ^ (kh << 5) ^ 64));
-            }
-            for (int u = 0; u < kN; ++u)
-                for (int v = 0; v < kN; ++v) {               // operands exchanged: a lane holds four neighbouring columns of a row of C
-                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
-                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
-                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
-                }
-        }
+        if (k + kStages < a.kc) load(k + kStages);
+        const char* next = lds[(k + 1) % kStages];
+        if (k + 1 < a.kc) f0.read(next + wr * 128, next + (T + wc) * 128, lane, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        f1.multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (kMode == kFinal) {
         if (a.guard && a.guard->status != 0) return;
     }
-    float scale = kInvScale;                                 // from the accumulator to C times 2^10
-    if (kMode != kPoly) {
-        const float f = a.factors[mat * CNF_NS_MAX_STEPS];
-        scale *= kMode == kGram ? f * f : kMode == kApply ? f / a.factors[mat * CNF_NS_MAX_STEPS + 1] : f * kInvScale;
-    }
-    for (int u = 0; u < kN; ++u)
-        for (int v = 0; v < kN; ++v)
-            for (int g = 0; g < 4; ++g) {
-                const long r = (long)ti * T + wr + u * 32 + (lane & 31), c = (long)tj * T + wc + v * 32 + g * 8 + (lane >> 5) * 4;
-                float val[4];
-                for (int e = 0; e < 4; ++e) val[e] = acc[u][v][g * 4 + e] * scale;
-                if constexpr (kMode == kFinal) {
-                    if (r < a.rows) put4<O, kMuon>(a, mat, r, c, val);
-                } else {
-                const long at = piece_at(r, c, a.kc0);
-                if (kMode == kPoly) {
-                    const char* pm = a.p + mat * a.bp;
-                    const half4 h = *(const half4*)(pm + at), l = *(const half4*)(pm + (at ^ 64));
-                    for (int e = 0; e < 4; ++e) {
-                        val[e] = fmaf(a.cc, val[e], a.cb * ((float)h[e] + (float)l[e]));
-                        if (r == c + e && r < a.m) val[e] += a.ca * kScale;
-                    }
-                }
-                half4 hi, lo;
-                for (int e = 0; e < 4; ++e) {
-                    f16 h, l;
-                    split(val[e], h, l);
-                    hi[e] = h;
-                    lo[e] = l;
-                }
-                char* c0 = a.c0 + mat * a.b0;
-                *(half4*)(c0 + at) = hi;
-                *(half4*)(c0 + (at ^ 64)) = lo;
-                if (kMode == kApply || ti != tj) {
-                    char* ct = kMode == kApply ? a.c1 + mat * a.b1 : c0;
-                    for (int e = 0; e < 4; ++e) {
-                        const long t = piece_at(c + e, r, kMode == kApply ? a.kc1 : a.kc0);
-                        *(f16*)(ct + t) = hi[e];
-                        *(f16*)(ct + (t ^ 64)) = lo[e];
-                    }
-                }
-                }
-            }
+    const float scale = scale_of<kMode>(a, mat);
+    const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
+    __syncthreads();
+    for (int u = 0; u < kNu; ++u)
+        for (int v = 0; v < kNv; ++v)
+            finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], (long)ti * T + wr + u * 32, (long)tj * T + wc + v * 32, flip, lane,
+                                    lds[0] + wave * kFlipBytes);
 }
 
 // Matrices of at most 64 x 64: one workgroup per matrix does the whole update, with X, X^T, A and a I + b A + c A^2 as piece matrices in LDS
@@ -474,47 +653,68 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
 
 long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 
-// The tile of a product of `tiles` 128 x 128 tiles: 128 reads its operands half as often, 64 has four times the workgroups.
-bool wide_tiles(long tiles) { return tiles >= 128; }
-
 struct Plan {
-    long m, n, mp, np;
-    bool wide_sym, wide_full;
+    long m, n;      // the shorter and the longer side
+    int pm, pn;     // in panels of 64
     bool small;     // one workgroup per matrix does everything in LDS
+    bool together;  // products of several steps' polynomials before they meet X
 };
 
-Plan plan_of(long count, long rows, long cols) {
+Plan plan_of(long rows, long cols) {
     Plan p{};
     p.m = rows < cols ? rows : cols;
     p.n = rows < cols ? cols : rows;
     p.small = p.n <= 64;
-    const long t = pad_to(p.m, 128) / 128, u = pad_to(p.n, 128) / 128;
-    p.wide_sym = wide_tiles(t * (t + 1) / 2 * count);
-    p.wide_full = wide_tiles(t * u * count);
-    const long to = p.wide_sym || p.wide_full ? 128 : 64;
-    p.mp = pad_to(p.m, to);
-    p.np = pad_to(p.n, to);
+    p.pm = (int)((p.m + 63) / 64);
+    p.pn = (int)((p.n + 63) / 64);
+    p.together = p.pn >= 2 * p.pm;
     return p;
 }
 
+// Which kernel computes a product: the one whose time for k = 4096 is least, from the times measured for few and for as many workgroups as run
+// at once, us:            64 x 64, split k by 4: 26 .. 30 a round of 256      by 2: 45 .. 58 of 512       not split: 75 .. 102 of 1024
+//              128 x 128: 75 .. 101 of 256       192 x 192: 150 .. 216 of 256       256 x 256: 205 .. 336 of 256
+struct Choice {
+    int tile, split;
+};
+
+Choice choose(long count, int panels_p, int panels_q, bool sym) {
+    struct Entry {
+        int tile, split, at_once;
+        double few, full;
+    };
+    static constexpr Entry entries[] = {{64, 4, 256, 26, 30},     {64, 2, 512, 45, 58},     {64, 1, 1024, 75, 102},
+                                        {128, 1, 256, 75, 101},   {192, 1, 256, 150, 216},  {256, 1, 256, 205, 336}};
+    Choice best{};
+    double least = 1e300;
+    for (const Entry& e : entries) {
+        const int t = e.tile / 64;
+        const long r = (panels_p + t - 1) / t, c = (panels_q + t - 1) / t, tiles = count * (sym ? r * (r + 1) / 2 : r * c);
+        const long rounds = (tiles + e.at_once - 1) / e.at_once;
+        const double time = rounds * e.few + (e.full - e.few) * tiles / e.at_once;
+        if (time < least) least = time, best = {e.tile, e.split};
+    }
+    return best;
+}
+
 template <int kMode, typename O = float, bool kMuon = false>
-void product(bool wide, const FinalArgs& args, const Plan& p, bool transposed, int count, hipStream_t s) {
-    FinalArgs g = args;
-    const int t = wide ? 128 : 64, tm = (int)(p.mp / t), tn = (int)(p.np / t);
-    const bool sym = kMode == kGram || kMode == kPoly;
-    g.tiles_r = transposed ? tn : tm;
-    g.tiles_c = sym ? tm : transposed ? tm : tn;
-    const dim3 grid(sym ? tm * (tm + 1) / 2 : tm * tn, count);
-    // at most one workgroup per CU: 128 KB of stages in flight each, else 64 KB and two workgroups
-    const bool deep = (long)grid.x * grid.y <= 256;
-    if (wide && deep)
-        gemm_kernel<128, 4, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
-    else if (wide)
-        gemm_kernel<128, 2, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
-    else if (deep)
-        gemm_kernel<64, 8, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+void product(const FinalArgs& g, int count, hipStream_t s) {
+    const Choice how = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>);
+    const int t = how.tile / 64;
+    const long r = (g.panels_p + t - 1) / t, c = (g.panels_q + t - 1) / t;
+    const dim3 grid((unsigned)(count * (kSymmetric<kMode> ? r * (r + 1) / 2 : r * c)));
+    if (how.tile == 256)
+        tile_kernel<256, 4, 2, 2, kMode, O, kMuon><<<grid, 512, 0, s>>>(g);
+    else if (how.tile == 192)
+        tile_kernel<192, 3, 3, 3, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+    else if (how.tile == 128)
+        tile_kernel<128, 2, 2, 2, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+    else if (how.split == 4)
+        tile64_kernel<4, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+    else if (how.split == 2)
+        tile64_kernel<2, kMode, O, kMuon><<<grid, 128, 0, s>>>(g);
     else
-        gemm_kernel<64, 4, kMode, O, kMuon><<<grid, kThreads, 0, s>>>(g);
+        tile64_kernel<1, kMode, O, kMuon><<<grid, 64, 0, s>>>(g);
 }
 
 template <typename O, bool kMuon>
@@ -529,7 +729,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         st.c[k] = (float)a.ns->c[k];
         st.grow[k] = (float)fmax(1., grow[k]);
     }
-    const Plan pl = plan_of(a.count, a.rows, a.cols);
+    const Plan pl = plan_of(a.rows, a.cols);
     Ptrs p{};
     bool vec_in = a.cols % 4 == 0 && a.ldg % 4 == 0 && (!kMuon || a.ldm % 4 == 0), vec_out = a.ldo % 4 == 0;
     for (int i = 0; i < a.count; ++i) {
@@ -542,7 +742,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     Dims d{};
     d.rows = a.rows, d.cols = a.cols, d.ldg = a.ldg, d.ldo = a.ldo, d.ldm = a.ldm;
     d.tall = a.rows > a.cols;
-    d.m = pl.m, d.n = pl.n, d.mp = pl.mp, d.np = pl.np;
+    d.m = pl.m, d.n = pl.n, d.mp = pl.pm * 64l, d.np = pl.pn * 64l;
     const float mu = kMuon ? (float)a.opts->momentum : 0.f;
     const int nesterov = kMuon ? a.opts->nesterov : 0;
     FinalArgs g{};
@@ -556,9 +756,9 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     }
     const long xb = d.mp * d.np * 4, ab = d.mp * d.mp * 4;
     double* part = (double*)a.ws;
-    char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *A = xt2 + a.count * xb,
-         *B = A + a.count * ab;
-    float* factors = (float*)(B + a.count * ab);
+    char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *sym[5];
+    for (int i = 0; i < 5; ++i) sym[i] = xt2 + a.count * (xb + i * ab);
+    float* factors = (float*)(sym[pl.together ? 4 : 1] + a.count * ab);
     // partial sums: enough workgroups for the device, at least 2 K elements each
     long parts = (d.rows * d.cols + 2047) / 2048, most = (2048 + a.count - 1) / a.count;
     most = most < kNormBlocks ? most : kNormBlocks;
@@ -571,28 +771,72 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     const long rp = d.tall ? d.np : d.mp, cp = d.tall ? d.mp : d.np;
     pieces_kernel<O, kMuon><<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), a.count), kThreads, 0, s>>>(p, d, x, xt, part, (int)parts, a.ns->eps,
                                                                                                          mu, nesterov, st, factors);
-    const int km = (int)(d.mp / 32), kn = (int)(d.np / 32);
-    for (int k = 0; k < st.n; ++k) {
-        g.factors = factors + k;
-        g.p = g.q = x, g.bp = g.bq = xb, g.kc = kn;
-        g.c0 = A, g.b0 = ab, g.kc0 = km;
-        product<kGram>(pl.wide_sym, g, pl, false, a.count, s);
-        g.p = g.q = A, g.bp = g.bq = ab, g.kc = km;
-        g.c0 = B;
-        g.ca = st.a[k], g.cb = st.b[k], g.cc = st.c[k], g.m = d.m;
-        product<kPoly>(pl.wide_sym, g, pl, false, a.count, s);
-        g.p = B, g.bp = ab, g.q = xt, g.bq = xb;
-        if (k + 1 < st.n) {
-            g.c0 = x, g.b0 = xb, g.kc0 = kn;
-            g.c1 = xt2, g.b1 = xb, g.kc1 = km;
-            product<kApply>(pl.wide_full, g, pl, false, a.count, s);
+    const int km = pl.pm * 2, kn = pl.pn * 2;
+    // `Q` times X: the steps k .. k + n - 1, to X and X^T, or to the output
+    auto apply = [&](char* Q, int k, int n) {
+        g.factors = factors + k, g.ahead = n;
+        g.kc = km;
+        g.p = Q, g.bp = ab, g.panels_p = pl.pm;
+        g.q = xt, g.bq = xb, g.panels_q = pl.pn;
+        if (k + n < st.n) {
+            g.c0 = x, g.b0 = xb;
+            g.c1 = xt2, g.b1 = xb;
+            product<kApply>(g, a.count, s);
             char* t = xt;
             xt = xt2;
             xt2 = t;
-            continue;
+            return;
         }
-        if (d.tall) g.p = xt, g.bp = xb, g.q = B, g.bq = ab;   // the output's rows are X^T's
-        product<kFinal, O, kMuon>(pl.wide_full, g, pl, d.tall, a.count, s);
+        if (d.tall) {                                        // the output's rows are X^T's
+            g.p = xt, g.bp = xb, g.panels_p = pl.pn;
+            g.q = Q, g.bq = ab, g.panels_q = pl.pm;
+        }
+        product<kFinal, O, kMuon>(g, a.count, s);
+    };
+    auto symmetric = [&](auto mode, const char* p, const char* q, long bytes, int kc, char* to) {
+        g.p = p, g.q = q, g.bp = g.bq = bytes, g.kc = kc;
+        g.panels_p = g.panels_q = pl.pm;
+        g.c0 = to, g.b0 = ab;
+        product<decltype(mode)::value>(g, a.count, s);
+    };
+    auto gram = [&](int k, char* to) {
+        g.factors = factors + k;
+        symmetric(std::integral_constant<int, kGram>{}, x, x, xb, kn, to);
+    };
+    auto poly = [&](int k, const char* A, char* to) {
+        g.ca = st.a[k], g.cb = st.b[k], g.cc = st.c[k], g.m = d.m;
+        symmetric(std::integral_constant<int, kPoly>{}, A, A, ab, km, to);
+    };
+    auto times = [&](const char* p, const char* q, char* to) { symmetric(std::integral_constant<int, kSym>{}, p, q, ab, km, to); };
+    for (int k = 0; k < st.n;) {
+        // how many steps to take on the m x m side: see the head of this file
+        int n = 1;
+        float up = st.grow[k];
+        while (pl.together && n < 3 && k + n < st.n && up * up <= 256.f && up * st.grow[k + n] <= 48.f) up *= st.grow[k + n++];
+        char *A = sym[0], *B = sym[1], *Q = B;
+        gram(k, A);
+        poly(k, A, B);
+        char *A2 = sym[2], *T = sym[3], *Q2 = sym[4];
+        for (int i = 1; i < n; ++i) {
+            // A <- B A B, the next polynomial to the place of T, Q <- B Q
+            times(A, B, T);
+            times(T, B, A2);
+            std::swap(A, A2);
+            if (i == 1) {                                    // Q is B itself: the next B gets another place
+                poly(k + i, A, T);
+                B = T;
+                times(B, Q, Q2);
+                T = A2;                                      // (the old A)
+                A2 = Q;                                      // (the old B, after this product)
+                Q = Q2;
+            } else {
+                poly(k + i, A, T);
+                times(T, Q, A2);
+                Q = A2;
+            }
+        }
+        apply(Q, k, n);
+        k += n;
     }
     return hipGetLastError();
 }
@@ -636,10 +880,10 @@ int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
 }
 
 size_t muon_workspace_bytes(long count, long rows, long cols) {
-    const Plan p = plan_of(count, rows, cols);
-    const size_t m = p.mp, n = p.np;
+    const Plan p = plan_of(rows, cols);
     if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)
-    return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + 2 * m * m) * 4 + CNF_NS_MAX_STEPS * sizeof(float));
+    const size_t m = p.pm * 64, n = p.pn * 64;
+    return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + (p.together ? 5 : 2) * m * m) * 4 + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
 }
 
 hipError_t launch_muon(int dtype, const MuonArgs& a, hipStream_t s) {

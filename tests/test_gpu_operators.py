@@ -321,6 +321,17 @@ def test_orthogonalize(rows, cols, dtype):
     check_ns(orthogonalize(g), g)
 
 
+@pytest.mark.parametrize("count, rows, cols", [(40, 130, 260), (9, 700, 500), (3, 1290, 520), (4, 1990, 2100), (1, 2900, 2950), (1, 300, 9000)])
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: IDS[t])
+def test_orthogonalize_larger_launches(count, rows, cols, dtype):
+    """Enough work for every tile the products are built for, at sizes that fill none of them."""
+    from gan_flow_amd.lib.optim import orthogonalize
+    g = torch.randn(count, rows, cols, generator=torch.Generator().manual_seed(count)).to(DEV, dtype)
+    out = orthogonalize(g)
+    for i in sorted({0, count // 2, count - 1}):
+        check_ns(out[i], g[i], "matrix %d" % i)
+
+
 @pytest.mark.parametrize("rows, cols", [(64, 64), (33, 50), (200, 90), (320, 320)])
 def test_orthogonalize_batches_and_strides(rows, cols):
     from gan_flow_amd.lib.optim import orthogonalize
