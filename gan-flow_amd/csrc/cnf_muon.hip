@@ -239,6 +239,8 @@ __device__ __forceinline__ void put4(const FinalArgs& a, int mat, long r, long c
     }
 }
 
+constexpr int kSchedMfma = 0x8, kSchedVmem = 0x10, kSchedLdsRead = 0x100;   // classes of __builtin_amdgcn_sched_group_barrier
+
 using gptr = const __attribute__((address_space(1))) void*;
 using lptr = __attribute__((address_space(3))) void*;
 
@@ -299,12 +301,10 @@ struct Frag {
     }
     // operands exchanged: a lane gets four neighbouring columns of a row of C
     __device__ __forceinline__ void multiply(float16v (&acc)[kNu][kNv]) const {
-        for (int u = 0; u < kNu; ++u)
-            for (int v = 0; v < kNv; ++v) {
-                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql[v], ph[u], acc[u][v], 0, 0, 0);
-                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], pl[u], acc[u][v], 0, 0, 0);
-                acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh[v], ph[u], acc[u][v], 0, 0, 0);
-            }
+        for (int j = 0; j < 3; ++j)                          // lo hi, hi lo, hi hi: the three on one tile as far apart as they can be
+            for (int u = 0; u < kNu; ++u)
+                for (int v = 0; v < kNv; ++v)
+                    acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(j == 0 ? ql[v] : qh[v], j == 1 ? pl[u] : ph[u], acc[u][v], 0, 0, 0);
     }
 };
 
@@ -409,22 +409,36 @@ __global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
         }
     };
     float16v acc[2][2] = {};
+    Frag<2, 2> f0, f1;
     for (int s = 0; s < kStages && s < stages; ++s) load(s);
-    for (int s = 0; s < stages; ++s) {
-        if (s + kStages <= stages)
+    int s = 0;
+    for (; s < stages - kStages; ++s) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
+        const char* st = lds[wave][s % kStages];
+        f0.read(st, st + 8192, lane, 0);
+        f1.read(st, st + 8192, lane, 1);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read: the next copy may take its place
+        load(s + kStages);
+        f0.multiply(acc);
+        f1.multiply(acc);
+        for (int i = 0; i < kLoads; ++i) {                   // copies dealt out between the products: in one go they hold the wave up
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedVmem, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 24 - kLoads, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; s < stages; ++s) {
+        if (s + 1 < stages)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         const char* st = lds[wave][s % kStages];
-        Frag<2, 2> f0, f1;
         f0.read(st, st + 8192, lane, 0);
         f1.read(st, st + 8192, lane, 1);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read: the next copy may take its place
-        __builtin_amdgcn_sched_barrier(0);
-        if (s + kStages < stages) load(s + kStages);
         f0.multiply(acc);
         f1.multiply(acc);
-        __builtin_amdgcn_sched_barrier(0);
     }
     if constexpr (kMode == kFinal) {
         if (a.guard && a.guard->status != 0) return;
@@ -463,11 +477,14 @@ __global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
 
 // T x T tiles for larger products: waves of kNu x kNv MFMA tiles share kStages stages of one block column each.  The operands of each 16 k are
 // read while the products of the 16 before are computed, and the stage's one barrier falls between the two halves, with products on
-// either side.  4096 x 4096 x 4096 with T = 256: 336 us (1.23 PFLOP/s of piece products), against 374 with reads and products in turn; the
-// products alone, on operands that stay in registers, take 252 us: the device's power limit (177 with zeros for operands).
+// either side; the loop holds no branch, so that the compiler (T = 256) or the group barriers (kDealt) can place the reads and copies
+// between the products.  4096 x 4096 x 4096 with T = 256: 300 us (1.38 PFLOP/s of piece products; a large library product of fp16 matrices: 1.35),
+// against 374 with reads and products in turn and 335 with the copies under a condition; the products alone, on operands that
+// stay in registers, take 252 us: the device's power limit (177 with zeros for operands).
 template <int T, int kNu, int kNv, int kStages, int kMode, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_kernel(ArgsOf<kMode> a) {
     constexpr int kAcross = T / 32 / kNv, kW = T / 32 / kNu * kAcross, kStage = 2 * T * 128, kLoads = kStage / 1024 / kW;
+    constexpr bool kDealt = T < 256;
     static_assert(kW * kFlipBytes <= kStage && kLoads * kW * 1024 == kStage, "");
     __shared__ __align__(16) char lds[kStages][kStage];
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
@@ -495,22 +512,49 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     f0.read(lds[0] + wr * 128, lds[0] + (T + wc) * 128, lane, 0);
-    for (int k = 0; k < a.kc; ++k) {
+    constexpr int kReads = 2 * (kNu + kNv), kMul = 3 * kNu * kNv;
+    int k = 0;
+    for (; k < a.kc - kStages; ++k) {
         f1.read(lds[k % kStages] + wr * 128, lds[k % kStages] + (T + wc) * 128, lane, 1);
-        __builtin_amdgcn_sched_barrier(0);
         f0.multiply(acc);
+        if (kDealt) {
+            for (int i = 0; i < kReads; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, kMul - kReads, 0);
+        }
         __builtin_amdgcn_sched_barrier(0);
         // the next stage has landed (the kStages - 2 after it may be on their way), and every wave has read this one
-        if (k + kStages <= a.kc)
-            asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((kStages - 2) * kLoads) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (k + kStages < a.kc) load(k + kStages);
+        const char* next = lds[(k + 1) % kStages];
+        f0.read(next + wr * 128, next + (T + wc) * 128, lane, 0);
+        load(k + kStages);
+        f1.multiply(acc);
+        if (kDealt) {
+            for (int i = 0; i < kReads / 2; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            }
+            for (int i = 0; i < kLoads; ++i) {
+                __builtin_amdgcn_sched_group_barrier(kSchedVmem, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, kMul, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; k < a.kc; ++k) {                                  // the last stages: nothing left to copy
+        f1.read(lds[k % kStages] + wr * 128, lds[k % kStages] + (T + wc) * 128, lane, 1);
+        f0.multiply(acc);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
         const char* next = lds[(k + 1) % kStages];
         if (k + 1 < a.kc) f0.read(next + wr * 128, next + (T + wc) * 128, lane, 0);
-        __builtin_amdgcn_sched_barrier(0);
         f1.multiply(acc);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -672,8 +716,8 @@ Plan plan_of(long rows, long cols) {
 }
 
 // Which kernel computes a product: the one whose time for k = 4096 is least, from the times measured for few and for as many workgroups as run
-// at once, us:            64 x 64, split k by 4: 26 .. 30 a round of 256      by 2: 45 .. 58 of 512       not split: 75 .. 102 of 1024
-//              128 x 128: 75 .. 101 of 256       192 x 192: 150 .. 216 of 256       256 x 256: 205 .. 336 of 256
+// at once, us:            64 x 64, split k by 4: 24 .. 29 a round of 256      by 2: 45 .. 53 of 512       not split: 75 .. 97 of 1024
+//              128 x 128: 77 .. 93 of 256       192 x 192: 138 .. 183 of 256       256 x 256: 194 .. 300 of 256
 struct Choice {
     int tile, split;
 };
@@ -683,8 +727,8 @@ Choice choose(long count, int panels_p, int panels_q, bool sym) {
         int tile, split, at_once;
         double few, full;
     };
-    static constexpr Entry entries[] = {{64, 4, 256, 26, 30},     {64, 2, 512, 45, 58},     {64, 1, 1024, 75, 102},
-                                        {128, 1, 256, 75, 101},   {192, 1, 256, 150, 216},  {256, 1, 256, 205, 336}};
+    static constexpr Entry entries[] = {{64, 4, 256, 24, 29}, {64, 2, 512, 45, 53},   {64, 1, 1024, 75, 97},
+                                        {128, 1, 256, 77, 93}, {192, 1, 256, 138, 183}, {256, 1, 256, 194, 300}};
     Choice best{};
     double least = 1e300;
     for (const Entry& e : entries) {
