@@ -309,8 +309,9 @@ struct Frag {
 };
 
 // What happens to a 32 x 32 tile of C whose first element is (r0, c0): lane l holds columns 8 g + 4 (l / 32) + e (register 4 g + e) of
-// row l % 32.  A row of the tile is one line of a piece matrix; the two lanes of a row exchange halves (hi of both to the first,
-// lo of both to the second) and store whole 16-byte slots.  A transposed copy goes through LDS (4.6 KB a wave, (hi, lo) as a word).
+// row l % 32.  In a piece matrix the tile's rows are 32 lines that follow each other, 4 KB, and so are the rows of its transpose; stored from where
+// the products leave it, it would go out in pieces of 16 bytes (a 256 x 256 tile of X and X^T: 14 us).  It goes through LDS instead
+// (4.6 KB a wave, hi and lo of an element in a word), and every store is a whole kilobyte.
 constexpr int kFlipBytes = 32 * 36 * 4;
 
 template <int kMode, typename O, bool kMuon>
@@ -318,64 +319,68 @@ __device__ __forceinline__ void finish(const ArgsOf<kMode>& a, int mat, float sc
                                        char* lds) {
     if (r0 >= (long)a.panels_p * 64 || c0 >= (long)a.panels_q * 64) return;     // (a tile larger than 64 can reach past the end)
     const int row = lane & 31, half = lane >> 5;
-    const long r = r0 + row;
-    const long kc0 = a.panels_q * 2;
-    const long line = piece_at(r, c0, kc0) & ~127l, sw = ((r >> 1) & 7) << 4;
+    const int by8 = lane >> 3, nth = lane & 7;               // as stored: line 8 i + by8, its nth 16 bytes
+    // (a wave's LDS operations are executed in order: reads see the writes before them, and writes come after the reads before them)
     if constexpr (kMode == kFinal) {
-        if (r < a.rows)
-            for (int g = 0; g < 4; ++g) {
-                float val[4];
-                for (int e = 0; e < 4; ++e) val[e] = acc[g * 4 + e] * scale;
-                const long c = c0 + g * 8 + half * 4;
-                if (c < a.cols) put4<O, kMuon>(a, mat, r, c, val);
-            }
+        float* t = (float*)lds;
+        for (int g = 0; g < 4; ++g)
+            *(float4*)(t + row * 36 + g * 8 + half * 4) = make_float4(acc[g * 4] * scale, acc[g * 4 + 1] * scale, acc[g * 4 + 2] * scale, acc[g * 4 + 3] * scale);
+        for (int i = 0; i < 4; ++i) {
+            const long r = r0 + i * 8 + by8, c = c0 + nth * 4;
+            const float4 x = *(const float4*)(t + (i * 8 + by8) * 36 + nth * 4);
+            const float val[4] = {x.x, x.y, x.z, x.w};
+            if (r < a.rows && c < a.cols) put4<O, kMuon>(a, mat, r, c, val);
+        }
     } else {
-        char* to = a.c0 + mat * a.b0 + line;
-        unsigned word[16];                                   // (hi, lo)
+        const long kc0 = a.panels_q * 2, kc1 = a.panels_p * 2;
+        const long at = ((r0 >> 6) * kc0 + (c0 >> 5)) * kBlockBytes + ((r0 & 63) << 7) + lane * 16;
+        half4 old_h[4], old_l[4];
+        if (kMode == kPoly) {                                // the same tile of P
+            const char* pm = a.p + mat * a.bp + at;
+            uint4 old[4];
+            for (int i = 0; i < 4; ++i) old[i] = *(const uint4*)(pm + i * 1024);
+            for (int i = 0; i < 4; ++i) *(uint4*)(lds + (i * 8 + by8) * 144 + nth * 16) = old[i];
+            const char* line = lds + row * 144 + half * 8;
+            const int sw = ((row >> 1) & 7) << 4;
+            for (int g = 0; g < 4; ++g) {
+                old_h[g] = *(const half4*)(line + ((g << 4) ^ sw));
+                old_l[g] = *(const half4*)(line + ((g << 4) ^ sw ^ 64));
+            }
+        }
+        unsigned* t = (unsigned*)lds;                        // (hi, lo) of element (r, c) at r * 36 + c
         for (int g = 0; g < 4; ++g) {
-            float val[4];
-            for (int e = 0; e < 4; ++e) val[e] = acc[g * 4 + e] * scale;
-            if (kMode == kPoly) {
-                const char* pm = a.p + mat * a.bp + line + half * 8;
-                const half4 h = *(const half4*)(pm + ((g << 4) ^ sw)), l = *(const half4*)(pm + ((g << 4) ^ sw ^ 64));
-                const int on = (int)(r - (c0 + g * 8 + half * 4));              // which of the four is on the diagonal
-                for (int e = 0; e < 4; ++e) {
-                    val[e] = fmaf(a.cc, val[e], a.cb * ((float)h[e] + (float)l[e]));
-                    val[e] += e == on && r < a.m ? a.ca * kScale : 0.f;
-                }
-            }
-            union { f16 e[4]; unsigned w[2]; } hi, lo;
+            unsigned word[4];
             for (int e = 0; e < 4; ++e) {
-                split(val[e], hi.e[e], lo.e[e]);
+                float val = acc[g * 4 + e] * scale;
+                if (kMode == kPoly) {
+                    val = fmaf(a.cc, val, a.cb * ((float)old_h[g][e] + (float)old_l[g][e]));
+                    val += r0 + row == c0 + g * 8 + half * 4 + e && r0 + row < a.m ? a.ca * kScale : 0.f;
+                }
                 union { f16 e[2]; unsigned w; } both;
-                both.e[0] = hi.e[e], both.e[1] = lo.e[e];
-                word[g * 4 + e] = both.w;
+                split(val, both.e[0], both.e[1]);
+                word[e] = both.w;
             }
-            uint4 slot;                                      // the first lane of a row: hi of both halves; the second: lo
-            const auto x = __builtin_amdgcn_permlane32_swap(hi.w[0], lo.w[0], false, false);
-            const auto y = __builtin_amdgcn_permlane32_swap(hi.w[1], lo.w[1], false, false);
-            slot.x = x[0], slot.y = y[0], slot.z = x[1], slot.w = y[1];
-            *(uint4*)(to + ((g << 4) ^ sw ^ (half << 6))) = slot;
+            *(uint4*)(t + row * 36 + g * 8 + half * 4) = make_uint4(word[0], word[1], word[2], word[3]);
+        }
+        auto pack = [&](const unsigned (&w)[8], unsigned part) {
+            return make_uint4(__builtin_amdgcn_perm(w[1], w[0], part), __builtin_amdgcn_perm(w[3], w[2], part),
+                              __builtin_amdgcn_perm(w[5], w[4], part), __builtin_amdgcn_perm(w[7], w[6], part));
+        };
+        char* to = a.c0 + mat * a.b0 + at;
+        for (int i = 0; i < 4; ++i) {
+            const int l = i * 8 + by8, slot = nth ^ ((l >> 1) & 7);              // slot 0 .. 3: hi of eight columns, 4 .. 7: lo
+            const uint4 x = *(const uint4*)(t + l * 36 + (slot & 3) * 8), y = *(const uint4*)(t + l * 36 + (slot & 3) * 8 + 4);
+            const unsigned w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            *(uint4*)(to + i * 1024) = pack(w, slot & 4 ? 0x07060302u : 0x05040100u);
         }
         if (flip) {
-            unsigned* t = (unsigned*)lds;
-            for (int g = 0; g < 4; ++g) *(uint4*)(t + row * 36 + g * 8 + half * 4) = make_uint4(word[g * 4], word[g * 4 + 1], word[g * 4 + 2], word[g * 4 + 3]);
-            // (a wave's LDS operations are executed in order: the reads see the writes)
-            const long c = c0 + row;                         // this lane's row of the transpose, k = 16 half ..
-            const long kc1 = a.panels_p * 2;
-            char* tc = (kMode == kApply ? a.c1 + mat * a.b1 : a.c0 + mat * a.b0) + (piece_at(c, r0, kMode == kApply ? kc1 : kc0) & ~127l);
-            const long tw = ((c >> 1) & 7) << 4;
-            for (int g = 0; g < 2; ++g) {
+            char* tc = (kMode == kApply ? a.c1 + mat * a.b1 : a.c0 + mat * a.b0) +
+                       ((c0 >> 6) * (kMode == kApply ? kc1 : kc0) + (r0 >> 5)) * kBlockBytes + ((c0 & 63) << 7) + lane * 16;
+            for (int i = 0; i < 4; ++i) {
+                const int l = i * 8 + by8, slot = nth ^ ((l >> 1) & 7);
                 unsigned w[8];
-                for (int i = 0; i < 8; ++i) w[i] = t[(half * 16 + g * 8 + i) * 36 + row];
-                uint4 h, l;
-                h.x = __builtin_amdgcn_perm(w[1], w[0], 0x05040100u), l.x = __builtin_amdgcn_perm(w[1], w[0], 0x07060302u);
-                h.y = __builtin_amdgcn_perm(w[3], w[2], 0x05040100u), l.y = __builtin_amdgcn_perm(w[3], w[2], 0x07060302u);
-                h.z = __builtin_amdgcn_perm(w[5], w[4], 0x05040100u), l.z = __builtin_amdgcn_perm(w[5], w[4], 0x07060302u);
-                h.w = __builtin_amdgcn_perm(w[7], w[6], 0x05040100u), l.w = __builtin_amdgcn_perm(w[7], w[6], 0x07060302u);
-                const long at = ((half * 2 + g) << 4) ^ tw;
-                *(uint4*)(tc + at) = h;
-                *(uint4*)(tc + (at ^ 64)) = l;
+                for (int e = 0; e < 8; ++e) w[e] = t[((slot & 3) * 8 + e) * 36 + l];
+                *(uint4*)(tc + i * 1024) = pack(w, slot & 4 ? 0x07060302u : 0x05040100u);
             }
         }
     }
@@ -564,7 +569,9 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     const float scale = scale_of<kMode>(a, mat);
     const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
     __syncthreads();
+#pragma unroll
     for (int u = 0; u < kNu; ++u)
+#pragma unroll
         for (int v = 0; v < kNv; ++v)
             finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], (long)ti * T + wr + u * 32, (long)tj * T + wc + v * 32, flip, lane,
                                     lds[0] + wave * kFlipBytes);
@@ -715,27 +722,29 @@ Plan plan_of(long rows, long cols) {
     return p;
 }
 
-// Which kernel computes a product: the one whose time for k = 4096 is least, from the times measured for few and for as many workgroups as run
-// at once, us:            64 x 64, split k by 4: 24 .. 29 a round of 256      by 2: 45 .. 53 of 512       not split: 75 .. 97 of 1024
-//              128 x 128: 77 .. 93 of 256       192 x 192: 138 .. 183 of 256       256 x 256: 194 .. 300 of 256
+// Which kernel computes a product: the one whose estimated time is least.  A round is as many workgroups as run at once; it takes `few` us per 4096
+// of k up to half full and `full` us when full, and `fixed` us whatever k is (its first copies, its results).  Measured on 6 .. 4096 tiles and
+// k = 256 .. 4096; the estimate is within a tenth or two of the measured time and never took a kernel 15 % behind the best.
 struct Choice {
     int tile, split;
 };
 
-Choice choose(long count, int panels_p, int panels_q, bool sym) {
+Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
     struct Entry {
-        int tile, split, at_once;
-        double few, full;
+        int tile, split;
+        long at_once;
+        double few, full, fixed;
     };
-    static constexpr Entry entries[] = {{64, 4, 256, 24, 29}, {64, 2, 512, 45, 53},   {64, 1, 1024, 75, 97},
-                                        {128, 1, 256, 77, 93}, {192, 1, 256, 138, 183}, {256, 1, 256, 194, 300}};
+    static constexpr Entry entries[] = {{64, 4, 256, 24, 29, 4.5}, {64, 2, 512, 45, 53, 5},    {64, 1, 1024, 72, 97, 7},
+                                        {128, 1, 512, 84, 178, 7}, {192, 1, 256, 135, 183, 14}, {256, 1, 256, 196, 298, 20}};
     Choice best{};
     double least = 1e300;
     for (const Entry& e : entries) {
         const int t = e.tile / 64;
         const long r = (panels_p + t - 1) / t, c = (panels_q + t - 1) / t, tiles = count * (sym ? r * (r + 1) / 2 : r * c);
-        const long rounds = (tiles + e.at_once - 1) / e.at_once;
-        const double time = rounds * e.few + (e.full - e.few) * tiles / e.at_once;
+        const long whole = tiles / e.at_once, rest = tiles % e.at_once;
+        const double last = rest ? e.few + (e.full - e.few) * std::fmax(0., 2. * rest / e.at_once - 1.) : 0.;
+        const double time = (whole * e.full + last) * kc / 128. + (whole + (rest > 0)) * e.fixed;
         if (time < least) least = time, best = {e.tile, e.split};
     }
     return best;
@@ -743,7 +752,7 @@ Choice choose(long count, int panels_p, int panels_q, bool sym) {
 
 template <int kMode, typename O = float, bool kMuon = false>
 void product(const FinalArgs& g, int count, hipStream_t s) {
-    const Choice how = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>);
+    const Choice how = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>, g.kc);
     const int t = how.tile / 64;
     const long r = (g.panels_p + t - 1) / t, c = (g.panels_q + t - 1) / t;
     const dim3 grid((unsigned)(count * (kSymmetric<kMode> ? r * (r + 1) / 2 : r * c)));
