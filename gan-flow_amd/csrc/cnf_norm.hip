@@ -4,26 +4,238 @@
 //   h = dy w,  xh = (x - mean) rstd:
 //   dx = rstd (h - mean(h) - xh mean(h xh)),   dw = sum over rows of dy xh,   db = sum over rows of dy
 //
-// All statistics and sums are fp32 (the variance from centred values, never as a difference of moments).  The column sums
-// go through partial sums per block of rows that a second kernel adds in a fixed order: no atomics, the same bits every run.
+// All statistics and sums are fp32 (the variance from centred values, never as a difference of moments).  Bound by memory: every element
+// is read once and written once, so a row stays in registers between its statistics and its result -- 16 bytes of it at a time per
+// thread, loaded at whatever alignment the rows have.  A row belongs to a power of two of a wave's lanes while it fits two chunks a
+// lane, to a workgroup of 256 threads beyond that (up to 8192 columns), and is read again for each pass in the kernels at the
+// end of this file beyond that.  The weights stay in registers while a workgroup goes through its rows.
+// The column sums of the backward pass are kept per thread over a workgroup's rows, written as one partial sum per workgroup, and added by a second
+// kernel in a fixed order: no atomics, the same bits every run.
 #include "cnf_ops.h"
 
 namespace cnf {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr long kMaxChunks = 256;
+constexpr long kMaxBlocks = 2048;     // forward: eight workgroups per CU
+constexpr long kMaxParts = 512;       // backward: two per CU, each with a partial sum to write
+constexpr long kInRegisters = 8192;   // columns
+
+template <typename T>
+constexpr int kVec = 16 / sizeof(T);
+
+// one chunk of a row: kVec<T> elements, the ones past the end 0
+template <typename T, typename E = T>
+struct Chunk {
+    static constexpr int V = kVec<T>;
+    E e[V];
+
+    __device__ __forceinline__ void load(const E* p, long at, long n) {
+        if (at + V <= n) {
+            __builtin_memcpy(e, (const char*)(p + at), sizeof e);
+        } else {
+            for (int k = 0; k < V; ++k) e[k] = at + k < n ? p[at + k] : from_f32<E>(0.f);
+        }
+    }
+    __device__ __forceinline__ void store(E* p, long at, long n) const {
+        if (at + V <= n) {
+            __builtin_memcpy((char*)(p + at), e, sizeof e);
+        } else {
+            for (int k = 0; k < V; ++k)
+                if (at + k < n) p[at + k] = e[k];
+        }
+    }
+    __device__ __forceinline__ float operator[](int k) const { return to_f32(e[k]); }
+};
+
+// sums over the `group` threads of a row (a power of two of a wave's lanes, or kBlock: the workgroup); red: this sum's own LDS words
+template <bool kBlock, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int group, float (*red)[N]) {
+    for (int o = (kBlock ? 64 : group) / 2; o > 0; o >>= 1)
+        for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o);
+    if (kBlock) {
+        if ((threadIdx.x & 63) == 0)
+            for (int k = 0; k < N; ++k) red[threadIdx.x >> 6][k] = v[k];
+        __syncthreads();
+        for (int k = 0; k < N; ++k) v[k] = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+    }
+}
+
+template <typename T, typename W, int NC, bool kBlock>
+__global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a, int group) {
+    constexpr int V = kVec<T>;
+    __shared__ float red[2][kThreads / 64][1];
+    const int lane = kBlock ? threadIdx.x : threadIdx.x & (group - 1), sub = kBlock ? 0 : threadIdx.x / group;
+    const int across = kBlock ? kThreads : group, high = kThreads / across;
+    const T* x = (const T*)a.x;
+    const W *w = (const W*)a.weight, *b = (const W*)a.bias;
+    T* y = (T*)a.y;
+    const float inv_n = 1.0f / (float)a.cols;
+    Chunk<T, W> wc[NC], bc[NC];
+    for (int j = 0; j < NC; ++j) {
+        const long c = (long)(j * across + lane) * V;
+        if (w) wc[j].load(w, c, a.cols);
+        if (b) bc[j].load(b, c, a.cols);
+    }
+    // (a group past the last row has no work, but goes round with its workgroup: uniform barriers)
+    for (long r0 = (long)blockIdx.x * high; r0 < a.rows; r0 += (long)gridDim.x * high) {
+        const long r = r0 + sub;
+        const bool on = kBlock || r < a.rows;
+        const T* xr = x + (on ? r : r0) * a.x_stride;
+        Chunk<T> xc[NC];
+        for (int j = 0; j < NC; ++j) xc[j].load(xr, (long)(j * across + lane) * V, a.cols);
+        float s[1] = {0.f};
+        for (int j = 0; j < NC; ++j)
+            for (int k = 0; k < V; ++k) s[0] += xc[j][k];
+        row_sum<kBlock>(s, group, red[0]);
+        const float mean = s[0] * inv_n;
+        float q[1] = {0.f};
+        for (int j = 0; j < NC; ++j)
+            for (int k = 0; k < V; ++k) {
+                const float d = xc[j][k] - mean;
+                q[0] = (long)(j * across + lane) * V + k < a.cols ? fmaf(d, d, q[0]) : q[0];
+            }
+        row_sum<kBlock>(q, group, red[1]);
+        const float rstd = 1.0f / sqrtf(q[0] * inv_n + a.eps);
+        if (!on) continue;
+        for (int j = 0; j < NC; ++j) {
+            const long c = (long)(j * across + lane) * V;
+            if (c >= a.cols) continue;
+            Chunk<T> out;
+            for (int k = 0; k < V; ++k) {
+                float v = (xc[j][k] - mean) * rstd;
+                if (w) v *= wc[j][k];
+                if (b) v += bc[j][k];
+                out.e[k] = from_f32<T>(v);
+            }
+            out.store(y + r * a.cols, c, a.cols);
+        }
+        if (lane == 0) {
+            if (a.mean) a.mean[r] = mean;
+            if (a.rstd) a.rstd[r] = rstd;
+        }
+    }
+}
+
+// dx of a workgroup's rows, and their partial column sums to part[block][0 | 1][col] (dy xh | dy)
+template <typename T, typename W, int NC, bool kBlock>
+__global__ __launch_bounds__(kThreads) void norm_bwd_kernel(NormArgs a, int group) {
+    constexpr int V = kVec<T>;
+    __shared__ float red[2][kThreads / 64][2];
+    __shared__ float sums[kBlock ? 1 : kThreads / 64][kBlock ? 1 : 64 * NC * V];
+    const int lane = kBlock ? threadIdx.x : threadIdx.x & (group - 1), sub = kBlock ? 0 : threadIdx.x / group;
+    const int across = kBlock ? kThreads : group, high = kThreads / across;
+    const T *x = (const T*)a.x, *dy = (const T*)a.dy;
+    const W* w = (const W*)a.weight;
+    T* dx = (T*)a.dx;
+    const float inv_n = 1.0f / (float)a.cols;
+    Chunk<T, W> wc[NC];
+    if (w)
+        for (int j = 0; j < NC; ++j) wc[j].load(w, (long)(j * across + lane) * V, a.cols);
+    float dw[NC][V] = {}, db[NC][V] = {};
+    int turn = 0;
+    for (long r0 = (long)blockIdx.x * high; r0 < a.rows; r0 += (long)gridDim.x * high) {
+        const long r = r0 + sub;
+        const bool on = kBlock || r < a.rows;
+        const long rr = on ? r : r0;
+        Chunk<T> xc[NC], gc[NC];
+        for (int j = 0; j < NC; ++j) {
+            const long c = (long)(j * across + lane) * V;
+            xc[j].load(x + rr * a.x_stride, c, a.cols);
+            gc[j].load(dy + rr * a.dy_stride, c, a.cols);
+        }
+        const float mean = a.mean[rr], rstd = a.rstd[rr];
+        float s[2] = {0.f, 0.f};
+        for (int j = 0; j < NC; ++j)
+            for (int k = 0; k < V; ++k) {
+                const bool in = (long)(j * across + lane) * V + k < a.cols;
+                const float g = gc[j][k], xh = in ? (xc[j][k] - mean) * rstd : 0.f, h = w ? g * wc[j][k] : g;
+                s[0] += h;
+                s[1] = fmaf(h, xh, s[1]);
+                if (on) {
+                    dw[j][k] = fmaf(g, xh, dw[j][k]);
+                    db[j][k] += g;
+                }
+            }
+        if (!dx) continue;                                   // (a kernel argument: the same way round for every thread)
+        row_sum<kBlock>(s, group, red[turn]);
+        turn ^= 1;
+        if (!on) continue;
+        const float mh = s[0] * inv_n, mx = s[1] * inv_n;
+        for (int j = 0; j < NC; ++j) {
+            const long c = (long)(j * across + lane) * V;
+            if (c >= a.cols) continue;
+            Chunk<T> out;
+            for (int k = 0; k < V; ++k) {
+                const float h = w ? gc[j][k] * wc[j][k] : gc[j][k];
+                out.e[k] = from_f32<T>(rstd * (h - mh - (xc[j][k] - mean) * rstd * mx));
+            }
+            out.store(dx + r * a.cols, c, a.cols);
+        }
+    }
+    if (!a.dweight && !a.dbias) return;
+    float* part = a.part + (long)blockIdx.x * 2 * a.cols;
+    if (kBlock) {
+        for (int j = 0; j < NC; ++j)
+            for (int k = 0; k < V; ++k) {
+                const long c = (long)(j * across + lane) * V + k;
+                if (c < a.cols) part[c] = dw[j][k], part[a.cols + c] = db[j][k];
+            }
+        return;
+    }
+    // the rows of a wave side by side, then the waves
+    for (int which = 0; which < 2; ++which) {
+        for (int j = 0; j < NC; ++j)
+            for (int k = 0; k < V; ++k) {
+                float v = which ? db[j][k] : dw[j][k];
+                for (int o = group; o < 64; o <<= 1) v += __shfl_xor(v, o);
+                if ((threadIdx.x & 63) < group) sums[threadIdx.x >> 6][(j * group + lane) * V + k] = v;
+            }
+        __syncthreads();
+        for (long c = threadIdx.x; c < a.cols; c += kThreads) part[which * a.cols + c] = (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+        __syncthreads();
+    }
+}
+
+// dweight and dbias: the sum of `parts` partial sums; 64 columns per workgroup, four waves over the partial sums
+template <typename W>
+__global__ __launch_bounds__(kThreads) void norm_cols_kernel(NormArgs a, long parts) {
+    __shared__ float red[kThreads];
+    const int which = blockIdx.y;
+    W* out = (W*)(which ? a.dbias : a.dweight);
+    if (!out) return;
+    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    if (c < a.cols) {
+        const float* p = a.part + which * a.cols + c;
+        const long step = 2 * a.cols;
+        long k = threadIdx.x >> 6;
+        for (; k + 12 < parts; k += 16) {
+            s0 += p[k * step];
+            s1 += p[(k + 4) * step];
+            s2 += p[(k + 8) * step];
+            s3 += p[(k + 12) * step];
+        }
+        for (; k < parts; k += 4) s0 += p[k * step];
+    }
+    red[threadIdx.x] = (s0 + s1) + (s2 + s3);
+    __syncthreads();
+    if (threadIdx.x < 64 && c < a.cols)
+        out[c] = from_f32<W>((red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]));
+}
+
+// ---- rows too long for registers: a workgroup per row, which reads it again for each pass ------------------------------------------
 
 __device__ __forceinline__ float block_sum(float v, float* red) {
     for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
-    return red[0] + red[1] + red[2] + red[3];
+    return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 template <typename T, typename W>
-__global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a) {
+__global__ __launch_bounds__(kThreads) void long_fwd_kernel(NormArgs a) {
     __shared__ float red[kThreads / 64];
     const T* x = (const T*)a.x;
     const W *w = (const W*)a.weight, *b = (const W*)a.bias;
@@ -53,7 +265,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a) {
 }
 
 template <typename T, typename W>
-__global__ __launch_bounds__(kThreads) void norm_dx_kernel(NormArgs a) {
+__global__ __launch_bounds__(kThreads) void long_dx_kernel(NormArgs a) {
     __shared__ float red[kThreads / 64];
     const T *x = (const T*)a.x, *dy = (const T*)a.dy;
     const W* w = (const W*)a.weight;
@@ -76,12 +288,12 @@ __global__ __launch_bounds__(kThreads) void norm_dx_kernel(NormArgs a) {
     }
 }
 
-// partial column sums of one chunk of rows: part[0][chunk][col] = sum dy xh, part[1][chunk][col] = sum dy
+// partial column sums of chunk blockIdx.y of the rows, 64 columns per workgroup
 template <typename T>
-__global__ __launch_bounds__(kThreads) void norm_part_kernel(NormArgs a, long chunks) {
+__global__ __launch_bounds__(kThreads) void long_part_kernel(NormArgs a, long parts) {
     __shared__ float red[2][kThreads];
     const T *x = (const T*)a.x, *dy = (const T*)a.dy;
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63), per = (a.rows + chunks - 1) / chunks;
+    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63), per = (a.rows + parts - 1) / parts;
     const long r0 = blockIdx.y * per, r1 = r0 + per < a.rows ? r0 + per : a.rows;
     float sw = 0.f, sb = 0.f;
     if (c < a.cols)
@@ -95,50 +307,81 @@ __global__ __launch_bounds__(kThreads) void norm_part_kernel(NormArgs a, long ch
     __syncthreads();
     if (threadIdx.x < 64 && c < a.cols)
         for (int k = 0; k < 2; ++k)
-            a.part[(k * chunks + blockIdx.y) * a.cols + c] =
+            a.part[((long)blockIdx.y * 2 + k) * a.cols + c] =
                 (red[k][threadIdx.x] + red[k][threadIdx.x + 64]) + (red[k][threadIdx.x + 128] + red[k][threadIdx.x + 192]);
 }
 
-template <typename W>
-__global__ __launch_bounds__(kThreads) void norm_cols_kernel(NormArgs a, long chunks) {
-    const long c = (long)blockIdx.x * kThreads + threadIdx.x;
-    W* out = (W*)(blockIdx.y ? a.dbias : a.dweight);
-    if (c >= a.cols || !out) return;
-    const float* p = a.part + (long)blockIdx.y * chunks * a.cols + c;
-    float s = 0.f;
-    for (long k = 0; k < chunks; ++k) s += p[k * a.cols];
-    out[c] = from_f32<W>(s);
+// ---- launches --------------------------------------------------------------------------------------------------------------------
+
+// threads per row and chunks per thread: a wave's lanes while two chunks each hold the row, else the workgroup
+struct Shape {
+    int group, chunks;
+    bool block;
+};
+
+Shape shape_of(long cols, int vec) {
+    const long n = (cols + vec - 1) / vec;
+    Shape s{1, 1, false};
+    while (s.group < 64 && s.group < n) s.group *= 2;
+    if (n > 128) s.block = true, s.group = kThreads;
+    while ((long)s.group * s.chunks < n) s.chunks *= 2;
+    return s;
 }
 
-long chunks_of(long rows) {
-    const long c = (rows + 63) / 64;
-    return c < kMaxChunks ? c : kMaxChunks;
+long parts_of(long rows, long cols, int vec) {
+    if (cols > kInRegisters) {
+        const long c = (rows + 63) / 64;
+        return c < kMaxParts / 2 ? c : kMaxParts / 2;
+    }
+    const long high = kThreads / shape_of(cols, vec).group, c = (rows + high - 1) / high;
+    return c < kMaxParts ? c : kMaxParts;
 }
 
 template <typename T, typename W>
 hipError_t fwd(const NormArgs& a, hipStream_t s) {
-    const long grid = a.rows < 65536 ? a.rows : 65536;
-    norm_fwd_kernel<T, W><<<dim3((unsigned)grid), dim3(kThreads), 0, s>>>(a);
+    if (a.cols > kInRegisters) {
+        long_fwd_kernel<T, W><<<dim3((unsigned)(a.rows < 65536 ? a.rows : 65536)), kThreads, 0, s>>>(a);
+        return hipGetLastError();
+    }
+    const Shape p = shape_of(a.cols, kVec<T>);
+    const long high = kThreads / p.group, blocks = (a.rows + high - 1) / high;
+    const dim3 grid((unsigned)(blocks < kMaxBlocks ? blocks : kMaxBlocks));
+    if (!p.block && p.chunks == 1) norm_fwd_kernel<T, W, 1, false><<<grid, kThreads, 0, s>>>(a, p.group);
+    else if (!p.block) norm_fwd_kernel<T, W, 2, false><<<grid, kThreads, 0, s>>>(a, p.group);
+    else if (p.chunks == 1) norm_fwd_kernel<T, W, 1, true><<<grid, kThreads, 0, s>>>(a, p.group);
+    else if (p.chunks == 2) norm_fwd_kernel<T, W, 2, true><<<grid, kThreads, 0, s>>>(a, p.group);
+    else if (p.chunks == 4) norm_fwd_kernel<T, W, 4, true><<<grid, kThreads, 0, s>>>(a, p.group);
+    else if constexpr (kVec<T> == 4) norm_fwd_kernel<T, W, 8, true><<<grid, kThreads, 0, s>>>(a, p.group);
     return hipGetLastError();
 }
 
 template <typename T, typename W>
 hipError_t bwd(const NormArgs& a, hipStream_t s) {
-    const long chunks = chunks_of(a.rows);
-    if (a.dx && a.rows > 0) {
-        const long grid = a.rows < 65536 ? a.rows : 65536;
-        norm_dx_kernel<T, W><<<dim3((unsigned)grid), dim3(kThreads), 0, s>>>(a);
+    const long parts = parts_of(a.rows, a.cols, kVec<T>);
+    const bool sums = a.dweight || a.dbias;
+    if (a.cols > kInRegisters) {
+        if (a.dx && a.rows > 0) long_dx_kernel<T, W><<<dim3((unsigned)(a.rows < 65536 ? a.rows : 65536)), kThreads, 0, s>>>(a);
+        if (sums && parts > 0) long_part_kernel<T><<<dim3((unsigned)((a.cols + 63) / 64), (unsigned)parts), kThreads, 0, s>>>(a, parts);
+    } else if (a.rows > 0) {
+        const Shape p = shape_of(a.cols, kVec<T>);
+        const dim3 grid((unsigned)parts);
+        if (!p.block && p.chunks == 1) norm_bwd_kernel<T, W, 1, false><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (!p.block) norm_bwd_kernel<T, W, 2, false><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (p.chunks == 1) norm_bwd_kernel<T, W, 1, true><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (p.chunks == 2) norm_bwd_kernel<T, W, 2, true><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (p.chunks == 4) norm_bwd_kernel<T, W, 4, true><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if constexpr (kVec<T> == 4) norm_bwd_kernel<T, W, 8, true><<<grid, kThreads, 0, s>>>(a, p.group);
     }
-    if (a.dweight || a.dbias) {
-        if (chunks > 0) norm_part_kernel<T><<<dim3((unsigned)((a.cols + 63) / 64), (unsigned)chunks), dim3(kThreads), 0, s>>>(a, chunks);
-        norm_cols_kernel<W><<<dim3((unsigned)((a.cols + kThreads - 1) / kThreads), 2), dim3(kThreads), 0, s>>>(a, chunks);
-    }
+    if (sums) norm_cols_kernel<W><<<dim3((unsigned)((a.cols + 63) / 64), 2), kThreads, 0, s>>>(a, parts);
     return hipGetLastError();
 }
 
 }  // namespace
 
-size_t layer_norm_workspace_bytes(long rows, long cols) { return (size_t)2 * chunks_of(rows) * cols * sizeof(float); }
+size_t layer_norm_workspace_bytes(long rows, long cols) {
+    const long p = parts_of(rows, cols, 4), q = parts_of(rows, cols, 8);
+    return (size_t)2 * (p > q ? p : q) * cols * sizeof(float);
+}
 
 #define CNF_NORM_DISPATCH(fn)                                                          \
     if (dtype == CNF_F32 && wdtype == CNF_F32) return fn<float, float>(a, s);           \
