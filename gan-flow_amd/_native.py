@@ -2,6 +2,7 @@
 device memory and the stream; every number is produced by the HIP kernels.  There is NO fallback: if the
 library is missing or the tensors are not on a HIP device the calls raise."""
 import ctypes
+import functools
 import os
 
 import torch
@@ -560,8 +561,33 @@ def _elem(t, name, dtypes=None):
     return t
 
 
+class _at:
+    """Within the block `index` is the current HIP device; nothing is done where it is already (the usual case, and a switch costs
+    more than a small kernel's launch).  Gives the raw handle of the device's current stream."""
+    __slots__ = ("index", "was")
+
+    def __init__(self, device):
+        self.index = device.index
+
+    def __enter__(self):
+        self.was = torch.cuda.current_device()
+        if self.was != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream if _RAW_STREAM is None else _RAW_STREAM(self.index)
+
+    def __exit__(self, *exc):
+        if self.was != self.index:
+            torch.cuda.set_device(self.was)
+        return False
+
+
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (what torch.cuda.current_stream wraps; 0.1 against 2.7 us)
+
+
 def _rows_of(t):
     """(tensor, row stride) of a (rows, cols) tensor whose rows are contiguous; a copy where they are not."""
+    if t.is_contiguous():
+        return t, t.shape[1]
     if t.stride(1) != 1 and t.shape[1] > 1:
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
@@ -571,7 +597,7 @@ def _norm_weight(t, name, x):
     if t is None:
         return None
     _elem(t, name, (torch.float32, x.dtype))
-    if t.shape != (x.shape[1],) or t.device != x.device:
+    if t.shape != x.shape[1:] or t.device != x.device:
         raise CnfError("%s must have shape (%d,) on %s (got %s on %s)" % (name, x.shape[1], x.device, tuple(t.shape), t.device))
     return t if t.is_contiguous() else t.contiguous()
 
@@ -581,32 +607,68 @@ def _norm_args(x, weight, bias):
     if x.dim() != 2 or x.shape[1] == 0:
         raise CnfError("x must be (rows, cols) with cols > 0 (got %s)" % (tuple(x.shape),))
     weight, bias = _norm_weight(weight, "weight", x), _norm_weight(bias, "bias", x)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+    if weight is None:
+        return None, bias, torch.float32 if bias is None else bias.dtype
+    if bias is not None and weight.dtype != bias.dtype:
         raise CnfError("weight and bias must have one type (got %s and %s)" % (weight.dtype, bias.dtype))
-    wd = weight.dtype if weight is not None else bias.dtype if bias is not None else torch.float32
-    return weight, bias, wd
+    return weight, bias, weight.dtype
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def norm_forward(x, weight, bias, eps, want_stats):
+    """layer_norm_fwd without the unpacking: (y, stats, x, weight, wdtype), stats (2, rows) or None, and x and weight as the kernel read
+    them (copies where rows were not contiguous) for norm_backward."""
+    lib = load_library()
+    weight, bias, wd = _norm_args(x, weight, bias)
+    x, stride = _rows_of(x)
+    rows, cols = x.shape
+    dt, dev = x.dtype, x.device
+    y = torch.empty((rows, cols), dtype=dt, device=dev)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if want_stats else None
+    mean = stats.data_ptr() if want_stats else None
+    with _at(dev) as stream:
+        rc = lib.cnf_layer_norm_fwd(x.data_ptr(), stride, DTYPE_IDS[dt], _addr(weight), _addr(bias), DTYPE_IDS[wd], rows, cols, float(eps),
+                                    y.data_ptr(), mean, mean + 4 * rows if want_stats else None, stream)
+    if rc:
+        _check(rc, lib)
+    return y, stats, x, weight, wd
+
+
+def norm_backward(dy, x, weight, wd, mean_ptr, rstd_ptr, want):
+    """layer_norm_bwd on operands that norm_forward (or layer_norm_bwd) has checked; dy: of x's type, shape and device."""
+    lib = load_library()
+    x, x_stride = _rows_of(x)
+    dy, dy_stride = _rows_of(dy)
+    rows, cols = x.shape
+    dt, dev = x.dtype, x.device
+    dx = torch.empty((rows, cols), dtype=dt, device=dev) if want[0] else None
+    dw = torch.empty(cols, dtype=wd, device=dev) if want[1] else None
+    db = torch.empty(cols, dtype=wd, device=dev) if want[2] else None
+    if dx is None and dw is None and db is None:
+        return None, None, None
+    need = lib.cnf_layer_norm_workspace_bytes(rows, cols) if want[1] or want[2] else 0
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    with _at(dev) as stream:
+        rc = lib.cnf_layer_norm_bwd(dy.data_ptr(), dy_stride, x.data_ptr(), x_stride, DTYPE_IDS[dt], _addr(weight), DTYPE_IDS[wd],
+                                    mean_ptr, rstd_ptr, rows, cols, _addr(dx), _addr(dw), _addr(db), _addr(ws), need, stream)
+    if rc:
+        _check(rc, lib)
+    return dx, dw, db
 
 
 def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, want_stats=True):
     """Layer normalisation of the rows of x (rows, cols).  Returns (y, mean, rstd); the two statistics (rows floats each, what
     layer_norm_bwd needs) are None where want_stats is false."""
-    lib = load_library()
-    weight, bias, wd = _norm_args(x, weight, bias)
-    x, stride = _rows_of(x)
-    rows, cols = x.shape
-    y = torch.empty((rows, cols), dtype=x.dtype, device=x.device)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if want_stats else None
-    with torch.cuda.device(x.device):
-        _check(lib.cnf_layer_norm_fwd(_ptr(x), stride, DTYPE_IDS[x.dtype], _ptr(weight), _ptr(bias), DTYPE_IDS[wd], rows, cols, float(eps),
-                                      _ptr(y), _ptr(mean), _ptr(rstd), _stream()), lib)
-    return y, mean, rstd
+    y, stats = norm_forward(x, weight, bias, eps, want_stats)[:2]
+    return (y, stats[0], stats[1]) if want_stats else (y, None, None)
 
 
 def layer_norm_bwd(dy, x, weight, mean, rstd, want=(True, True, True), wdtype=None):
     """Gradients of layer_norm_fwd: (dx, dweight, dbias), each None where `want` says so.  wdtype: the type of dweight and
     dbias where there is no weight to take it from."""
-    lib = load_library()
     weight, _, wd = _norm_args(x, weight, None)
     if weight is None and wdtype is not None:
         wd = wdtype
@@ -615,83 +677,119 @@ def layer_norm_bwd(dy, x, weight, mean, rstd, want=(True, True, True), wdtype=No
     _elem(dy, "dy", (x.dtype,))
     if dy.shape != x.shape or dy.device != x.device:
         raise CnfError("dy must have x's shape %s and device (got %s on %s)" % (tuple(x.shape), tuple(dy.shape), dy.device))
-    x, x_stride = _rows_of(x)
-    dy, dy_stride = _rows_of(dy)
-    rows, cols = x.shape
-    mean, rstd = _dev(mean, "mean", (rows,)), _dev(rstd, "rstd", (rows,))
-    dx = torch.empty((rows, cols), dtype=x.dtype, device=x.device) if want[0] else None
-    dw = torch.empty(cols, dtype=wd, device=x.device) if want[1] else None
-    db = torch.empty(cols, dtype=wd, device=x.device) if want[2] else None
-    if dx is None and dw is None and db is None:
-        return None, None, None
-    with torch.cuda.device(x.device):
-        ws = torch.empty(int(lib.cnf_layer_norm_workspace_bytes(rows, cols)) if want[1] or want[2] else 0, dtype=torch.uint8, device=x.device)
-        _check(lib.cnf_layer_norm_bwd(_ptr(dy), dy_stride, _ptr(x), x_stride, DTYPE_IDS[x.dtype], _ptr(weight), DTYPE_IDS[wd], _ptr(mean),
-                                      _ptr(rstd), rows, cols, _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), ws.numel(), _stream()), lib)
-    return dx, dw, db
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        if _dev(t, name, x.shape[:1]).data_ptr() != t.data_ptr() or t.device != x.device:
+            raise CnfError("%s must be contiguous and on %s" % (name, x.device))
+    return norm_backward(dy, x, weight, wd, mean.data_ptr(), rstd.data_ptr(), want)
 
 
-def newton_schulz(steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
-    """CnfNewtonSchulz of `steps` steps; coefficients: one (a, b, c), or a sequence of one per step."""
-    steps = int(steps)
+@functools.lru_cache(maxsize=64)
+def _newton_schulz(steps, coefficients, eps):
     if not 1 <= steps <= NS_MAX_STEPS:
         raise CnfError("between 1 and %d Newton-Schulz steps (got %d)" % (NS_MAX_STEPS, steps))
-    coefficients = list(coefficients)
-    if len(coefficients) == 3 and not any(hasattr(c, "__len__") for c in coefficients):
-        coefficients = [coefficients] * steps
-    if len(coefficients) != steps or any(len(t) != 3 for t in coefficients):
+    if len(coefficients) == 3 and not any(isinstance(c, tuple) for c in coefficients):
+        coefficients = (coefficients,) * steps
+    if len(coefficients) != steps or any(not isinstance(t, tuple) or len(t) != 3 for t in coefficients):
         raise CnfError("coefficients must be (a, b, c), or one (a, b, c) for each of the %d steps" % steps)
     ns = CnfNewtonSchulz()
-    ns.steps, ns.eps = steps, float(eps)
+    ns.steps, ns.eps = steps, eps
     for k, (a, b, c) in enumerate(coefficients):
         ns.a[k], ns.b[k], ns.c[k] = float(a), float(b), float(c)
     return ns
 
 
-def _matrices(ts, name, dtype, like=None):
-    """Checks a list of equally shaped and strided matrices with contiguous rows; returns (pointer array, row stride)."""
-    t0 = ts[0]
-    for t in ts:
+def newton_schulz(steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7):
+    """CnfNewtonSchulz of `steps` steps; coefficients: one (a, b, c), or a sequence of one per step."""
+    ns = CnfNewtonSchulz()
+    ctypes.pointer(ns)[0] = ns_params(steps, coefficients, eps)
+    return ns
+
+
+def ns_params(steps, coefficients, eps):
+    """newton_schulz, shared by all calls with the same numbers: not to be changed."""
+    if type(coefficients) is not tuple or any(hasattr(c, "__len__") for c in coefficients):
+        coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
+    return _newton_schulz(int(steps), coefficients, float(eps))
+
+
+def _stack(t, name, dtype):
+    """Pointer array and row stride of a (count, rows, cols) tensor, or of a list of matrices of one shape, device and stride, with
+    contiguous rows that do not overlap."""
+    if torch.is_tensor(t):
         _elem(t, name, (dtype,))
-        if t.dim() != 2 or t.shape != t0.shape or t.device != t0.device or t.stride() != t0.stride() or \
-                (like is not None and (t.shape != like.shape or t.device != like.device)):
-            raise CnfError("%s: matrices of one shape, device and stride are wanted" % name)
-        if t.shape[1] > 1 and t.stride(1) != 1:
-            raise CnfError("%s: rows must be contiguous (strides %s)" % (name, tuple(t.stride())))
-    ld = t0.stride(0) if t0.shape[0] > 1 else t0.shape[1]
-    if t0.shape[0] > 1 and ld < t0.shape[1]:
-        raise CnfError("%s: rows overlap (strides %s)" % (name, tuple(t0.stride())))
-    return (ctypes.c_void_p * len(ts))(*[t.data_ptr() for t in ts]), ld
+        n, rows, cols = t.shape
+        one, ld, inner = t.stride()
+        base, step = t.data_ptr(), one * t.element_size()
+        ptrs = (ctypes.c_void_p * n)(*[base + i * step for i in range(n)])
+    else:
+        t0 = t[0]
+        shape, strides, dev = t0.shape, t0.stride(), t0.device
+        for m in t:
+            _elem(m, name, (dtype,))
+            if m.shape != shape or m.stride() != strides or m.device != dev:
+                raise CnfError("%s: matrices of one shape, device and stride are wanted" % name)
+        if len(shape) != 2:
+            raise CnfError("%s: matrices are wanted (got shape %s)" % (name, tuple(shape)))
+        rows, cols = shape
+        ld, inner = strides
+        ptrs = (ctypes.c_void_p * len(t))(*[m.data_ptr() for m in t])
+    if cols > 1 and inner != 1:
+        raise CnfError("%s: rows must be contiguous (strides %s)" % (name, (ld, inner)))
+    if rows > 1 and ld < cols:
+        raise CnfError("%s: rows overlap (strides %s)" % (name, (ld, inner)))
+    return ptrs, ld if rows > 1 else cols
+
+
+def _shape_of(t):
+    return (len(t),) + tuple(t[0].shape[-2:])
+
+
+def matrix_workspace_bytes(count, rows, cols):
+    """Bytes cnf_orthogonalize and cnf_muon_step need; 0 where the sizes are not supported."""
+    return load_library().cnf_orthogonalize_workspace_bytes(count, rows, cols)
 
 
 def orthogonalize(gs, outs, ns):
-    """cnf_orthogonalize: writes the orthogonalised matrices of the list `gs` to those of `outs` (one shape, at most MAX_MATRICES)."""
+    """cnf_orthogonalize: writes the orthogonalised matrices of `gs` (a (count, rows, cols) tensor, or a list of matrices of one shape and
+    stride; at most MAX_MATRICES) to those of `outs`."""
     lib = load_library()
-    g, ldg = _matrices(gs, "g", _elem(gs[0], "g").dtype)
-    out, ldo = _matrices(outs, "out", gs[0].dtype, gs[0])
-    rows, cols = gs[0].shape
-    dev = gs[0].device
-    with torch.cuda.device(dev):
-        ws = torch.empty(int(lib.cnf_orthogonalize_workspace_bytes(len(gs), rows, cols)), dtype=torch.uint8, device=dev)
-        _check(lib.cnf_orthogonalize(g, ldg, out, ldo, DTYPE_IDS[gs[0].dtype], len(gs), rows, cols, ctypes.byref(ns), _ptr(ws), ws.numel(),
-                                     _stream()), lib)
+    g0 = gs[0]
+    dt, dev = g0.dtype, g0.device
+    _elem(g0, "g")
+    g, ldg = _stack(gs, "g", dt)
+    out, ldo = _stack(outs, "out", dt)
+    count, rows, cols = shape = _shape_of(gs)
+    if _shape_of(outs) != shape or outs[0].device != dev:
+        raise CnfError("out must have g's shape %s and device (got %s on %s)" % (shape, _shape_of(outs), outs[0].device))
+    need = lib.cnf_orthogonalize_workspace_bytes(count, rows, cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _at(dev) as stream:
+        rc = lib.cnf_orthogonalize(g, ldg, out, ldo, DTYPE_IDS[dt], count, rows, cols, ctypes.byref(ns), ws.data_ptr(), need, stream)
+    _check(rc, lib)
     return outs
 
 
 def muon_step(params, grads, momenta, ns, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, guard=None):
-    """cnf_muon_step: one Muon update, in place, of the matrices `params` (a list of one shape, at most MAX_MATRICES) from `grads`
-    (of their type) with the fp32 momenta.  guard: stats words as in adam_step."""
+    """cnf_muon_step: one Muon update, in place, of the matrices `params` (as in orthogonalize) from `grads` (of their type) with the fp32
+    momenta.  guard: stats words as in adam_step."""
     lib = load_library()
-    p, ldp = _matrices(params, "params", _elem(params[0], "params").dtype)
-    g, ldg = _matrices(grads, "grads", params[0].dtype, params[0])
-    m, ldm = _matrices(momenta, "momenta", torch.float32, params[0])
-    rows, cols = params[0].shape
-    dev = params[0].device
-    o = CnfMuonOpts(float(lr), float(momentum), float(weight_decay), float(scale), 1 if nesterov else 0, 0)
-    with torch.cuda.device(dev):
-        ws = torch.empty(int(lib.cnf_orthogonalize_workspace_bytes(len(params), rows, cols)), dtype=torch.uint8, device=dev)
-        _check(lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[params[0].dtype], len(params), rows, cols, ctypes.byref(o),
-                                 ctypes.byref(ns), ctypes.c_void_p(_stats_ptr(guard)), _ptr(ws), ws.numel(), _stream()), lib)
+    p0 = params[0]
+    dt, dev = p0.dtype, p0.device
+    _elem(p0, "params")
+    p, ldp = _stack(params, "params", dt)
+    g, ldg = _stack(grads, "grads", dt)
+    m, ldm = _stack(momenta, "momenta", torch.float32)
+    count, rows, cols = shape = _shape_of(params)
+    for name, t in (("grads", grads), ("momenta", momenta)):
+        if _shape_of(t) != shape or t[0].device != dev:
+            raise CnfError("%s must have the parameters' shape %s and device (got %s on %s)" % (name, shape, _shape_of(t), t[0].device))
+    o = CnfMuonOpts(lr, momentum, weight_decay, scale, 1 if nesterov else 0, 0)
+    need = lib.cnf_orthogonalize_workspace_bytes(count, rows, cols)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    with _at(dev) as stream:
+        rc = lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[dt], count, rows, cols, ctypes.byref(o), ctypes.byref(ns),
+                               _stats_ptr(guard), ws.data_ptr(), need, stream)
+    _check(rc, lib)
 
 
 def gu_desc(mean, sigma, unif_intsect, unif_p, extend_dim):

@@ -18,7 +18,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr long kMaxBlocks = 2048;     // forward: eight workgroups per CU
-constexpr long kMaxParts = 512;       // backward: two per CU, each with a partial sum to write
+constexpr long kMaxParts = 768;       // backward: three per CU, each with a partial sum to write
 constexpr long kInRegisters = 8192;   // columns
 
 template <typename T>
@@ -133,18 +133,27 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(NormArgs a, int grou
     if (w)
         for (int j = 0; j < NC; ++j) wc[j].load(w, (long)(j * across + lane) * V, a.cols);
     float dw[NC][V] = {}, db[NC][V] = {};
-    int turn = 0;
-    for (long r0 = (long)blockIdx.x * high; r0 < a.rows; r0 += (long)gridDim.x * high) {
-        const long r = r0 + sub;
-        const bool on = kBlock || r < a.rows;
-        const long rr = on ? r : r0;
-        Chunk<T> xc[NC], gc[NC];
+    Chunk<T> xn[NC], gn[NC];                                 // the next row, on its way while this one is worked on
+    float mean_n = 0.f, rstd_n = 0.f;
+    auto fetch = [&](long r0) {
+        const long rr = kBlock || r0 + sub < a.rows ? r0 + sub : r0;
         for (int j = 0; j < NC; ++j) {
             const long c = (long)(j * across + lane) * V;
-            xc[j].load(x + rr * a.x_stride, c, a.cols);
-            gc[j].load(dy + rr * a.dy_stride, c, a.cols);
+            xn[j].load(x + rr * a.x_stride, c, a.cols);
+            gn[j].load(dy + rr * a.dy_stride, c, a.cols);
         }
-        const float mean = a.mean[rr], rstd = a.rstd[rr];
+        mean_n = a.mean[rr], rstd_n = a.rstd[rr];
+    };
+    int turn = 0;
+    const long step = (long)gridDim.x * high;
+    if ((long)blockIdx.x * high < a.rows) fetch((long)blockIdx.x * high);
+    for (long r0 = (long)blockIdx.x * high; r0 < a.rows; r0 += step) {
+        const long r = r0 + sub;
+        const bool on = kBlock || r < a.rows;
+        Chunk<T> xc[NC], gc[NC];
+        for (int j = 0; j < NC; ++j) xc[j] = xn[j], gc[j] = gn[j];
+        const float mean = mean_n, rstd = rstd_n;
+        if (r0 + step < a.rows) fetch(r0 + step);
         float s[2] = {0.f, 0.f};
         for (int j = 0; j < NC; ++j)
             for (int k = 0; k < V; ++k) {
@@ -197,31 +206,35 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(NormArgs a, int grou
     }
 }
 
-// dweight and dbias: the sum of `parts` partial sums; 64 columns per workgroup, four waves over the partial sums
+// dweight and dbias: the sum of `parts` partial sums; 32 columns per workgroup, 32 threads over the partial sums of each
+constexpr int kSumThreads = 1024;
+
 template <typename W>
-__global__ __launch_bounds__(kThreads) void norm_cols_kernel(NormArgs a, long parts) {
-    __shared__ float red[kThreads];
-    const int which = blockIdx.y;
+__global__ __launch_bounds__(kSumThreads) void norm_cols_kernel(NormArgs a, long parts) {
+    __shared__ float red[32][33];
+    const int which = blockIdx.y, col = threadIdx.x & 31, split = threadIdx.x >> 5;
     W* out = (W*)(which ? a.dbias : a.dweight);
     if (!out) return;
-    const long c = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-    float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
+    const long c = (long)blockIdx.x * 32 + col;
+    float s[4] = {};
     if (c < a.cols) {
         const float* p = a.part + which * a.cols + c;
         const long step = 2 * a.cols;
-        long k = threadIdx.x >> 6;
-        for (; k + 12 < parts; k += 16) {
-            s0 += p[k * step];
-            s1 += p[(k + 4) * step];
-            s2 += p[(k + 8) * step];
-            s3 += p[(k + 12) * step];
+        long k = split;
+        for (; k + 224 < parts; k += 256) {                  // (eight loads at a time: the latency of one)
+            float v[8];
+            for (int u = 0; u < 8; ++u) v[u] = p[(k + u * 32) * step];
+            for (int u = 0; u < 8; ++u) s[u & 3] += v[u];
         }
-        for (; k < parts; k += 4) s0 += p[k * step];
+        for (; k < parts; k += 32) s[0] += p[k * step];
     }
-    red[threadIdx.x] = (s0 + s1) + (s2 + s3);
+    red[split][col] = (s[0] + s[1]) + (s[2] + s[3]);
     __syncthreads();
-    if (threadIdx.x < 64 && c < a.cols)
-        out[c] = from_f32<W>((red[threadIdx.x] + red[threadIdx.x + 64]) + (red[threadIdx.x + 128] + red[threadIdx.x + 192]));
+    for (int half = 16; half > 0; half >>= 1) {
+        if (split < half) red[split][col] += red[split + half][col];
+        __syncthreads();
+    }
+    if (split == 0 && c < a.cols) out[c] = from_f32<W>(red[0][col]);
 }
 
 // ---- rows too long for registers: a workgroup per row, which reads it again for each pass ------------------------------------------
@@ -372,7 +385,7 @@ hipError_t bwd(const NormArgs& a, hipStream_t s) {
         else if (p.chunks == 4) norm_bwd_kernel<T, W, 4, true><<<grid, kThreads, 0, s>>>(a, p.group);
         else if constexpr (kVec<T> == 4) norm_bwd_kernel<T, W, 8, true><<<grid, kThreads, 0, s>>>(a, p.group);
     }
-    if (sums) norm_cols_kernel<W><<<dim3((unsigned)((a.cols + 63) / 64), 2), kThreads, 0, s>>>(a, parts);
+    if (sums) norm_cols_kernel<W><<<dim3((unsigned)((a.cols + 31) / 32), 2), kSumThreads, 0, s>>>(a, parts);
     return hipGetLastError();
 }
 

@@ -106,16 +106,17 @@ class MovingBatchNorm1d(MovingBatchNormNd):
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _native.layer_norm_fwd(x, weight, bias, eps)
-        ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.wdtype = None if bias is None else bias.dtype
+        y, stats, x, weight, ctx.wdtype = _native.norm_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
         return y
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        return _native.layer_norm_bwd(dy, x, weight, mean, rstd, ctx.needs_input_grad[:3], ctx.wdtype) + (None,)
+    def backward(ctx, dy):   # (autograd gives dy the output's type, shape and device)
+        x, weight, stats = ctx.saved_tensors
+        mean = stats.data_ptr()
+        dx, dw, db = _native.norm_backward(dy, x, weight, ctx.wdtype, mean, mean + 4 * stats.shape[1], ctx.needs_input_grad)
+        return dx, dw, db, None
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -128,7 +129,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _LayerNormFn.apply(x2, weight, bias, eps)
     else:
-        y = _native.layer_norm_fwd(x2, weight, bias, eps, want_stats=False)[0]
+        y = _native.norm_forward(x2, weight, bias, eps, False)[0]
     return y if x.dim() == 2 else y.view(x.shape)
 
 

@@ -12,32 +12,37 @@ DEFAULT_COEFFICIENTS = (3.4445, -4.7750, 2.0315)   # steep at 0 (3.44), hovers a
 _WORKSPACE_BUDGET = 8 << 30
 
 
-def _chunks(n, rows, cols):
-    lib = _native.load_library()
-    one = int(lib.cnf_orthogonalize_workspace_bytes(1, rows, cols))
+def _at_once(n, rows, cols):
+    """How many of n matrices one call takes."""
+    one = _native.matrix_workspace_bytes(1, rows, cols)
     if not one:
         raise _native.CnfError("matrices of 1..%d rows and columns (got %d x %d)" % (_native.MAX_MATRIX_DIM, rows, cols))
-    step = max(1, min(_native.MAX_MATRICES, _WORKSPACE_BUDGET // one))
-    return [(i, min(n, i + step)) for i in range(0, n, step)]
+    return max(1, min(n, _native.MAX_MATRICES, _WORKSPACE_BUDGET // one))
 
 
 def orthogonalize(g, steps=5, coefficients=DEFAULT_COEFFICIENTS, eps=1e-7):
     """X = g / (|g|_F + eps), then `steps` times X <- a X + (b X X^T + c (X X^T)^2) X, for every matrix of g (..., rows, cols);
     fp32, fp16 or bf16, returned in g's type.  coefficients: (a, b, c), or one such triple per step.  Matrices of zeros
-    stay zero."""
+    stay zero.  Not differentiable."""
     _native._elem(g, "g")
     if g.dim() < 2:
         raise _native.CnfError("g must be a matrix or a stack of matrices (got shape %s)" % (tuple(g.shape),))
-    ns = _native.newton_schulz(steps, coefficients, eps)
+    ns = _native.ns_params(steps, coefficients, eps)
     out = torch.empty(g.shape, dtype=g.dtype, device=g.device)
     if g.numel() == 0:
         return out
-    g3 = g.detach().reshape((-1,) + tuple(g.shape[-2:]))
-    if (g3.shape[2] > 1 and g3.stride(2) != 1) or (g3.shape[1] > 1 and g3.stride(1) < g3.shape[2]):
+    rows, cols = g.shape[-2:]
+    g3 = g.detach()
+    if g3.dim() != 3:
+        g3 = g3.reshape(-1, rows, cols)
+    if (cols > 1 and g3.stride(2) != 1) or (rows > 1 and g3.stride(1) < cols):
         g3 = g3.contiguous()
-    o3 = out.view(g3.shape)
-    for lo, hi in _chunks(len(g3), *g3.shape[1:]):
-        _native.orthogonalize(g3[lo:hi].unbind(0), o3[lo:hi].unbind(0), ns)
+    o3 = out if out.dim() == 3 else out.view(g3.shape)
+    n = len(g3)
+    step = _at_once(n, rows, cols)
+    for lo in range(0, n, step):
+        whole = step == n
+        _native.orthogonalize(g3 if whole else g3[lo:lo + step], o3 if whole else o3[lo:lo + step], ns)
     return out
 
 
@@ -47,11 +52,10 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
         m <- momentum m + g;   u = g + momentum m (nesterov) or m;   p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)
     grads: of the parameters' types; momenta: fp32.  Matrices of one shape, type and stride are updated side by side.  The
     matrices must not overlap.  guard: the stats words of the solve that made the gradients (a failed one changes nothing)."""
-    params, grads, momenta = list(params), list(grads), list(momenta)
     if not len(params) == len(grads) == len(momenta):
         raise _native.CnfError("%d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
-    ns = _native.newton_schulz(steps, coefficients, eps)
-    groups = {}
+    ns = _native.ns_params(steps, coefficients, eps)
+    groups, seen = {}, set()
     for p, g, m in zip(params, grads, momenta):
         for name, t in (("params", p), ("grads", g), ("momenta", m)):
             _native._elem(t, name)
@@ -59,16 +63,19 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
                 raise _native.CnfError("%s: Muon updates matrices (got shape %s)" % (name, tuple(t.shape)))
         if p.numel() == 0:
             continue
-        if g.shape[1] > 1 and g.stride(1) != 1 or g.shape[0] > 1 and g.stride(0) < g.shape[1]:
+        gs = g.stride()
+        if g.shape[1] > 1 and gs[1] != 1 or g.shape[0] > 1 and gs[0] < g.shape[1]:
             g = g.contiguous()
-        groups.setdefault((p.shape, p.dtype, p.device, p.stride(), g.stride(), m.stride()), []).append((p, g, m))
-    for what in (params, momenta):
-        seen = [t.data_ptr() for t in what if t.numel()]
-        if len(set(seen)) < len(seen):
-            raise _native.CnfError("the same parameter or momentum is given twice")
+            gs = g.stride()
+        for address in (p.data_ptr(), m.data_ptr()):
+            if address in seen:
+                raise _native.CnfError("the same parameter or momentum is given twice")
+            seen.add(address)
+        groups.setdefault((p.shape, p.dtype, p.device, p.stride(), gs, m.stride()), []).append((p, g, m))
     for key, members in groups.items():
-        for lo, hi in _chunks(len(members), *key[0]):
-            ps, gs, ms = zip(*members[lo:hi])
+        step = _at_once(len(members), *key[0])
+        for lo in range(0, len(members), step):
+            ps, gs, ms = zip(*members[lo:lo + step])
             _native.muon_step(ps, gs, ms, ns, lr, momentum, nesterov, weight_decay, scale, guard)
 
 
@@ -94,7 +101,7 @@ class Muon(torch.optim.Optimizer):
         if not (lr >= 0.0 and 0.0 <= momentum < 1.0 and weight_decay >= 0.0 and eps > 0.0):
             raise ValueError("invalid hyper-parameters (lr %r, momentum %r, weight_decay %r, eps %r)" % (lr, momentum, weight_decay, eps))
         adjusted_scale(adjust_lr, 1, 1)
-        _native.newton_schulz(ns_steps, ns_coefficients, eps)
+        _native.ns_params(ns_steps, ns_coefficients, eps)
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_steps=ns_steps,
                                       ns_coefficients=ns_coefficients, eps=eps, adjust_lr=adjust_lr))
         for group in self.param_groups:
