@@ -18,7 +18,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr long kMaxBlocks = 2048;     // forward: eight workgroups per CU
-constexpr long kMaxParts = 768;       // backward: three per CU, each with a partial sum to write
 constexpr long kInRegisters = 8192;   // columns
 
 template <typename T>
@@ -48,23 +47,27 @@ struct Chunk {
     __device__ __forceinline__ float operator[](int k) const { return to_f32(e[k]); }
 };
 
-// sums over the `group` threads of a row (a power of two of a wave's lanes, or kBlock: the workgroup); red: this sum's own LDS words
-template <bool kBlock, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], int group, float (*red)[N]) {
-    for (int o = (kBlock ? 64 : group) / 2; o > 0; o >>= 1)
+// sums over the threads of a row: `group`, a power of two of a wave's lanes, or (TB > 0) the workgroup's TB; red: this sum's own LDS words
+template <int TB, int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], int group, float (*red)[TB > 0 ? TB / 64 : 1]) {
+    for (int o = (TB > 0 ? 64 : group) / 2; o > 0; o >>= 1)
         for (int k = 0; k < N; ++k) v[k] += __shfl_xor(v[k], o);
-    if (kBlock) {
+    if constexpr (TB > 0) {
         if ((threadIdx.x & 63) == 0)
-            for (int k = 0; k < N; ++k) red[threadIdx.x >> 6][k] = v[k];
+            for (int k = 0; k < N; ++k) red[k][threadIdx.x >> 6] = v[k];
         __syncthreads();
-        for (int k = 0; k < N; ++k) v[k] = (red[0][k] + red[1][k]) + (red[2][k] + red[3][k]);
+        for (int k = 0; k < N; ++k) {
+            v[k] = 0.f;
+            for (int u = 0; u < TB / 64; u += 4) v[k] += (red[k][u] + red[k][u + 1]) + (red[k][u + 2] + red[k][u + 3]);
+        }
     }
 }
 
 template <typename T, typename W, int NC, bool kBlock>
 __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a, int group) {
     constexpr int V = kVec<T>;
-    __shared__ float red[2][kThreads / 64][1];
+    constexpr int TB = kBlock ? kThreads : 0;
+    __shared__ float red[2][1][kBlock ? kThreads / 64 : 1];
     const int lane = kBlock ? threadIdx.x : threadIdx.x & (group - 1), sub = kBlock ? 0 : threadIdx.x / group;
     const int across = kBlock ? kThreads : group, high = kThreads / across;
     const T* x = (const T*)a.x;
@@ -87,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a, int grou
         float s[1] = {0.f};
         for (int j = 0; j < NC; ++j)
             for (int k = 0; k < V; ++k) s[0] += xc[j][k];
-        row_sum<kBlock>(s, group, red[0]);
+        row_sum<TB>(s, group, red[0]);
         const float mean = s[0] * inv_n;
         float q[1] = {0.f};
         for (int j = 0; j < NC; ++j)
@@ -95,7 +98,7 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a, int grou
                 const float d = xc[j][k] - mean;
                 q[0] = (long)(j * across + lane) * V + k < a.cols ? fmaf(d, d, q[0]) : q[0];
             }
-        row_sum<kBlock>(q, group, red[1]);
+        row_sum<TB>(q, group, red[1]);
         const float rstd = 1.0f / sqrtf(q[0] * inv_n + a.eps);
         if (!on) continue;
         for (int j = 0; j < NC; ++j) {
@@ -118,13 +121,15 @@ __global__ __launch_bounds__(kThreads) void norm_fwd_kernel(NormArgs a, int grou
 }
 
 // dx of a workgroup's rows, and their partial column sums to part[block][0 | 1][col] (dy xh | dy)
-template <typename T, typename W, int NC, bool kBlock>
-__global__ __launch_bounds__(kThreads) void norm_bwd_kernel(NormArgs a, int group) {
+// TB: threads that share a row, or 0: a wave's lanes by `group`, 256 threads
+template <typename T, typename W, int NC, int TB>
+__global__ __launch_bounds__(TB > 0 ? TB : kThreads) void norm_bwd_kernel(NormArgs a, int group) {
     constexpr int V = kVec<T>;
-    __shared__ float red[2][kThreads / 64][2];
+    constexpr bool kBlock = TB > 0;
+    __shared__ float red[2][2][kBlock ? TB / 64 : 1];
     __shared__ float sums[kBlock ? 1 : kThreads / 64][kBlock ? 1 : 64 * NC * V];
     const int lane = kBlock ? threadIdx.x : threadIdx.x & (group - 1), sub = kBlock ? 0 : threadIdx.x / group;
-    const int across = kBlock ? kThreads : group, high = kThreads / across;
+    const int across = kBlock ? TB : group, high = kBlock ? 1 : kThreads / group;
     const T *x = (const T*)a.x, *dy = (const T*)a.dy;
     const W* w = (const W*)a.weight;
     T* dx = (T*)a.dx;
@@ -154,30 +159,30 @@ __global__ __launch_bounds__(kThreads) void norm_bwd_kernel(NormArgs a, int grou
         for (int j = 0; j < NC; ++j) xc[j] = xn[j], gc[j] = gn[j];
         const float mean = mean_n, rstd = rstd_n;
         if (r0 + step < a.rows) fetch(r0 + step);
+        // (past the end of the row dy and w are 0: nothing to leave out)
         float s[2] = {0.f, 0.f};
         for (int j = 0; j < NC; ++j)
             for (int k = 0; k < V; ++k) {
-                const bool in = (long)(j * across + lane) * V + k < a.cols;
-                const float g = gc[j][k], xh = in ? (xc[j][k] - mean) * rstd : 0.f, h = w ? g * wc[j][k] : g;
+                const float g = gc[j][k], xm = xc[j][k] - mean, h = w ? g * wc[j][k] : g;
                 s[0] += h;
-                s[1] = fmaf(h, xh, s[1]);
-                if (on) {
-                    dw[j][k] = fmaf(g, xh, dw[j][k]);
-                    db[j][k] += g;
-                }
+                s[1] = fmaf(h, xm, s[1]);
+                const float gr = on ? g * rstd : 0.f;
+                dw[j][k] = fmaf(gr, xm, dw[j][k]);
+                db[j][k] += on ? g : 0.f;
             }
         if (!dx) continue;                                   // (a kernel argument: the same way round for every thread)
-        row_sum<kBlock>(s, group, red[turn]);
+        row_sum<TB>(s, group, red[turn]);
         turn ^= 1;
         if (!on) continue;
-        const float mh = s[0] * inv_n, mx = s[1] * inv_n;
+        // dx = rstd h - (x - mean) rstd^2 mean(h xh) - rstd mean(h)
+        const float c0 = -rstd * (s[0] * inv_n), c1 = -(rstd * rstd) * ((s[1] * rstd) * inv_n);
         for (int j = 0; j < NC; ++j) {
             const long c = (long)(j * across + lane) * V;
             if (c >= a.cols) continue;
             Chunk<T> out;
             for (int k = 0; k < V; ++k) {
                 const float h = w ? gc[j][k] * wc[j][k] : gc[j][k];
-                out.e[k] = from_f32<T>(rstd * (h - mh - (xc[j][k] - mean) * rstd * mx));
+                out.e[k] = from_f32<T>(fmaf(h, rstd, fmaf(xc[j][k] - mean, c1, c0)));
             }
             out.store(dx + r * a.cols, c, a.cols);
         }
@@ -326,7 +331,9 @@ __global__ __launch_bounds__(kThreads) void long_part_kernel(NormArgs a, long pa
 
 // ---- launches --------------------------------------------------------------------------------------------------------------------
 
-// threads per row and chunks per thread: a wave's lanes while two chunks each hold the row, else the workgroup
+// threads per row and chunks per thread: a wave's lanes while kWaveChunks chunks each hold the row, else the workgroup
+constexpr int kWaveChunks = 2;
+constexpr long kBwdThreads = 1024 * 256;   // resident in the backward kernel, about
 struct Shape {
     int group, chunks;
     bool block;
@@ -336,18 +343,36 @@ Shape shape_of(long cols, int vec) {
     const long n = (cols + vec - 1) / vec;
     Shape s{1, 1, false};
     while (s.group < 64 && s.group < n) s.group *= 2;
-    if (n > 128) s.block = true, s.group = kThreads;
+    if (n > 64 * kWaveChunks) s.block = true, s.group = kThreads;
     while ((long)s.group * s.chunks < n) s.chunks *= 2;
+    return s;
+}
+
+// backward: past a wave one chunk per thread and as many threads as the row needs -- a thread holds 2 kVec column sums per chunk, and what
+// bounds the kernel is how many loads are in flight.  `most`: workgroups, each with a partial sum to write: as many as are resident.
+// us for 16-bit rows, x, dy and dx 402 MB: 2048 columns 105, 4096 columns 106 (two chunks on 256 threads: 112 .. 150), 8192 columns
+// 118 (four chunks on 256: 220 .. 250); 1024 columns, two chunks a lane, 98 with 768 workgroups and 133 with 1024.
+Shape bwd_shape(long cols, int vec, long& most) {
+    Shape s = shape_of(cols, vec);
+    most = s.chunks == 2 && vec == 8 ? 768 : 1024;
+    if (s.block) {
+        const long n = (cols + vec - 1) / vec;
+        s.group = n <= 256 ? 256 : n <= 512 ? 512 : 1024;
+        s.chunks = n <= 1024 ? 1 : 2;
+        most = kBwdThreads / s.group;
+    }
     return s;
 }
 
 long parts_of(long rows, long cols, int vec) {
     if (cols > kInRegisters) {
         const long c = (rows + 63) / 64;
-        return c < kMaxParts / 2 ? c : kMaxParts / 2;
+        return c < 256 ? c : 256;
     }
-    const long high = kThreads / shape_of(cols, vec).group, c = (rows + high - 1) / high;
-    return c < kMaxParts ? c : kMaxParts;
+    long most;
+    const Shape s = bwd_shape(cols, vec, most);
+    const long high = s.block ? 1 : kThreads / s.group, c = (rows + high - 1) / high;
+    return c < most ? c : most;
 }
 
 template <typename T, typename W>
@@ -376,14 +401,15 @@ hipError_t bwd(const NormArgs& a, hipStream_t s) {
         if (a.dx && a.rows > 0) long_dx_kernel<T, W><<<dim3((unsigned)(a.rows < 65536 ? a.rows : 65536)), kThreads, 0, s>>>(a);
         if (sums && parts > 0) long_part_kernel<T><<<dim3((unsigned)((a.cols + 63) / 64), (unsigned)parts), kThreads, 0, s>>>(a, parts);
     } else if (a.rows > 0) {
-        const Shape p = shape_of(a.cols, kVec<T>);
+        long most;
+        const Shape p = bwd_shape(a.cols, kVec<T>, most);
         const dim3 grid((unsigned)parts);
-        if (!p.block && p.chunks == 1) norm_bwd_kernel<T, W, 1, false><<<grid, kThreads, 0, s>>>(a, p.group);
-        else if (!p.block) norm_bwd_kernel<T, W, 2, false><<<grid, kThreads, 0, s>>>(a, p.group);
-        else if (p.chunks == 1) norm_bwd_kernel<T, W, 1, true><<<grid, kThreads, 0, s>>>(a, p.group);
-        else if (p.chunks == 2) norm_bwd_kernel<T, W, 2, true><<<grid, kThreads, 0, s>>>(a, p.group);
-        else if (p.chunks == 4) norm_bwd_kernel<T, W, 4, true><<<grid, kThreads, 0, s>>>(a, p.group);
-        else if constexpr (kVec<T> == 4) norm_bwd_kernel<T, W, 8, true><<<grid, kThreads, 0, s>>>(a, p.group);
+        if (!p.block && p.chunks == 1) norm_bwd_kernel<T, W, 1, 0><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (!p.block) norm_bwd_kernel<T, W, 2, 0><<<grid, kThreads, 0, s>>>(a, p.group);
+        else if (p.group == 256) norm_bwd_kernel<T, W, 1, 256><<<grid, 256, 0, s>>>(a, p.group);
+        else if (p.group == 512) norm_bwd_kernel<T, W, 1, 512><<<grid, 512, 0, s>>>(a, p.group);
+        else if (p.chunks == 1) norm_bwd_kernel<T, W, 1, 1024><<<grid, 1024, 0, s>>>(a, p.group);
+        else if constexpr (kVec<T> == 4) norm_bwd_kernel<T, W, 2, 1024><<<grid, 1024, 0, s>>>(a, p.group);
     }
     if (sums) norm_cols_kernel<W><<<dim3((unsigned)((a.cols + 31) / 32), 2), kSumThreads, 0, s>>>(a, parts);
     return hipGetLastError();
