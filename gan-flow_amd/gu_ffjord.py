@@ -13,6 +13,7 @@ import torch
 
 from .gu import make_gu
 from .lib.layers import CNF, MovingBatchNorm1d, ODEfunc, ODEnet, SequentialFlow
+from .lib.optim import MuonWithAdam
 from .util import count_parameters, get_logger, makedirs, w_distance
 
 
@@ -185,10 +186,14 @@ class FusedTrainStep:
     are updated in place through ODEnet.flatten_parameters(), so `model` (state_dict, evaluation) always sees the
     trained weights.  As in the reference, `sqrt_end_time` receives no gradient (T enters the solve detached).
     With graph=True the iteration is captured once and replayed as one hipGraph; the solver status words stay on the
-    device until .check()."""
+    device until .check().
+
+    optimizer="muon": the weights from hidden to hidden layers are updated by cnf_muon_step (all blocks' in one set of launches, guarded
+    by the last adjoint solve: a failed iteration leaves them alone), everything else by cnf_adam_step as before -- the
+    arithmetic of lib.optim.MuonWithAdam.  `muon`: its arguments, as in lib.optim.Muon."""
 
     def __init__(self, model, example_batch, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.0, graph=True,
-                 warmup_batches=(), spread=True, fuse_tail=True, sampler=None, warmup=0, reg_coeffs=None):
+                 warmup_batches=(), spread=True, fuse_tail=True, sampler=None, warmup=0, reg_coeffs=None, optimizer="adam", muon=None):
         # sampler: a gu.DeviceSampler (or anything with .fill(tensor)): every iteration starts by drawing its batch on the
         # device straight into the static input (one more kernel in the captured graph, no host sampler, no copy) and
         # step() takes no argument; `warmup` such iterations run before the capture (warmup_batches is for fed batches)
@@ -197,8 +202,12 @@ class FusedTrainStep:
             raise ValueError("with a device sampler the warm-up iterations draw their own batches: pass warmup=N")
         if sampler is not None:
             warmup_batches = [None] * int(warmup)
-        # fuse_tail: use cnf_solve_bwd_train (same arithmetic, fewer kernels) where it is built
-        self.fuse_tail = bool(fuse_tail)
+        if optimizer not in ("adam", "muon"):
+            raise ValueError("optimizer must be 'adam' or 'muon' (got %r)" % (optimizer,))
+        if muon is not None and optimizer != "muon":
+            raise ValueError("muon= holds the arguments of optimizer='muon'")
+        # fuse_tail: use cnf_solve_bwd_train (same arithmetic, fewer kernels) where it is built (its epilogue is Adam's)
+        self.fuse_tail = bool(fuse_tail) and optimizer == "adam"
         # spread: flag the adjoint solves CNF_FLAG_SPREAD (include/cnf_hip.h): two workgroups per 16-row tile when the
         # batch would leave half the compute units idle.  Same results; must be False for trials that share a GPU
         # (ConcurrentTrials), whose solves have to be resident side by side.
@@ -226,7 +235,28 @@ class FusedTrainStep:
         self.exp_avg = [torch.zeros_like(f) for f in self.flats]
         self.exp_avg_sq = [torch.zeros_like(f) for f in self.flats]
         dev = example_batch.device
+        self.muon = None
+        # the stretches of each flat vector that Adam updates, each with its step count: one, or what lies between the hidden matrices
+        self.stretches = [[(0, f.numel())] for f in self.flats]
+        if optimizer == "muon":
+            from .lib.optim import Muon, adjusted_scale
+            groups = Muon([p for net in self.nets for p in self._hidden(net)], **dict(muon or {})).param_groups[0]   # (checks the arguments)
+            self.muon = {k: groups[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "eps")}
+            self.muon.update(steps=groups["ns_steps"], coefficients=groups["ns_coefficients"])
+            self.muon_params, self.muon_views, self.muon_scales = [], [], []
+            for i, net in enumerate(self.nets):
+                cuts = [0]
+                for p in self._hidden(net):
+                    off, hk = p.storage_offset(), net.kernel_hidden()      # (a view of the flat vector: flatten_parameters)
+                    cuts += [off, off + hk * hk]
+                    self.muon_params.append(p.detach())
+                    self.muon_views.append((i, p.shape, p.stride(), off))
+                    self.muon_scales.append(adjusted_scale(groups["adjust_lr"], *p.shape))
+                cuts.append(self.flats[i].numel())
+                self.stretches[i] = [(a, b) for a, b in zip(cuts[::2], cuts[1::2]) if b > a]
+            self.momenta = [torch.zeros(p.shape, dtype=torch.float32, device=dev) for p in self.muon_params]
         self.adam_state = [torch.zeros(2, dtype=torch.int32, device=dev) for _ in self.flats]
+        self.more_states = [[torch.zeros(2, dtype=torch.int32, device=dev) for _ in s[1:]] for s in self.stretches]
         self.stats = torch.zeros(len(self.blocks), 2, 8, dtype=torch.int32, device=dev)   # [block][fwd, bwd][CnfStats words]
         # a workspace of its own, zero-initialised and only ever used by CNF_FLAG_CLEAN calls: the solves enqueue no memsets
         need = max(_native.workspace_bytes(_inner(blk.odefunc).net_desc(), example_batch.shape[0]) for blk in self.blocks)
@@ -269,11 +299,29 @@ class FusedTrainStep:
 
     def _dry_run(self):
         """A forward + adjoint solve that changes nothing (sizes the cached workspace before capture)."""
-        saved = [f.clone() for f in self.flats], [s.clone() for s in self.adam_state]
-        m, v = [t.clone() for t in self.exp_avg], [t.clone() for t in self.exp_avg_sq]
+        state = self.flats + self.exp_avg + self.exp_avg_sq + self.adam_state + sum(self.more_states, []) + (self.momenta if self.muon else [])
+        saved = [t.clone() for t in state]
         self._iteration()
-        for dst, src in zip(self.flats + self.adam_state + self.exp_avg + self.exp_avg_sq, saved[0] + saved[1] + m + v):
+        for dst, src in zip(state, saved):
             dst.copy_(src)
+
+    @staticmethod
+    def _hidden(net):
+        """The weights from hidden to hidden layers."""
+        return [layer._layer.weight for layer in list(net.layers)[1:-1]]
+
+    def _adam(self, i, grad, guard):
+        for (a, b), state in zip(self.stretches[i], [self.adam_state[i]] + self.more_states[i]):
+            self._native.adam_step(self.flats[i][a:b], grad[a:b], self.exp_avg[i][a:b], self.exp_avg_sq[i][a:b], state, guard=guard, **self.hyper)
+
+    def _muon(self, grads, guard):
+        """The hidden matrices of all blocks from their places in the blocks' flat gradients."""
+        from .lib.optim import muon_step
+        by_scale = {}
+        for p, m, (i, shape, stride, off), scale in zip(self.muon_params, self.momenta, self.muon_views, self.muon_scales):
+            by_scale.setdefault(scale, []).append((p, grads[i].as_strided(shape, stride, off), m))
+        for scale, members in by_scale.items():
+            muon_step(*zip(*members), scale=scale, guard=guard, **self.muon)
 
     def _iteration(self):
         nat = self._native
@@ -307,6 +355,7 @@ class FusedTrainStep:
         fused = [self.fuse_tail and tape[i][0].hidden == 64 and z.shape[0] <= 4096 and not (fixed[i] and tape[i][0].dim > 2)
                  and tape[i][7] is None for i in range(last + 1)]
         loss = gz = gl = None
+        grads = [None] * len(self.blocks)
         if not fused[last] or fixed[last]:
             loss, gz, gl = nat.nll_loss(z, lp)
         for i in range(last, -1, -1):
@@ -315,7 +364,8 @@ class FusedTrainStep:
             if regd is not None:
                 gz, gl, gp, prev = nat.solve_bwd_reg(net, regd[0], self.flats[i], z1, lp1, regd[1], gz, gl, self.reg_coeffs, t0, t1, opts, e,
                                                      stats=self.stats[i, 1])
-                nat.adam_step(self.flats[i], gp, self.exp_avg[i], self.exp_avg_sq[i], self.adam_state[i], guard=prev, **self.hyper)
+                self._adam(i, gp, prev)
+                grads[i] = gp
             elif fused[i]:
                 gz, gl, _, l_, prev = nat.solve_bwd_train(net, self.flats[i], z1, lp1, gz, gl, t0, t1, opts, self.exp_avg[i],
                                                           self.exp_avg_sq[i], self.adam_state[i], e, stats=self.stats[i, 1],
@@ -324,9 +374,12 @@ class FusedTrainStep:
             else:
                 gz, gl, gp, prev = nat.solve_bwd(net, self.flats[i], z1, lp1, gz, gl, t0, t1, opts, e, stats=self.stats[i, 1],
                                                  workspace=self.workspace)
-                nat.adam_step(self.flats[i], gp, self.exp_avg[i], self.exp_avg_sq[i], self.adam_state[i], guard=prev, **self.hyper)
+                self._adam(i, gp, prev)
+                grads[i] = gp
             if self.consts[i] is not None:
                 self.flats[i].index_copy_(0, *self.consts[i])
+        if self.muon:
+            self._muon(grads, prev)
         for term in reg_terms:
             loss = loss + term
         return loss
@@ -367,11 +420,22 @@ class FusedTrainStep:
         return int(self.adam_state[0][0].item())
 
     def state_dict(self):
-        """Optimizer state (Adam moments and step counts per block) for checkpoint / resume."""
-        return {"exp_avg": [t.clone() for t in self.exp_avg], "exp_avg_sq": [t.clone() for t in self.exp_avg_sq],
-                "step": [int(s[0].item()) for s in self.adam_state], "hyper": dict(self.hyper)}
+        """Optimizer state (Adam moments and step counts per block, Muon's momenta) for checkpoint / resume."""
+        out = {"exp_avg": [t.clone() for t in self.exp_avg], "exp_avg_sq": [t.clone() for t in self.exp_avg_sq],
+               "step": [int(s[0].item()) for s in self.adam_state], "hyper": dict(self.hyper)}
+        if self.muon:
+            out["momenta"] = [t.clone() for t in self.momenta]
+        return out
 
     def load_state_dict(self, state):
+        if ("momenta" in state) != bool(self.muon):
+            raise ValueError("the state is another optimizer's (Muon's momenta are %s)" % ("missing" if self.muon else "not wanted"))
+        if self.muon:
+            for dst, src in zip(self.momenta, state["momenta"]):
+                dst.copy_(src)
+        for more, n in zip(self.more_states, state["step"]):
+            for s in more:
+                s.copy_(torch.tensor([int(n), 0], dtype=torch.int32))
         for dst, src in zip(self.exp_avg + self.exp_avg_sq, list(state["exp_avg"]) + list(state["exp_avg_sq"])):
             dst.copy_(src)
         for s, n in zip(self.adam_state, state["step"]):
@@ -490,6 +554,11 @@ def parse_args(argv=None):
     p.add_argument("--log_interval", type=int, default=1000)
     p.add_argument("--lr", type=float, default=1e-3)
     p.add_argument("--weight_decay", type=float, default=1e-5)
+    p.add_argument("--optimizer", type=str, default="adam", choices=["adam", "muon"], help="muon: the hidden matrices by Muon (lib/optim.py), "
+                   "everything else by Adam (not in the reference)")
+    p.add_argument("--muon_lr", type=float, default=0.02)
+    p.add_argument("--muon_momentum", type=float, default=0.95)
+    p.add_argument("--muon_weight_decay", type=float, default=0.0)
     p.add_argument("--dims", type=str, default="64-64-64")
     p.add_argument("--num_blocks", type=int, default=1)
     p.add_argument("--layer_type", type=str, default="concatsquash",
@@ -574,16 +643,19 @@ def main(argv=None):
                 block.solver_options["step_size"] = args.step_size
     logger.info("parameters: %d" % count_parameters(model))
     model.train()
+    muon = dict(lr=args.muon_lr, momentum=args.muon_momentum, weight_decay=args.muon_weight_decay)
+    step_args = dict(optimizer="muon", muon=muon) if args.optimizer == "muon" else {}
     fused = optimizer = graphed = None
     on_device = data.device_sampler(device) if args.device_sampler else None
     train_sampler = on_device if (args.fused and on_device is not None) else None
     if args.fused:
         x = data.get_sample(args.batch_size).to(device)
-        fused = FusedTrainStep(model, x, lr=args.lr, weight_decay=args.weight_decay, sampler=train_sampler, reg_coeffs=reg_coeffs or None)
+        fused = FusedTrainStep(model, x, lr=args.lr, weight_decay=args.weight_decay, sampler=train_sampler, reg_coeffs=reg_coeffs or None,
+                               **step_args)
     else:
         graphed_ok = bool(args.graphed) and not args.batch_norm and not args.resume
-        optimizer = torch.optim.Adam(model.parameters(), lr=args.lr, weight_decay=args.weight_decay,
-                                     **(dict(capturable=True) if graphed_ok else dict(fused=True)))
+        adam = dict(lr=args.lr, weight_decay=args.weight_decay, **(dict(capturable=True) if graphed_ok else dict(fused=True)))
+        optimizer = MuonWithAdam(model, muon, adam) if args.optimizer == "muon" else torch.optim.Adam(model.parameters(), **adam)
         for block in model.chain:          # one training per GPU: the adjoint may use both halves of the chip
             if isinstance(block, CNF):
                 block.spread_adjoint = True
@@ -604,7 +676,7 @@ def main(argv=None):
             train_sampler = on_device if args.fused else None
         if fused is not None:
             fused = FusedTrainStep(model, x, lr=args.lr, weight_decay=args.weight_decay, sampler=train_sampler,
-                                   reg_coeffs=reg_coeffs or None)   # parameters were re-assigned: re-alias
+                                   reg_coeffs=reg_coeffs or None, **step_args)   # parameters were re-assigned: re-alias
             fused.load_state_dict(ck["optimizer"])
         else:
             optimizer.load_state_dict(ck["optimizer"])

@@ -131,7 +131,7 @@ class Muon(torch.optim.Optimizer):
                 if p.grad.is_sparse:
                     raise _native.CnfError("Muon does not take sparse gradients")
                 state = self.state[p]
-                if not state:
+                if "momentum_buffer" not in state:
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 by_shape.setdefault(p.shape, []).append((p, p.grad, state["momentum_buffer"]))
             for shape, members in by_shape.items():
@@ -139,4 +139,42 @@ class Muon(torch.optim.Optimizer):
                 muon_step(ps, gs, ms, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
                           weight_decay=group["weight_decay"], scale=adjusted_scale(group["adjust_lr"], *shape), steps=group["ns_steps"],
                           coefficients=group["ns_coefficients"], eps=group["eps"])
+                torch.autograd.graph.increment_version(ps)   # (written through raw pointers: autograd is told)
         return loss
+
+
+class MuonWithAdam:
+    """Muon for the hidden matrices of the ODE nets of a flow (the weights from hidden to hidden layers), torch.optim.Adam for every other
+    parameter: first and last layers, biases, time terms, end times.  `muon`, `adam`: the arguments of the two.  Behaves as an
+    optimizer where gu_ffjord's training loops need one (zero_grad, step, state_dict, load_state_dict)."""
+
+    def __init__(self, model, muon=None, adam=None):
+        hidden = hidden_matrices(model)
+        taken = {id(p) for p in hidden}
+        self.muon = Muon(hidden, **dict(muon or {}))
+        self.adam = torch.optim.Adam([p for p in model.parameters() if id(p) not in taken], **dict(adam or {}))
+
+    def zero_grad(self, set_to_none=True):
+        self.muon.zero_grad(set_to_none)
+        self.adam.zero_grad(set_to_none)
+
+    def step(self):
+        self.muon.step()
+        self.adam.step()
+
+    def state_dict(self):
+        return {"muon": self.muon.state_dict(), "adam": self.adam.state_dict()}
+
+    def load_state_dict(self, state):
+        self.muon.load_state_dict(state["muon"])
+        self.adam.load_state_dict(state["adam"])
+
+
+def hidden_matrices(model):
+    """The weights from hidden to hidden layers of every ODE net of a flow, in the order of its blocks."""
+    from .layers.cnf import CNF, _inner
+    out = []
+    for blk in model.chain:
+        if isinstance(blk, CNF):
+            out += [layer._layer.weight for layer in list(_inner(blk.odefunc).diffeq.layers)[1:-1]]
+    return out
