@@ -713,35 +713,35 @@ def ns_params(steps, coefficients, eps):
 
 
 def _stack(t, name, dtype):
-    """Pointer array and row stride of a (count, rows, cols) tensor, or of a list of matrices of one shape, device and stride, with
-    contiguous rows that do not overlap."""
+    """(pointer array, row stride, (count, rows, cols), device) of a (count, rows, cols) tensor, or of a list of matrices of one shape,
+    device and stride, with contiguous rows that do not overlap."""
     if torch.is_tensor(t):
         _elem(t, name, (dtype,))
         n, rows, cols = t.shape
         one, ld, inner = t.stride()
-        base, step = t.data_ptr(), one * t.element_size()
+        base, step, dev = t.data_ptr(), one * t.element_size(), t.device
         ptrs = (ctypes.c_void_p * n)(*[base + i * step for i in range(n)])
     else:
-        t0 = t[0]
+        t0, n = t[0], len(t)
         shape, strides, dev = t0.shape, t0.stride(), t0.device
+        if len(shape) != 2:
+            raise CnfError("%s: matrices are wanted (got shape %s)" % (name, tuple(shape)))
         for m in t:
             _elem(m, name, (dtype,))
             if m.shape != shape or m.stride() != strides or m.device != dev:
                 raise CnfError("%s: matrices of one shape, device and stride are wanted" % name)
-        if len(shape) != 2:
-            raise CnfError("%s: matrices are wanted (got shape %s)" % (name, tuple(shape)))
         rows, cols = shape
         ld, inner = strides
-        ptrs = (ctypes.c_void_p * len(t))(*[m.data_ptr() for m in t])
+        ptrs = (ctypes.c_void_p * n)(*[m.data_ptr() for m in t])
     if cols > 1 and inner != 1:
         raise CnfError("%s: rows must be contiguous (strides %s)" % (name, (ld, inner)))
     if rows > 1 and ld < cols:
         raise CnfError("%s: rows overlap (strides %s)" % (name, (ld, inner)))
-    return ptrs, ld if rows > 1 else cols
+    return ptrs, ld if rows > 1 else cols, (n, rows, cols), dev
 
 
-def _shape_of(t):
-    return (len(t),) + tuple(t[0].shape[-2:])
+def _dtype_of(ts):
+    return ts.dtype if torch.is_tensor(ts) else ts[0].dtype
 
 
 def matrix_workspace_bytes(count, rows, cols):
@@ -753,19 +753,20 @@ def orthogonalize(gs, outs, ns):
     """cnf_orthogonalize: writes the orthogonalised matrices of `gs` (a (count, rows, cols) tensor, or a list of matrices of one shape and
     stride; at most MAX_MATRICES) to those of `outs`."""
     lib = load_library()
-    g0 = gs[0]
-    dt, dev = g0.dtype, g0.device
-    _elem(g0, "g")
-    g, ldg = _stack(gs, "g", dt)
-    out, ldo = _stack(outs, "out", dt)
-    count, rows, cols = shape = _shape_of(gs)
-    if _shape_of(outs) != shape or outs[0].device != dev:
-        raise CnfError("out must have g's shape %s and device (got %s on %s)" % (shape, _shape_of(outs), outs[0].device))
+    dt = _dtype_of(gs)
+    if dt not in DTYPE_IDS:
+        raise CnfError("g must be %s (got %s)" % (" or ".join(str(d) for d in DTYPE_IDS), dt))
+    g, ldg, shape, dev = _stack(gs, "g", dt)
+    out, ldo, oshape, odev = _stack(outs, "out", dt)
+    if oshape != shape or odev != dev:
+        raise CnfError("out must have g's shape %s and device (got %s on %s)" % (shape, oshape, odev))
+    count, rows, cols = shape
     need = lib.cnf_orthogonalize_workspace_bytes(count, rows, cols)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     with _at(dev) as stream:
         rc = lib.cnf_orthogonalize(g, ldg, out, ldo, DTYPE_IDS[dt], count, rows, cols, ctypes.byref(ns), ws.data_ptr(), need, stream)
-    _check(rc, lib)
+    if rc:
+        _check(rc, lib)
     return outs
 
 
@@ -773,23 +774,24 @@ def muon_step(params, grads, momenta, ns, lr=1e-3, momentum=0.95, nesterov=True,
     """cnf_muon_step: one Muon update, in place, of the matrices `params` (as in orthogonalize) from `grads` (of their type) with the fp32
     momenta.  guard: stats words as in adam_step."""
     lib = load_library()
-    p0 = params[0]
-    dt, dev = p0.dtype, p0.device
-    _elem(p0, "params")
-    p, ldp = _stack(params, "params", dt)
-    g, ldg = _stack(grads, "grads", dt)
-    m, ldm = _stack(momenta, "momenta", torch.float32)
-    count, rows, cols = shape = _shape_of(params)
-    for name, t in (("grads", grads), ("momenta", momenta)):
-        if _shape_of(t) != shape or t[0].device != dev:
-            raise CnfError("%s must have the parameters' shape %s and device (got %s on %s)" % (name, shape, _shape_of(t), t[0].device))
+    dt = _dtype_of(params)
+    if dt not in DTYPE_IDS:
+        raise CnfError("params must be %s (got %s)" % (" or ".join(str(d) for d in DTYPE_IDS), dt))
+    p, ldp, shape, dev = _stack(params, "params", dt)
+    g, ldg, gshape, gdev = _stack(grads, "grads", dt)
+    m, ldm, mshape, mdev = _stack(momenta, "momenta", torch.float32)
+    if gshape != shape or mshape != shape or gdev != dev or mdev != dev:
+        raise CnfError("grads and momenta must have the parameters' shape %s and device (got %s on %s, %s on %s)"
+                       % (shape, gshape, gdev, mshape, mdev))
+    count, rows, cols = shape
     o = CnfMuonOpts(lr, momentum, weight_decay, scale, 1 if nesterov else 0, 0)
     need = lib.cnf_orthogonalize_workspace_bytes(count, rows, cols)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     with _at(dev) as stream:
         rc = lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[dt], count, rows, cols, ctypes.byref(o), ctypes.byref(ns),
                                _stats_ptr(guard), ws.data_ptr(), need, stream)
-    _check(rc, lib)
+    if rc:
+        _check(rc, lib)
 
 
 def gu_desc(mean, sigma, unif_intsect, unif_p, extend_dim):

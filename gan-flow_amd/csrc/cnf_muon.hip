@@ -59,13 +59,25 @@ __device__ __forceinline__ long piece_at(long r, long c, long kc) {
     return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ ((r >> 1) & 7)) << 4) + ((c & 7) << 1);
 }
 
-// The value is settled before it is split: the compiler otherwise folds the operation that makes v into one of the two conversions
-// (fp32 arithmetic with an fp16 result, rounded once), and a hi from the unrounded value beside a lo from the rounded one is a
-// whole fp16 step off where the two round differently.
-__device__ __forceinline__ void split(float v, f16& hi, f16& lo) {
-    asm("" : "+v"(v));
-    hi = (f16)v;
-    lo = (f16)(v - (float)hi);
+// The pieces of two values.  The values are settled before they are split: the compiler otherwise folds the operation that makes one into one
+// of its conversions (fp32 arithmetic with an fp16 result, rounded once), and a hi from the unrounded value beside a lo from the
+// rounded one is a whole fp16 step off where the two round differently.
+typedef float float2v __attribute__((ext_vector_type(2)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ void split2(float v0, float v1, half2& hi, half2& lo) {
+    asm("" : "+v"(v0), "+v"(v1));
+    hi = __builtin_convertvector((float2v){v0, v1}, half2);
+    // v - hi is exact; as a multiply-add it reads hi's halves without converting them first
+    lo = __builtin_convertvector((float2v){__builtin_fmaf(-1.f, (float)hi[0], v0), __builtin_fmaf(-1.f, (float)hi[1], v1)}, half2);
+}
+
+__device__ __forceinline__ void split4(const float (&v)[4], half4& hi, half4& lo) {
+    half2 h0, l0, h1, l1;
+    split2(v[0], v[1], h0, l0);
+    split2(v[2], v[3], h1, l1);
+    hi = __builtin_shufflevector(h0, h1, 0, 1, 2, 3);
+    lo = __builtin_shufflevector(l0, l1, 0, 1, 2, 3);
 }
 
 // four neighbouring elements of a row, or the last ones of it
@@ -135,44 +147,46 @@ __device__ __forceinline__ double start_scale(double norm, double eps, float& f)
     return (double)kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
 }
 
-// X0 = G / (|G| + eps) as the piece matrices X (m x n) and X^T (n x m); one 64 x 64 tile of G per workgroup, through LDS
-template <typename T, bool kMuon>
+// X0 = G / (|G| + eps) as the piece matrices X (m x n) and X^T (n x m); one 64 x 64 tile of G per workgroup, through LDS.  Thread (tr, tc)
+// loads columns 4 tc .. of rows tr, tr + 16, ..; what is outside G is read at its last row and not used.
+template <typename T, bool kMuon, bool kVec>
 __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* x, char* xt, const double* part, int parts, double eps, float mu,
                                                           int nesterov, Steps st, float* factors) {
-    __shared__ float tile[64][65];
-    __shared__ double scale;     // (double: the largest and smallest fp32 gradients have a scale outside fp32)
-    const int mat = blockIdx.z;
-    if (threadIdx.x < 64) {
-        double s = 0.;
-        for (int k = threadIdx.x; k < parts; k += 64) s += part[mat * kNormBlocks + k];
-        for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        if (threadIdx.x == 0) {
-            float f;
-            scale = start_scale(sqrt(s), eps, f);
-            if (blockIdx.x == 0 && blockIdx.y == 0) {
-                for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
-                    factors[mat * (CNF_NS_MAX_STEPS + 1) + k] = f;
-                    if (k < st.n) f = fminf(1.f, f * st.grow[k]);
-                }
-            }
+    __shared__ float tile[64][68];
+    __shared__ double red[kThreads / 64];
+    const int mat = blockIdx.z, tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
+    const T* g = (const T*)p.g[mat];
+    const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 64, c = c0 + tc;
+    const long left = d.cols - c;                            // columns from here on
+    float v[4][4], m[4][4];
+    for (int i = 0; i < 4; ++i) {
+        const long r = min(r0 + tr + i * 16, d.rows - 1);
+        for (int k = 0; k < 4; ++k) v[i][k] = m[i][k] = 0.f;
+        if (left > 0) {
+            load4<T, kVec>(g + r * d.ldg + c, left, v[i]);
+            if (kMuon) load4<float, kVec>(p.m[mat] + r * d.ldm + c, left, m[i]);      // the new momentum
         }
     }
-    const T* g = (const T*)p.g[mat];
-    const long r0 = (long)blockIdx.y * 64, c0 = (long)blockIdx.x * 64;
+    double s = 0.;
+    for (int k = threadIdx.x; k < parts; k += kThreads) s += part[mat * kNormBlocks + k];
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
     __syncthreads();
-    for (int e = threadIdx.x; e < 4096; e += kThreads) {
-        const int i = e >> 6, j = e & 63;
-        const long r = r0 + i, c = c0 + j;
-        float v = 0.f;
-        if (r < d.rows && c < d.cols) {
-            v = to_f32(g[r * d.ldg + c]);
-            if (kMuon) {
-                const float mv = p.m[mat][r * d.ldm + c];     // the new momentum
-                v = nesterov ? fmaf(mu, mv, v) : mv;
-            }
-            v = (float)((double)v * scale);
+    float f;
+    // (double: the largest and smallest fp32 gradients have a scale outside fp32)
+    const double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
+    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
+        for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
+            factors[mat * (CNF_NS_MAX_STEPS + 1) + k] = f;
+            if (k < st.n) f = fminf(1.f, f * st.grow[k]);
         }
-        tile[i][j] = v;
+    for (int i = 0; i < 4; ++i) {
+        const bool in = r0 + tr + i * 16 < d.rows;
+        for (int k = 0; k < 4; ++k) {
+            const float u = kMuon ? (nesterov ? fmaf(mu, m[i][k], v[i][k]) : m[i][k]) : v[i][k];
+            v[i][k] = in ? (float)((double)u * scale) : 0.f;
+        }
+        *(float4*)&tile[tr + i * 16][tc] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
     }
     __syncthreads();
     // (rows, cols) as they are, then transposed; X gets the one whose rows are the shorter side
@@ -181,17 +195,15 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
     const long kc_s = (d.tall ? d.mp : d.np) >> 5, kc_f = (d.tall ? d.np : d.mp) >> 5;
     for (int e = threadIdx.x; e < 1024; e += kThreads) {
         const int i = (e & 511) >> 3, q = (e & 7) * 8;
-        half8 hi, lo;
-        for (int k = 0; k < 8; ++k) {
-            f16 h, l;
-            split(e < 512 ? tile[i][q + k] : tile[q + k][i], h, l);
-            hi[k] = h;
-            lo[k] = l;
-        }
+        float w[8];
+        for (int k = 0; k < 8; ++k) w[k] = e < 512 ? tile[i][q + k] : tile[q + k][i];
+        half4 h0, l0, h1, l1;
+        split4({w[0], w[1], w[2], w[3]}, h0, l0);
+        split4({w[4], w[5], w[6], w[7]}, h1, l1);
         char* base = e < 512 ? straight : flipped;
         const long at = e < 512 ? piece_at(r0 + i, c0 + q, kc_s) : piece_at(c0 + i, r0 + q, kc_f);
-        *(half8*)(base + at) = hi;
-        *(half8*)(base + (at ^ 64)) = lo;
+        *(half8*)(base + at) = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+        *(half8*)(base + (at ^ 64)) = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
 
@@ -349,18 +361,20 @@ __device__ __forceinline__ void finish(const ArgsOf<kMode>& a, int mat, float sc
         }
         unsigned* t = (unsigned*)lds;                        // (hi, lo) of element (r, c) at r * 36 + c
         for (int g = 0; g < 4; ++g) {
-            unsigned word[4];
+            float val[4];
             for (int e = 0; e < 4; ++e) {
-                float val = acc[g * 4 + e] * scale;
+                val[e] = acc[g * 4 + e] * scale;
                 if (kMode == kPoly) {
-                    val = fmaf(a.cc, val, a.cb * ((float)old_h[g][e] + (float)old_l[g][e]));
-                    val += r0 + row == c0 + g * 8 + half * 4 + e && r0 + row < a.m ? a.ca * kScale : 0.f;
+                    val[e] = fmaf(a.cc, val[e], a.cb * ((float)old_h[g][e] + (float)old_l[g][e]));
+                    val[e] += r0 + row == c0 + g * 8 + half * 4 + e && r0 + row < a.m ? a.ca * kScale : 0.f;
                 }
-                union { f16 e[2]; unsigned w; } both;
-                split(val, both.e[0], both.e[1]);
-                word[e] = both.w;
             }
-            *(uint4*)(t + row * 36 + g * 8 + half * 4) = make_uint4(word[0], word[1], word[2], word[3]);
+            half4 h, l;
+            split4(val, h, l);
+            union { half4 v; unsigned w[2]; } hi = {h}, lo = {l};
+            *(uint4*)(t + row * 36 + g * 8 + half * 4) =
+                make_uint4(__builtin_amdgcn_perm(lo.w[0], hi.w[0], 0x05040100u), __builtin_amdgcn_perm(lo.w[0], hi.w[0], 0x07060302u),
+                           __builtin_amdgcn_perm(lo.w[1], hi.w[1], 0x05040100u), __builtin_amdgcn_perm(lo.w[1], hi.w[1], 0x07060302u));
         }
         auto pack = [&](const unsigned (&w)[8], unsigned part) {
             return make_uint4(__builtin_amdgcn_perm(w[1], w[0], part), __builtin_amdgcn_perm(w[3], w[2], part),
@@ -619,13 +633,8 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
         for (int k = 0; k < 4; ++k) v[i][k] = (float)((double)v[i][k] * scale);
     for (int i = 0; i < 4; ++i) {
         half4 h, l, ht, lt;
-        for (int k = 0; k < 4; ++k) {
-            f16 hi, lo;
-            split(v[i][k], hi, lo);
-            h[k] = hi, l[k] = lo;
-            split(v[k][i], hi, lo);
-            ht[k] = hi, lt[k] = lo;
-        }
+        split4(v[i], h, l);
+        split4({v[0][i], v[1][i], v[2][i], v[3][i]}, ht, lt);
         const long at = piece_at(tr * 4 + i, tc, 2), att = piece_at(tc + i, tr * 4, 2);
         *(half4*)(straight + at) = h;
         *(half4*)(straight + (at ^ 64)) = l;
@@ -653,11 +662,7 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
     auto store = [&](char* to, char* flip, const float16v& x) {      // pieces of the quadrant, and of its transpose where flip is given
         for (int q = 0; q < 4; ++q) {
             half4 h, l;
-            for (int e = 0; e < 4; ++e) {
-                f16 hi, lo;
-                split(x[q * 4 + e], hi, lo);
-                h[e] = hi, l[e] = lo;
-            }
+            split4({x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]}, h, l);
             const long at = piece_at(row, col + q * 8, 2);
             *(half4*)(to + at) = h;
             *(half4*)(to + (at ^ 64)) = l;
@@ -704,29 +709,12 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
 
 long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 
-struct Plan {
-    long m, n;      // the shorter and the longer side
-    int pm, pn;     // in panels of 64
-    bool small;     // one workgroup per matrix does everything in LDS
-    bool together;  // products of several steps' polynomials before they meet X
-};
-
-Plan plan_of(long rows, long cols) {
-    Plan p{};
-    p.m = rows < cols ? rows : cols;
-    p.n = rows < cols ? cols : rows;
-    p.small = p.n <= 64;
-    p.pm = (int)((p.m + 63) / 64);
-    p.pn = (int)((p.n + 63) / 64);
-    p.together = p.pn >= 2 * p.pm;
-    return p;
-}
-
 // Which kernel computes a product: the one whose estimated time is least.  A round is as many workgroups as run at once; it takes `few` us per 4096
 // of k up to half full and `full` us when full, and `fixed` us whatever k is (its first copies, its results).  Measured on 6 .. 4096 tiles and
 // k = 256 .. 4096; the estimate is within a tenth or two of the measured time and never took a kernel 15 % behind the best.
 struct Choice {
     int tile, split;
+    double time;
 };
 
 Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
@@ -745,9 +733,38 @@ Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
         const long whole = tiles / e.at_once, rest = tiles % e.at_once;
         const double last = rest ? e.few + (e.full - e.few) * std::fmax(0., 2. * rest / e.at_once - 1.) : 0.;
         const double time = (whole * e.full + last) * kc / 128. + (whole + (rest > 0)) * e.fixed;
-        if (time < least) least = time, best = {e.tile, e.split};
+        if (time < least) least = time, best = {e.tile, e.split, time};
     }
     return best;
+}
+
+struct Plan {
+    long m, n;      // the shorter and the longer side
+    int pm, pn;     // in panels of 64
+    bool small;     // one workgroup per matrix does everything in LDS
+    bool together;  // several steps at a time on the m x m side (decided for three steps, from the estimated times of the products)
+};
+
+Plan plan_of(long count, long rows, long cols) {
+    Plan p{};
+    p.m = rows < cols ? rows : cols;
+    p.n = rows < cols ? cols : rows;
+    p.small = p.n <= 64;
+    p.pm = (int)((p.m + 63) / 64);
+    p.pn = (int)((p.n + 63) / 64);
+    const double gram = choose(count, p.pm, p.pm, true, 2 * p.pn).time, sym = choose(count, p.pm, p.pm, true, 2 * p.pm).time,
+                 full = choose(count, p.pm, p.pn, false, 2 * p.pm).time;
+    p.together = gram + 9 * sym + full < 3 * (gram + sym + full);
+    return p;
+}
+
+// how many of the steps from k on to take together: the matrix A <- B A B loses what its small eigenvalues' growth leaves of fp32 (their growth
+// twice, up to 256), and the polynomials' product Q has to stay within the pieces' 64
+int steps_together(const Plan& p, int steps, const double (&grow)[CNF_NS_MAX_STEPS], int k) {
+    int n = 1;
+    double up = std::fmax(1., grow[k]);
+    while (p.together && n < 3 && k + n < steps && up * up <= 256. && up * std::fmax(1., grow[k + n]) <= 48.) up *= std::fmax(1., grow[k + n++]);
+    return n;
 }
 
 template <int kMode, typename O = float, bool kMuon = false>
@@ -782,7 +799,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         st.c[k] = (float)a.ns->c[k];
         st.grow[k] = (float)fmax(1., grow[k]);
     }
-    const Plan pl = plan_of(a.rows, a.cols);
+    const Plan pl = plan_of(a.count, a.rows, a.cols);
     Ptrs p{};
     bool vec_in = a.cols % 4 == 0 && a.ldg % 4 == 0 && (!kMuon || a.ldm % 4 == 0), vec_out = a.ldo % 4 == 0;
     for (int i = 0; i < a.count; ++i) {
@@ -822,8 +839,11 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     else
         begin_kernel<O, kMuon, false><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
     const long rp = d.tall ? d.np : d.mp, cp = d.tall ? d.mp : d.np;
-    pieces_kernel<O, kMuon><<<dim3((unsigned)(cp / 64), (unsigned)(rp / 64), a.count), kThreads, 0, s>>>(p, d, x, xt, part, (int)parts, a.ns->eps,
-                                                                                                         mu, nesterov, st, factors);
+    const dim3 tiles((unsigned)(cp / 64), (unsigned)(rp / 64), a.count);
+    if (vec_in)
+        pieces_kernel<O, kMuon, true><<<tiles, kThreads, 0, s>>>(p, d, x, xt, part, (int)parts, a.ns->eps, mu, nesterov, st, factors);
+    else
+        pieces_kernel<O, kMuon, false><<<tiles, kThreads, 0, s>>>(p, d, x, xt, part, (int)parts, a.ns->eps, mu, nesterov, st, factors);
     const int km = pl.pm * 2, kn = pl.pn * 2;
     // `Q` times X: the steps k .. k + n - 1, to X and X^T, or to the output
     auto apply = [&](char* Q, int k, int n) {
@@ -862,10 +882,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     };
     auto times = [&](const char* p, const char* q, char* to) { symmetric(std::integral_constant<int, kSym>{}, p, q, ab, km, to); };
     for (int k = 0; k < st.n;) {
-        // how many steps to take on the m x m side: see the head of this file
-        int n = 1;
-        float up = st.grow[k];
-        while (pl.together && n < 3 && k + n < st.n && up * up <= 256.f && up * st.grow[k + n] <= 48.f) up *= st.grow[k + n++];
+        const int n = steps_together(pl, st.n, grow, k);
         char *A = sym[0], *B = sym[1], *Q = B;
         gram(k, A);
         poly(k, A, B);
@@ -933,7 +950,7 @@ int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
 }
 
 size_t muon_workspace_bytes(long count, long rows, long cols) {
-    const Plan p = plan_of(rows, cols);
+    const Plan p = plan_of(count, rows, cols);
     if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)
     const size_t m = p.pm * 64, n = p.pn * 64;
     return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + (p.together ? 5 : 2) * m * m) * 4 + (CNF_NS_MAX_STEPS + 1) * sizeof(float));

@@ -32,17 +32,19 @@ def orthogonalize(g, steps=5, coefficients=DEFAULT_COEFFICIENTS, eps=1e-7):
     if g.numel() == 0:
         return out
     rows, cols = g.shape[-2:]
-    g3 = g.detach()
-    if g3.dim() != 3:
-        g3 = g3.reshape(-1, rows, cols)
-    if (cols > 1 and g3.stride(2) != 1) or (rows > 1 and g3.stride(1) < cols):
+    g3, o3 = g, out
+    if g.dim() != 3:
+        g3 = g.reshape(-1, rows, cols)
+        o3 = out.view(-1, rows, cols)
+    if not g3.is_contiguous() and ((cols > 1 and g3.stride(2) != 1) or (rows > 1 and g3.stride(1) < cols)):
         g3 = g3.contiguous()
-    o3 = out if out.dim() == 3 else out.view(g3.shape)
-    n = len(g3)
+    n = g3.shape[0]
     step = _at_once(n, rows, cols)
-    for lo in range(0, n, step):
-        whole = step == n
-        _native.orthogonalize(g3 if whole else g3[lo:lo + step], o3 if whole else o3[lo:lo + step], ns)
+    if step == n:
+        _native.orthogonalize(g3, o3, ns)
+    else:
+        for lo in range(0, n, step):
+            _native.orthogonalize(g3[lo:lo + step], o3[lo:lo + step], ns)
     return out
 
 
@@ -55,23 +57,23 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
     if not len(params) == len(grads) == len(momenta):
         raise _native.CnfError("%d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
     ns = _native.ns_params(steps, coefficients, eps)
-    groups, seen = {}, set()
+    groups, seen, given = {}, set(), 0
     for p, g, m in zip(params, grads, momenta):
         for name, t in (("params", p), ("grads", g), ("momenta", m)):
-            _native._elem(t, name)
-            if t.dim() != 2:
+            if not torch.is_tensor(t) or not t.is_cuda or t.dim() != 2:
+                _native._elem(t, name)
                 raise _native.CnfError("%s: Muon updates matrices (got shape %s)" % (name, tuple(t.shape)))
         if p.numel() == 0:
             continue
-        gs = g.stride()
-        if g.shape[1] > 1 and gs[1] != 1 or g.shape[0] > 1 and gs[0] < g.shape[1]:
+        gs, (rows, cols) = g.stride(), g.shape
+        if cols > 1 and gs[1] != 1 or rows > 1 and gs[0] < cols:
             g = g.contiguous()
             gs = g.stride()
-        for address in (p.data_ptr(), m.data_ptr()):
-            if address in seen:
-                raise _native.CnfError("the same parameter or momentum is given twice")
-            seen.add(address)
+        seen.update((p.data_ptr(), m.data_ptr()))
+        given += 2
         groups.setdefault((p.shape, p.dtype, p.device, p.stride(), gs, m.stride()), []).append((p, g, m))
+    if len(seen) != given:
+        raise _native.CnfError("the same parameter or momentum is given twice")
     for key, members in groups.items():
         step = _at_once(len(members), *key[0])
         for lo in range(0, len(members), step):
