@@ -408,23 +408,22 @@ __device__ __forceinline__ float scale_of(const ArgsOf<kMode>& a, int mat) {
     return kInvScale * (kMode == kGram ? f[0] * f[0] : kMode == kApply ? f[0] / f[a.ahead] : f[0] * kInvScale);
 }
 
-// 64 x 64 tiles.  Each of kW waves computes the whole tile over every kW-th block of k -- a wave copies its own operands to its own part of
-// LDS, so nothing but its own counters holds it up -- and the partial sums are added at the end, in a fixed order.
-template <int kW, int kMode, typename O = float, bool kMuon = false>
-__global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
+// 64 x 64 tiles of many products, a wave each: it copies its own operands, so nothing but its own counters holds it up.
+template <int kMode, typename O = float, bool kMuon = false>
+__global__ __launch_bounds__(64) void tile64_kernel(ArgsOf<kMode> a) {
     constexpr int kStages = 2, kStage = 2 * 64 * 128, kLoads = kStage / 1024;
-    __shared__ __align__(16) char lds[kW][kStages][kStage];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __shared__ __align__(16) char lds[kStages][kStage];
+    const int lane = threadIdx.x;
     int mat, ti, tj;
     my_tile(a.panels_p, a.panels_q, kSymmetric<kMode>, mat, ti, tj);
-    const char* ps = a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes + lane * 16;
-    const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes + lane * 16;
-    const int stages = (a.kc - wave + kW - 1) / kW;          // of this wave: blocks wave, wave + kW, ..
+    const char* ps = a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes;
+    const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes;
+    const int stages = a.kc;
     auto load = [&](int s) {
-        const long off = (long)(s * kW + wave) * kBlockBytes;
+        const long off = (long)s * kBlockBytes;
         for (int i = 0; i < kLoads / 2; ++i) {
-            __builtin_amdgcn_global_load_lds((gptr)(ps + off + i * 1024), (lptr)(&lds[wave][s % kStages][i * 1024]), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr)(qs + off + i * 1024), (lptr)(&lds[wave][s % kStages][8192 + i * 1024]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)(ps + off + i * 1024 + lane * 16), (lptr)(&lds[s % kStages][i * 1024]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)(qs + off + i * 1024 + lane * 16), (lptr)(&lds[s % kStages][8192 + i * 1024]), 16, 0, 0);
         }
     };
     float16v acc[2][2] = {};
@@ -433,7 +432,7 @@ __global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
     int s = 0;
     for (; s < stages - kStages; ++s) {
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
-        const char* st = lds[wave][s % kStages];
+        const char* st = lds[s % kStages];
         f0.read(st, st + 8192, lane, 0);
         f1.read(st, st + 8192, lane, 1);
         __builtin_amdgcn_sched_barrier(0);
@@ -453,7 +452,7 @@ __global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
         else
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const char* st = lds[wave][s % kStages];
+        const char* st = lds[s % kStages];
         f0.read(st, st + 8192, lane, 0);
         f1.read(st, st + 8192, lane, 1);
         f0.multiply(acc);
@@ -464,33 +463,132 @@ __global__ __launch_bounds__(kW * 64) void tile64_kernel(ArgsOf<kMode> a) {
     }
     const float scale = scale_of<kMode>(a, mat);
     const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
-    if constexpr (kW == 1) {
-        for (int u = 0; u < 2; ++u)
-            for (int v = 0; v < 2; ++v) finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], ti * 64l + u * 32, tj * 64l + v * 32, flip, lane, lds[0][0]);
-    } else if constexpr (kW == 2) {                          // a wave finishes a row of quadrants
-        __syncthreads();
-        float* sums = (float*)&lds[0][0][0];                 // [register][wave][lane], 16 KB
-        for (int i = 0; i < 32; ++i) sums[(i * 2 + wave) * 64 + lane] = wave == 0 ? acc[1][i >> 4][i & 15] : acc[0][i >> 4][i & 15];
-        __syncthreads();
-        for (int v = 0; v < 2; ++v) {
-            float16v mine = wave == 0 ? acc[0][v] : acc[1][v];
-            for (int i = 0; i < 16; ++i) mine[i] += sums[((v * 16 + i) * 2 + (wave ^ 1)) * 64 + lane];
-            finish<kMode, O, kMuon>(a, mat, scale, mine, ti * 64l + wave * 32, tj * 64l + v * 32, flip, lane, &lds[1][0][0] + wave * kFlipBytes);
+    for (int u = 0; u < 2; ++u)
+        for (int v = 0; v < 2; ++v) finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], ti * 64l + u * 32, tj * 64l + v * 32, flip, lane, lds[0]);
+}
+
+// s_waitcnt for all but n of a wave's copies, and for its LDS reads
+template <int n>
+__device__ __forceinline__ void await_copies() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
+}
+
+// 64 x 64 tiles of fewer products, kSlices waves each: a wave computes the whole tile over its 16 of the 16 kSlices columns of k that a stage
+// holds, and the partial sums are added at the end, in a fixed order.  The operands of a stage are read while the products of the one
+// before are computed, and copies run three stages ahead (136 tiles, k = 1024, 2 slices: 12.6 us; each wave with blocks of its own, two of them
+// ahead, 14.5).
+template <int kSlices, int kMode, typename O = float, bool kMuon = false>
+__global__ __launch_bounds__(kSlices * 64) void split_kernel(ArgsOf<kMode> a) {
+    static_assert(kSlices == 2 || kSlices == 4, "a wave takes half a block of k");
+    constexpr int kStages = 4, kBlocks = kSlices / 2, kStage = kBlocks * 16384, kLoads = 8;
+    __shared__ __align__(16) char lds[kStages][kStage];      // of a stage: block, operand
+    const int slice = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int mat, ti, tj;
+    my_tile(a.panels_p, a.panels_q, kSymmetric<kMode>, mat, ti, tj);
+    // a wave copies one operand of one block
+    const char* src = (slice & 1 ? a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes : a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes) +
+                      (slice >> 1) * kBlockBytes;
+    const int steps = a.kc / kBlocks;                        // (kc is even)
+    auto load = [&](int s) {
+        for (int i = 0; i < kLoads; ++i)
+            __builtin_amdgcn_global_load_lds((gptr)(src + (long)s * (kBlocks * kBlockBytes) + i * 1024 + lane * 16),
+                                             (lptr)(&lds[s % kStages][slice * 8192 + i * 1024]), 16, 0, 0);
+    };
+    float16v acc[2][2] = {};
+    Frag<2, 2> f0, f1;
+    auto read = [&](Frag<2, 2>& f, int s) {
+        const char* st = lds[s % kStages] + (slice >> 1) * 16384;
+        f.read(st, st + 8192, lane, slice & 1);
+    };
+    auto step = [&](int s, const Frag<2, 2>& now, Frag<2, 2>& next) {
+        await_copies<(kStages - 2) * kLoads>();              // the next stage has landed, and this one is read
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        read(next, s + 1);
+        load(s + kStages);
+        now.multiply(acc);
+        for (int i = 0; i < 8; ++i) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedVmem, 1, 0);
         }
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 4, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    int s = 0;
+    auto last = [&](Frag<2, 2>& fa, Frag<2, 2>& fb) {        // the last kStages steps, or fewer: nothing left to copy
+#pragma unroll
+        for (int r = 0; r < kStages; ++r) {
+            if (s + r < steps) {
+                if (r == 0)
+                    await_copies<2 * kLoads>();
+                else if (r == 1)
+                    await_copies<kLoads>();
+                else
+                    await_copies<0>();
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                if (s + r + 1 < steps) read(r & 1 ? fa : fb, s + r + 1);
+                (r & 1 ? fb : fa).multiply(acc);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
+    for (int k = 0; k < kStages && k < steps; ++k) load(k);
+    if (steps >= kStages)
+        await_copies<(kStages - 1) * kLoads>();
+    else
+        await_copies<0>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    read(f0, 0);
+    for (; s + 1 < steps - kStages; s += 2) {
+        step(s, f0, f1);
+        step(s + 1, f1, f0);
+    }
+    if (steps - s > kStages) {
+        step(s, f0, f1);
+        ++s;
+        last(f1, f0);
     } else {
-        static_assert(kW == 4, "a wave per quadrant");
+        last(f0, f1);
+    }
+    if constexpr (kMode == kFinal) {
+        if (a.guard && a.guard->status != 0) return;
+    }
+    const float scale = scale_of<kMode>(a, mat);
+    const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
+    const long r0 = (long)ti * 64, c0 = (long)tj * 64;
+    float* sums = (float*)lds;
+    __syncthreads();
+    if constexpr (kSlices == 2) {                            // a wave finishes half the rows; [register][slice][lane], 16 KB
+        char* own = (char*)lds + 16384 + slice * kFlipBytes;
+        static_assert(16384 + kSlices * kFlipBytes <= sizeof(lds), "");
+        float16v mine[2];
+#pragma unroll
+        for (int v = 0; v < 2; ++v)
+            for (int i = 0; i < 16; ++i) {
+                const float x = acc[0][v][i], y = acc[1][v][i];
+                mine[v][i] = slice == 0 ? x : y;
+                sums[((v * 16 + i) * 2 + slice) * 64 + lane] = slice == 0 ? y : x;
+            }
         __syncthreads();
-        float* sums = (float*)&lds[0][0][0];                 // [quadrant][register][wave][lane]
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+            for (int i = 0; i < 16; ++i) mine[v][i] += sums[((v * 16 + i) * 2 + (slice ^ 1)) * 64 + lane];
+            finish<kMode, O, kMuon>(a, mat, scale, mine[v], r0 + slice * 32, c0 + v * 32, flip, lane, own);
+        }
+    } else {                                                 // a wave finishes a quadrant; [quadrant][other wave][register][lane], 48 KB
+#pragma unroll
         for (int t = 0; t < 4; ++t)
-            if (t != wave)
-                for (int i = 0; i < 16; ++i) sums[((t * 16 + i) * 4 + wave) * 64 + lane] = acc[t >> 1][t & 1][i];
+            if (t != slice)
+                for (int i = 0; i < 16; ++i) sums[((t * 3 + (slice - (slice > t))) * 16 + i) * 64 + lane] = acc[t >> 1][t & 1][i];
         __syncthreads();
-        float16v mine = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1];
-        for (int w = 0; w < 4; ++w)
-            if (w != wave)
-                for (int i = 0; i < 16; ++i) mine[i] += sums[((wave * 16 + i) * 4 + w) * 64 + lane];
-        // (the transposition's LDS lies behind the sums' 64 KB, which other waves may still read)
-        finish<kMode, O, kMuon>(a, mat, scale, mine, ti * 64l + (wave >> 1) * 32, tj * 64l + (wave & 1) * 32, flip, lane, &lds[2][0][0] + wave * kFlipBytes);
+        float16v mine = slice == 0 ? acc[0][0] : slice == 1 ? acc[0][1] : slice == 2 ? acc[1][0] : acc[1][1];
+        for (int w = 0; w < 3; ++w)
+            for (int i = 0; i < 16; ++i) mine[i] += sums[((slice * 3 + w) * 16 + i) * 64 + lane];
+        static_assert(49152 + kSlices * kFlipBytes <= sizeof(lds), "");
+        finish<kMode, O, kMuon>(a, mat, scale, mine, r0 + (slice >> 1) * 32, c0 + (slice & 1) * 32, flip, lane, (char*)lds + 49152 + slice * kFlipBytes);
     }
 }
 
@@ -506,7 +604,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     constexpr bool kDealt = T < 256;
     static_assert(kW * kFlipBytes <= kStage && kLoads * kW * 1024 == kStage, "");
     __shared__ __align__(16) char lds[kStages][kStage];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int mat, ti, tj;
     my_tile((a.panels_p + T / 64 - 1) / (T / 64), (a.panels_q + T / 64 - 1) / (T / 64), kSymmetric<kMode>, mat, ti, tj);
     const char* src[kLoads];
@@ -514,11 +612,11 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
         const int kb = wave * kLoads + i, row = (kb % (T / 8)) * 8;             // KB of the stage: P's rows by eight, then Q's
         const bool is_p = kb < T / 8;
         const int panel = min((is_p ? ti : tj) * (T / 64) + (row >> 6), (is_p ? a.panels_p : a.panels_q) - 1);   // (past the end: the last one again)
-        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + (long)panel * a.kc * kBlockBytes + (row & 63) * 128 + lane * 16;
+        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + (long)panel * a.kc * kBlockBytes + (row & 63) * 128;
     }
     auto load = [&](int k) {
         for (int i = 0; i < kLoads; ++i)
-            __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes), (lptr)(&lds[k % kStages][(wave * kLoads + i) * 1024]), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((gptr)(src[i] + k * kBlockBytes + lane * 16), (lptr)(&lds[k % kStages][(wave * kLoads + i) * 1024]), 16, 0, 0);
     };
     const int wr = (wave / kAcross) * kNu * 32, wc = (wave % kAcross) * kNv * 32;
     float16v acc[kNu][kNv] = {};
@@ -723,7 +821,7 @@ Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
         long at_once;
         double few, full, fixed;
     };
-    static constexpr Entry entries[] = {{64, 4, 256, 24, 29, 4.5}, {64, 2, 512, 45, 53, 5},    {64, 1, 1024, 72, 97, 7},
+    static constexpr Entry entries[] = {{64, 4, 256, 24, 29, 4.5}, {64, 2, 512, 33, 45, 4.5},    {64, 1, 1024, 72, 97, 7},
                                         {128, 1, 512, 84, 178, 7}, {192, 1, 256, 135, 183, 14}, {256, 1, 256, 196, 298, 20}};
     Choice best{};
     double least = 1e300;
@@ -780,11 +878,11 @@ void product(const FinalArgs& g, int count, hipStream_t s) {
     else if (how.tile == 128)
         tile_kernel<128, 2, 2, 2, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
     else if (how.split == 4)
-        tile64_kernel<4, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+        split_kernel<4, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
     else if (how.split == 2)
-        tile64_kernel<2, kMode, O, kMuon><<<grid, 128, 0, s>>>(g);
+        split_kernel<2, kMode, O, kMuon><<<grid, 128, 0, s>>>(g);
     else
-        tile64_kernel<1, kMode, O, kMuon><<<grid, 64, 0, s>>>(g);
+        tile64_kernel<kMode, O, kMuon><<<grid, 64, 0, s>>>(g);
 }
 
 template <typename O, bool kMuon>
