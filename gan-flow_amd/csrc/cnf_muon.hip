@@ -17,9 +17,9 @@
 // before s has reached 1:   A = s^2 Y Y^T,   Y' = (s / s') (a I + b A + c A^2) Y.
 //
 // LAYOUT ("piece matrix").  R x K, padded with zeros to multiples of 64 and stored in blocks of 64 rows x 32 columns, 8 KB
-// each, block (r / 64, k / 32) after block along k.  A row of a block is one 128-byte line: four 16-byte slots of hi, four of lo, slot s
-// at s ^ (row / 2 & 7): a block copied to LDS as it lies is read as MFMA operands (a 16-byte slot of 16 rows per cycle, two rows
-// to a line of the 64 banks) without bank conflicts.
+// each, block (r / 64, k / 32) after block along k.  A block is eight fragments of 1 KB -- by 16 columns, 32 rows, piece (hi, lo) -- and a
+// fragment is one operand of a 32 x 32 x 16 MFMA as its 64 lanes take it: row l % 32, columns 8 (l / 32) .. + 7 at 16 l.  So an operand is one
+// access of a whole kilobyte, from memory, into LDS and out of it without bank conflicts.
 // Every product is of the form C[r][c] = sum_k P[r][k] Q[c][k] with both operands contiguous along k: A = X X^T, A A (A is
 // symmetric) and X' = (a I + b A + c A^2) X with Q = X^T, which the step that makes X writes beside it.  A and A^2 are symmetric: only
 // tiles on and below the diagonal are computed, and written twice.
@@ -54,9 +54,10 @@ struct Dims {
     int tall;       // rows > cols: the iteration runs on the transposed matrix
 };
 
-// byte offset of element (r, c)'s hi piece in a piece matrix of kc blocks per row panel; its lo piece is at this ^ 64
+// byte offset of element (r, c)'s hi piece in a piece matrix of kc blocks per row panel; its lo piece is kLo behind
+constexpr int kLo = 1024;
 __device__ __forceinline__ long piece_at(long r, long c, long kc) {
-    return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((r & 63) << 7) + ((((c >> 3) & 3) ^ ((r >> 1) & 7)) << 4) + ((c & 7) << 1);
+    return ((r >> 6) * kc + (c >> 5)) * kBlockBytes + ((c >> 4 & 1) << 12) + ((r >> 5 & 1) << 11) + ((c >> 3 & 1) << 9) + ((r & 31) << 4) + ((c & 7) << 1);
 }
 
 // The pieces of two values.  The values are settled before they are split: the compiler otherwise folds the operation that makes one into one
@@ -194,7 +195,7 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
     char* flipped = (d.tall ? x : xt) + mat * d.mp * d.np * 4;
     const long kc_s = (d.tall ? d.mp : d.np) >> 5, kc_f = (d.tall ? d.np : d.mp) >> 5;
     for (int e = threadIdx.x; e < 1024; e += kThreads) {
-        const int i = (e & 511) >> 3, q = (e & 7) * 8;
+        const int i = e & 63, q = (e >> 6 & 7) * 8;
         float w[8];
         for (int k = 0; k < 8; ++k) w[k] = e < 512 ? tile[i][q + k] : tile[q + k][i];
         half4 h0, l0, h1, l1;
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
         char* base = e < 512 ? straight : flipped;
         const long at = e < 512 ? piece_at(r0 + i, c0 + q, kc_s) : piece_at(c0 + i, r0 + q, kc_f);
         *(half8*)(base + at) = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-        *(half8*)(base + (at ^ 64)) = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+        *(half8*)(base + at + kLo) = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
     }
 }
 
@@ -295,20 +296,19 @@ __device__ __forceinline__ void my_tile(int tiles_r, int tiles_c, bool sym, int&
     }
 }
 
-// Operands of the products of 16 k: kNu x kNv tiles of 32 x 32 from a block column of P and of Q in LDS
+// Operands of the products of 16 k: kNu x kNv tiles of 32 x 32
 template <int kNu, int kNv>
 struct Frag {
     half8 ph[kNu], pl[kNu], qh[kNv], ql[kNv];
-    // p, q: the wave's first rows of the two blocks; h: which 16 of the 32 k
-    __device__ __forceinline__ void read(const char* p, const char* q, int lane, int h) {
-        const int at = ((lane & 31) << 7) + ((((lane >> 5) ^ ((lane >> 1) & 7)) << 4) ^ (h << 5));
+    // p, q: the first of the wave's fragments of either operand, in LDS or in memory
+    __device__ __forceinline__ void read(const char* p, const char* q, int lane) {
         for (int v = 0; v < kNv; ++v) {
-            ql[v] = *(const half8*)(q + v * 32 * 128 + (at ^ 64));
-            qh[v] = *(const half8*)(q + v * 32 * 128 + at);
+            ql[v] = *(const half8*)(q + v * 2048 + kLo + lane * 16);
+            qh[v] = *(const half8*)(q + v * 2048 + lane * 16);
         }
         for (int u = 0; u < kNu; ++u) {
-            ph[u] = *(const half8*)(p + u * 32 * 128 + at);
-            pl[u] = *(const half8*)(p + u * 32 * 128 + (at ^ 64));
+            ph[u] = *(const half8*)(p + u * 2048 + lane * 16);
+            pl[u] = *(const half8*)(p + u * 2048 + kLo + lane * 16);
         }
     }
     // operands exchanged: a lane gets four neighbouring columns of a row of C
@@ -321,9 +321,9 @@ struct Frag {
 };
 
 // What happens to a 32 x 32 tile of C whose first element is (r0, c0): lane l holds columns 8 g + 4 (l / 32) + e (register 4 g + e) of
-// row l % 32.  In a piece matrix the tile's rows are 32 lines that follow each other, 4 KB, and so are the rows of its transpose; stored from where
-// the products leave it, it would go out in pieces of 16 bytes (a 256 x 256 tile of X and X^T: 14 us).  It goes through LDS instead
-// (4.6 KB a wave, hi and lo of an element in a word), and every store is a whole kilobyte.
+// row l % 32.  It goes through LDS (4.6 KB a wave, hi and lo of an element in a word), and its fragments and those of its transpose
+// are stored a whole kilobyte at a time; stored from where the products leave it, it would go out in pieces of 8 bytes
+// (a 256 x 256 tile of X and X^T in pieces of 16: 14 us).
 constexpr int kFlipBytes = 32 * 36 * 4;
 
 template <int kMode, typename O, bool kMuon>
@@ -331,32 +331,25 @@ __device__ __forceinline__ void finish(const ArgsOf<kMode>& a, int mat, float sc
                                        char* lds) {
     if (r0 >= (long)a.panels_p * 64 || c0 >= (long)a.panels_q * 64) return;     // (a tile larger than 64 can reach past the end)
     const int row = lane & 31, half = lane >> 5;
-    const int by8 = lane >> 3, nth = lane & 7;               // as stored: line 8 i + by8, its nth 16 bytes
     // (a wave's LDS operations are executed in order: reads see the writes before them, and writes come after the reads before them)
     if constexpr (kMode == kFinal) {
         float* t = (float*)lds;
         for (int g = 0; g < 4; ++g)
             *(float4*)(t + row * 36 + g * 8 + half * 4) = make_float4(acc[g * 4] * scale, acc[g * 4 + 1] * scale, acc[g * 4 + 2] * scale, acc[g * 4 + 3] * scale);
-        for (int i = 0; i < 4; ++i) {
-            const long r = r0 + i * 8 + by8, c = c0 + nth * 4;
-            const float4 x = *(const float4*)(t + (i * 8 + by8) * 36 + nth * 4);
+        for (int i = 0; i < 4; ++i) {                        // stored eight rows of 32 columns at a time
+            const long r = r0 + i * 8 + (lane >> 3), c = c0 + (lane & 7) * 4;
+            const float4 x = *(const float4*)(t + (i * 8 + (lane >> 3)) * 36 + (lane & 7) * 4);
             const float val[4] = {x.x, x.y, x.z, x.w};
             if (r < a.rows && c < a.cols) put4<O, kMuon>(a, mat, r, c, val);
         }
     } else {
-        const long kc0 = a.panels_q * 2, kc1 = a.panels_p * 2;
-        const long at = ((r0 >> 6) * kc0 + (c0 >> 5)) * kBlockBytes + ((r0 & 63) << 7) + lane * 16;
+        const long kc0 = a.panels_q * 2, kc1 = a.panels_p * 2, at = piece_at(r0, c0, kc0);
         half4 old_h[4], old_l[4];
-        if (kMode == kPoly) {                                // the same tile of P
-            const char* pm = a.p + mat * a.bp + at;
-            uint4 old[4];
-            for (int i = 0; i < 4; ++i) old[i] = *(const uint4*)(pm + i * 1024);
-            for (int i = 0; i < 4; ++i) *(uint4*)(lds + (i * 8 + by8) * 144 + nth * 16) = old[i];
-            const char* line = lds + row * 144 + half * 8;
-            const int sw = ((row >> 1) & 7) << 4;
+        if (kMode == kPoly) {                                // the same elements of P
+            const char* pm = a.p + mat * a.bp + at + row * 16 + half * 8;
             for (int g = 0; g < 4; ++g) {
-                old_h[g] = *(const half4*)(line + ((g << 4) ^ sw));
-                old_l[g] = *(const half4*)(line + ((g << 4) ^ sw ^ 64));
+                old_h[g] = *(const half4*)(pm + (g >> 1) * 4096 + (g & 1) * 512);
+                old_l[g] = *(const half4*)(pm + (g >> 1) * 4096 + (g & 1) * 512 + kLo);
             }
         }
         unsigned* t = (unsigned*)lds;                        // (hi, lo) of element (r, c) at r * 36 + c
@@ -380,21 +373,21 @@ __device__ __forceinline__ void finish(const ArgsOf<kMode>& a, int mat, float sc
             return make_uint4(__builtin_amdgcn_perm(w[1], w[0], part), __builtin_amdgcn_perm(w[3], w[2], part),
                               __builtin_amdgcn_perm(w[5], w[4], part), __builtin_amdgcn_perm(w[7], w[6], part));
         };
-        char* to = a.c0 + mat * a.b0 + at;
-        for (int i = 0; i < 4; ++i) {
-            const int l = i * 8 + by8, slot = nth ^ ((l >> 1) & 7);              // slot 0 .. 3: hi of eight columns, 4 .. 7: lo
-            const uint4 x = *(const uint4*)(t + l * 36 + (slot & 3) * 8), y = *(const uint4*)(t + l * 36 + (slot & 3) * 8 + 4);
-            const unsigned w[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-            *(uint4*)(to + i * 1024) = pack(w, slot & 4 ? 0x07060302u : 0x05040100u);
+        auto put = [&](char* to, const unsigned (&w)[8]) {
+            *(uint4*)(to + lane * 16) = pack(w, 0x05040100u);
+            *(uint4*)(to + lane * 16 + kLo) = pack(w, 0x07060302u);
+        };
+        for (int k = 0; k < 2; ++k) {
+            const unsigned* from = t + row * 36 + k * 16 + half * 8;
+            const uint4 x = *(const uint4*)from, y = *(const uint4*)(from + 4);
+            put(a.c0 + mat * a.b0 + at + k * 4096, {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w});
         }
         if (flip) {
-            char* tc = (kMode == kApply ? a.c1 + mat * a.b1 : a.c0 + mat * a.b0) +
-                       ((c0 >> 6) * (kMode == kApply ? kc1 : kc0) + (r0 >> 5)) * kBlockBytes + ((c0 & 63) << 7) + lane * 16;
-            for (int i = 0; i < 4; ++i) {
-                const int l = i * 8 + by8, slot = nth ^ ((l >> 1) & 7);
+            char* tc = (kMode == kApply ? a.c1 + mat * a.b1 : a.c0 + mat * a.b0) + piece_at(c0, r0, kMode == kApply ? kc1 : kc0);
+            for (int k = 0; k < 2; ++k) {
                 unsigned w[8];
-                for (int e = 0; e < 8; ++e) w[e] = t[((slot & 3) * 8 + e) * 36 + l];
-                *(uint4*)(tc + i * 1024) = pack(w, slot & 4 ? 0x07060302u : 0x05040100u);
+                for (int e = 0; e < 8; ++e) w[e] = t[(k * 16 + half * 8 + e) * 36 + row];
+                put(tc + k * 4096, w);
             }
         }
     }
@@ -408,188 +401,63 @@ __device__ __forceinline__ float scale_of(const ArgsOf<kMode>& a, int mat) {
     return kInvScale * (kMode == kGram ? f[0] * f[0] : kMode == kApply ? f[0] / f[a.ahead] : f[0] * kInvScale);
 }
 
-// 64 x 64 tiles of many products, a wave each: it copies its own operands, so nothing but its own counters holds it up.
+// 64 x 64 tiles: each of four waves computes the whole tile over every fourth 16 columns of k, on operands that it loads from memory into
+// registers kAhead steps before it needs them, and the partial sums are added at the end, in a fixed order.  The waves share no operands,
+// so LDS would only add its own traffic: four matrices' 1024 x 1024 x 1024 symmetric products take 24 us, and 27 with operands copied to LDS
+// (by one, two or four waves, which then wait for LDS).  What bounds it is the operands' way from L2, 16 TB/s.
 template <int kMode, typename O = float, bool kMuon = false>
-__global__ __launch_bounds__(64) void tile64_kernel(ArgsOf<kMode> a) {
-    constexpr int kStages = 2, kStage = 2 * 64 * 128, kLoads = kStage / 1024;
-    __shared__ __align__(16) char lds[kStages][kStage];
-    const int lane = threadIdx.x;
+__global__ __launch_bounds__(256) void tile64_kernel(ArgsOf<kMode> a) {
+    constexpr int kW = 4, kAhead = 4;
+    __shared__ __align__(16) char lds[49152];                // partial sums: [quadrant][other wave][register][lane]; then finish()'s
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     int mat, ti, tj;
     my_tile(a.panels_p, a.panels_q, kSymmetric<kMode>, mat, ti, tj);
-    const char* ps = a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes;
-    const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes;
-    const int stages = a.kc;
-    auto load = [&](int s) {
-        const long off = (long)s * kBlockBytes;
-        for (int i = 0; i < kLoads / 2; ++i) {
-            __builtin_amdgcn_global_load_lds((gptr)(ps + off + i * 1024 + lane * 16), (lptr)(&lds[s % kStages][i * 1024]), 16, 0, 0);
-            __builtin_amdgcn_global_load_lds((gptr)(qs + off + i * 1024 + lane * 16), (lptr)(&lds[s % kStages][8192 + i * 1024]), 16, 0, 0);
-        }
-    };
+    const char* ps = a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes + wave * 4096;
+    const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes + wave * 4096;
+    const int steps = 2 * a.kc / kW;                         // (kc is even)
     float16v acc[2][2] = {};
-    Frag<2, 2> f0, f1;
-    for (int s = 0; s < kStages && s < stages; ++s) load(s);
-    int s = 0;
-    for (; s < stages - kStages; ++s) {
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
-        const char* st = lds[s % kStages];
-        f0.read(st, st + 8192, lane, 0);
-        f1.read(st, st + 8192, lane, 1);
-        __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // read: the next copy may take its place
-        load(s + kStages);
-        f0.multiply(acc);
-        f1.multiply(acc);
-        for (int i = 0; i < kLoads; ++i) {                   // copies dealt out between the products: in one go they hold the wave up
-            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kSchedVmem, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 24 - kLoads, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    }
-    for (; s < stages; ++s) {
-        if (s + 1 < stages)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
-        else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        const char* st = lds[s % kStages];
-        f0.read(st, st + 8192, lane, 0);
-        f1.read(st, st + 8192, lane, 1);
-        f0.multiply(acc);
-        f1.multiply(acc);
-    }
-    if constexpr (kMode == kFinal) {
-        if (a.guard && a.guard->status != 0) return;
-    }
-    const float scale = scale_of<kMode>(a, mat);
-    const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
-    for (int u = 0; u < 2; ++u)
-        for (int v = 0; v < 2; ++v) finish<kMode, O, kMuon>(a, mat, scale, acc[u][v], ti * 64l + u * 32, tj * 64l + v * 32, flip, lane, lds[0]);
-}
-
-// s_waitcnt for all but n of a wave's copies, and for its LDS reads
-template <int n>
-__device__ __forceinline__ void await_copies() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(n) : "memory");
-}
-
-// 64 x 64 tiles of fewer products, kSlices waves each: a wave computes the whole tile over its 16 of the 16 kSlices columns of k that a stage
-// holds, and the partial sums are added at the end, in a fixed order.  The operands of a stage are read while the products of the one
-// before are computed, and copies run three stages ahead (136 tiles, k = 1024, 2 slices: 12.6 us; each wave with blocks of its own, two of them
-// ahead, 14.5).
-template <int kSlices, int kMode, typename O = float, bool kMuon = false>
-__global__ __launch_bounds__(kSlices * 64) void split_kernel(ArgsOf<kMode> a) {
-    static_assert(kSlices == 2 || kSlices == 4, "a wave takes half a block of k");
-    constexpr int kStages = 4, kBlocks = kSlices / 2, kStage = kBlocks * 16384, kLoads = 8;
-    __shared__ __align__(16) char lds[kStages][kStage];      // of a stage: block, operand
-    const int slice = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    int mat, ti, tj;
-    my_tile(a.panels_p, a.panels_q, kSymmetric<kMode>, mat, ti, tj);
-    // a wave copies one operand of one block
-    const char* src = (slice & 1 ? a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes : a.p + mat * a.bp + (long)ti * a.kc * kBlockBytes) +
-                      (slice >> 1) * kBlockBytes;
-    const int steps = a.kc / kBlocks;                        // (kc is even)
-    auto load = [&](int s) {
-        for (int i = 0; i < kLoads; ++i)
-            __builtin_amdgcn_global_load_lds((gptr)(src + (long)s * (kBlocks * kBlockBytes) + i * 1024 + lane * 16),
-                                             (lptr)(&lds[s % kStages][slice * 8192 + i * 1024]), 16, 0, 0);
-    };
-    float16v acc[2][2] = {};
-    Frag<2, 2> f0, f1;
-    auto read = [&](Frag<2, 2>& f, int s) {
-        const char* st = lds[s % kStages] + (slice >> 1) * 16384;
-        f.read(st, st + 8192, lane, slice & 1);
-    };
-    auto step = [&](int s, const Frag<2, 2>& now, Frag<2, 2>& next) {
-        await_copies<(kStages - 2) * kLoads>();              // the next stage has landed, and this one is read
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        read(next, s + 1);
-        load(s + kStages);
-        now.multiply(acc);
-        for (int i = 0; i < 8; ++i) {
-            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(kSchedVmem, 1, 0);
-        }
-        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 4, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    int s = 0;
-    auto last = [&](Frag<2, 2>& fa, Frag<2, 2>& fb) {        // the last kStages steps, or fewer: nothing left to copy
+    Frag<2, 2> f[kAhead];
+    auto load = [&](int d, int s) { f[d].read(ps + (long)s * (kW * 4096), qs + (long)s * (kW * 4096), lane); };
 #pragma unroll
-        for (int r = 0; r < kStages; ++r) {
-            if (s + r < steps) {
-                if (r == 0)
-                    await_copies<2 * kLoads>();
-                else if (r == 1)
-                    await_copies<kLoads>();
-                else
-                    await_copies<0>();
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                if (s + r + 1 < steps) read(r & 1 ? fa : fb, s + r + 1);
-                (r & 1 ? fb : fa).multiply(acc);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+    for (int d = 0; d < kAhead; ++d)
+        if (d < steps) load(d, d);
+    int s = 0;
+    for (; s + 2 * kAhead <= steps; s += kAhead) {
+#pragma unroll
+        for (int d = 0; d < kAhead; ++d) {
+            f[d].multiply(acc);
+            load(d, s + d + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
         }
-    };
-    for (int k = 0; k < kStages && k < steps; ++k) load(k);
-    if (steps >= kStages)
-        await_copies<(kStages - 1) * kLoads>();
-    else
-        await_copies<0>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    read(f0, 0);
-    for (; s + 1 < steps - kStages; s += 2) {
-        step(s, f0, f1);
-        step(s + 1, f1, f0);
     }
-    if (steps - s > kStages) {
-        step(s, f0, f1);
-        ++s;
-        last(f1, f0);
-    } else {
-        last(f0, f1);
-    }
+    // up to 2 kAhead - 1 are left, kAhead of them loaded
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+        if (s + d < steps) {
+            f[d].multiply(acc);
+            if (s + d + kAhead < steps) load(d, s + d + kAhead);
+        }
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d)
+        if (s + kAhead + d < steps) f[d].multiply(acc);
     if constexpr (kMode == kFinal) {
         if (a.guard && a.guard->status != 0) return;
     }
     const float scale = scale_of<kMode>(a, mat);
     const bool flip = kMode == kApply || (kSymmetric<kMode> && ti != tj);
-    const long r0 = (long)ti * 64, c0 = (long)tj * 64;
     float* sums = (float*)lds;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+        if (t != wave)
+            for (int i = 0; i < 16; ++i) sums[((t * 3 + (wave - (wave > t))) * 16 + i) * 64 + lane] = acc[t >> 1][t & 1][i];
     __syncthreads();
-    if constexpr (kSlices == 2) {                            // a wave finishes half the rows; [register][slice][lane], 16 KB
-        char* own = (char*)lds + 16384 + slice * kFlipBytes;
-        static_assert(16384 + kSlices * kFlipBytes <= sizeof(lds), "");
-        float16v mine[2];
-#pragma unroll
-        for (int v = 0; v < 2; ++v)
-            for (int i = 0; i < 16; ++i) {
-                const float x = acc[0][v][i], y = acc[1][v][i];
-                mine[v][i] = slice == 0 ? x : y;
-                sums[((v * 16 + i) * 2 + slice) * 64 + lane] = slice == 0 ? y : x;
-            }
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < 2; ++v) {
-            for (int i = 0; i < 16; ++i) mine[v][i] += sums[((v * 16 + i) * 2 + (slice ^ 1)) * 64 + lane];
-            finish<kMode, O, kMuon>(a, mat, scale, mine[v], r0 + slice * 32, c0 + v * 32, flip, lane, own);
-        }
-    } else {                                                 // a wave finishes a quadrant; [quadrant][other wave][register][lane], 48 KB
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-            if (t != slice)
-                for (int i = 0; i < 16; ++i) sums[((t * 3 + (slice - (slice > t))) * 16 + i) * 64 + lane] = acc[t >> 1][t & 1][i];
-        __syncthreads();
-        float16v mine = slice == 0 ? acc[0][0] : slice == 1 ? acc[0][1] : slice == 2 ? acc[1][0] : acc[1][1];
-        for (int w = 0; w < 3; ++w)
-            for (int i = 0; i < 16; ++i) mine[i] += sums[((slice * 3 + w) * 16 + i) * 64 + lane];
-        static_assert(49152 + kSlices * kFlipBytes <= sizeof(lds), "");
-        finish<kMode, O, kMuon>(a, mat, scale, mine, r0 + (slice >> 1) * 32, c0 + (slice & 1) * 32, flip, lane, (char*)lds + 49152 + slice * kFlipBytes);
-    }
+    float16v mine = wave == 0 ? acc[0][0] : wave == 1 ? acc[0][1] : wave == 2 ? acc[1][0] : acc[1][1];
+    for (int w = 0; w < 3; ++w)
+        for (int i = 0; i < 16; ++i) mine[i] += sums[((wave * 3 + w) * 16 + i) * 64 + lane];
+    // (settled before the barrier: the compiler moves a read whose value only one side of a branch needs past it)
+    for (int i = 0; i < 16; ++i) asm volatile("" ::"v"(mine[i]));
+    __syncthreads();                                     // everybody has read the sums
+    finish<kMode, O, kMuon>(a, mat, scale, mine, ti * 64l + (wave >> 1) * 32, tj * 64l + (wave & 1) * 32, flip, lane, lds + wave * kFlipBytes);
 }
 
 // T x T tiles for larger products: waves of kNu x kNv MFMA tiles share kStages stages of one block column each.  The operands of each 16 k are
@@ -609,10 +477,11 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     my_tile((a.panels_p + T / 64 - 1) / (T / 64), (a.panels_q + T / 64 - 1) / (T / 64), kSymmetric<kMode>, mat, ti, tj);
     const char* src[kLoads];
     for (int i = 0; i < kLoads; ++i) {
-        const int kb = wave * kLoads + i, row = (kb % (T / 8)) * 8;             // KB of the stage: P's rows by eight, then Q's
-        const bool is_p = kb < T / 8;
-        const int panel = min((is_p ? ti : tj) * (T / 64) + (row >> 6), (is_p ? a.panels_p : a.panels_q) - 1);   // (past the end: the last one again)
-        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + (long)panel * a.kc * kBlockBytes + (row & 63) * 128;
+        // a stage in LDS: by 16 k (half a stage), operand, 32 rows, piece, a kilobyte each
+        const int kb = wave * kLoads + i, half = kb / (T / 8), row32 = kb / 2 % (T / 32);
+        const bool is_p = kb / (T / 16) % 2 == 0;
+        const int panel = min((is_p ? ti : tj) * (T / 64) + row32 / 2, (is_p ? a.panels_p : a.panels_q) - 1);   // (past the end: the last one again)
+        src[i] = (is_p ? a.p + mat * a.bp : a.q + mat * a.bq) + (long)panel * a.kc * kBlockBytes + half * 4096 + row32 % 2 * 2048 + kb % 2 * kLo;
     }
     auto load = [&](int k) {
         for (int i = 0; i < kLoads; ++i)
@@ -628,11 +497,11 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    f0.read(lds[0] + wr * 128, lds[0] + (T + wc) * 128, lane, 0);
+    f0.read(lds[0] + wr * 64, lds[0] + (T + wc) * 64, lane);
     constexpr int kReads = 2 * (kNu + kNv), kMul = 3 * kNu * kNv;
     int k = 0;
     for (; k < a.kc - kStages; ++k) {
-        f1.read(lds[k % kStages] + wr * 128, lds[k % kStages] + (T + wc) * 128, lane, 1);
+        f1.read(lds[k % kStages] + (2 * T + wr) * 64, lds[k % kStages] + (3 * T + wc) * 64, lane);
         f0.multiply(acc);
         if (kDealt) {
             for (int i = 0; i < kReads; ++i) {
@@ -647,7 +516,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const char* next = lds[(k + 1) % kStages];
-        f0.read(next + wr * 128, next + (T + wc) * 128, lane, 0);
+        f0.read(next + wr * 64, next + (T + wc) * 64, lane);
         load(k + kStages);
         f1.multiply(acc);
         if (kDealt) {
@@ -664,14 +533,14 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
         __builtin_amdgcn_sched_barrier(0);
     }
     for (; k < a.kc; ++k) {                                  // the last stages: nothing left to copy
-        f1.read(lds[k % kStages] + wr * 128, lds[k % kStages] + (T + wc) * 128, lane, 1);
+        f1.read(lds[k % kStages] + (2 * T + wr) * 64, lds[k % kStages] + (3 * T + wc) * 64, lane);
         f0.multiply(acc);
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         const char* next = lds[(k + 1) % kStages];
-        if (k + 1 < a.kc) f0.read(next + wr * 128, next + (T + wc) * 128, lane, 0);
+        if (k + 1 < a.kc) f0.read(next + wr * 64, next + (T + wc) * 64, lane);
         f1.multiply(acc);
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -735,21 +604,19 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
         split4({v[0][i], v[1][i], v[2][i], v[3][i]}, ht, lt);
         const long at = piece_at(tr * 4 + i, tc, 2), att = piece_at(tc + i, tr * 4, 2);
         *(half4*)(straight + at) = h;
-        *(half4*)(straight + (at ^ 64)) = l;
+        *(half4*)(straight + at + kLo) = l;
         *(half4*)(flipped + att) = ht;
-        *(half4*)(flipped + (att ^ 64)) = lt;
+        *(half4*)(flipped + att + kLo) = lt;
     }
     const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-    const int slot = ((lane >> 5) ^ ((lane >> 1) & 7)) << 4, line = (lane & 31) << 7;
     // quadrant (pr, qr) of sum_k P[r][k] Q[c][k]: a lane holds columns 8 g + 4 (lane / 32) + e of row lane % 32
     auto multiply = [&](const char* p, int pr, const char* q, int qr) {
         float16v acc = {};
 #pragma unroll
         for (int kb = 0; kb < 4; ++kb) {
-            const char *pp = p + (kb >> 1) * kBlockBytes + pr * 128 + line, *qq = q + (kb >> 1) * kBlockBytes + qr * 128 + line;
-            const int so = slot ^ ((kb & 1) << 5);
-            const half8 ph = *(const half8*)(pp + so), pl = *(const half8*)(pp + (so ^ 64));
-            const half8 qh = *(const half8*)(qq + so), ql = *(const half8*)(qq + (so ^ 64));
+            const char *pp = p + kb * 4096 + pr * 64 + lane * 16, *qq = q + kb * 4096 + qr * 64 + lane * 16;
+            const half8 ph = *(const half8*)pp, pl = *(const half8*)(pp + kLo);
+            const half8 qh = *(const half8*)qq, ql = *(const half8*)(qq + kLo);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
             acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
@@ -763,12 +630,12 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
             split4({x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]}, h, l);
             const long at = piece_at(row, col + q * 8, 2);
             *(half4*)(to + at) = h;
-            *(half4*)(to + (at ^ 64)) = l;
+            *(half4*)(to + at + kLo) = l;
             if (flip)
                 for (int e = 0; e < 4; ++e) {
                     const long t = piece_at(col + q * 8 + e, row, 2);
                     *(f16*)(flip + t) = h[e];
-                    *(f16*)(flip + (t ^ 64)) = l[e];
+                    *(f16*)(flip + t + kLo) = l[e];
                 }
         }
     };
@@ -807,31 +674,33 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
 
 long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 
-// Which kernel computes a product: the one whose estimated time is least.  A round is as many workgroups as run at once; it takes `few` us per 4096
-// of k up to half full and `full` us when full, and `fixed` us whatever k is (its first copies, its results).  Measured on 6 .. 4096 tiles and
-// k = 256 .. 4096; the estimate is within a tenth or two of the measured time and never took a kernel 15 % behind the best.
+// Which kernel computes a product: the one whose estimated time is least.  A round is as many workgroups as run at once; it takes `few` us per
+// 4096 of k with few of them and `full` us when full, and `fixed` us whatever k is (its first operands, its results).  Where two run on a
+// CU, a round takes `full` as soon as one CU has two; where one does, what lies behind the CUs slows down from half full on.  Fitted
+// to products of 1 .. 1024 tiles and k = 256 .. 4096 (within a tenth for most, a quarter at worst); of those no choice was 5 % behind the best.
+constexpr long kCus = 256;
 struct Choice {
-    int tile, split;
+    int tile;
     double time;
 };
 
 Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
     struct Entry {
-        int tile, split;
+        int tile;
         long at_once;
         double few, full, fixed;
     };
-    static constexpr Entry entries[] = {{64, 4, 256, 24, 29, 4.5}, {64, 2, 512, 33, 45, 4.5},    {64, 1, 1024, 72, 97, 7},
-                                        {128, 1, 512, 84, 178, 7}, {192, 1, 256, 135, 183, 14}, {256, 1, 256, 196, 298, 20}};
+    static constexpr Entry entries[] = {{64, 512, 22, 50, 4}, {128, 512, 84, 178, 7}, {192, 256, 135, 183, 14}, {256, 256, 196, 298, 20}};
     Choice best{};
     double least = 1e300;
     for (const Entry& e : entries) {
         const int t = e.tile / 64;
         const long r = (panels_p + t - 1) / t, c = (panels_q + t - 1) / t, tiles = count * (sym ? r * (r + 1) / 2 : r * c);
         const long whole = tiles / e.at_once, rest = tiles % e.at_once;
-        const double last = rest ? e.few + (e.full - e.few) * std::fmax(0., 2. * rest / e.at_once - 1.) : 0.;
+        double last = 0.;
+        if (rest) last = e.at_once > kCus ? (rest > kCus ? e.full : e.few) : e.few + (e.full - e.few) * std::fmax(0., 2. * rest / kCus - 1.);
         const double time = (whole * e.full + last) * kc / 128. + (whole + (rest > 0)) * e.fixed;
-        if (time < least) least = time, best = {e.tile, e.split, time};
+        if (time < least) least = time, best = {e.tile, time};
     }
     return best;
 }
@@ -877,12 +746,8 @@ void product(const FinalArgs& g, int count, hipStream_t s) {
         tile_kernel<192, 3, 3, 3, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
     else if (how.tile == 128)
         tile_kernel<128, 2, 2, 2, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
-    else if (how.split == 4)
-        split_kernel<4, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
-    else if (how.split == 2)
-        split_kernel<2, kMode, O, kMuon><<<grid, 128, 0, s>>>(g);
     else
-        tile64_kernel<kMode, O, kMuon><<<grid, 64, 0, s>>>(g);
+        tile64_kernel<kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
 }
 
 template <typename O, bool kMuon>
