@@ -559,28 +559,37 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
 }
 
 // Matrices of at most 64 x 64: one workgroup per matrix does the whole update, with X, X^T, A and a I + b A + c A^2 as piece matrices in LDS
-// (two blocks of 8 KB each).  A wave computes one 32 x 32 quadrant of every product.  What bounds it is the chain: 3 products per
-// step, each a barrier, its operands' LDS reads, 12 dependent MFMAs and the split of its result.
+// (two blocks of 8 KB each), where the rows of every 8 columns are in another order: threads write what is 8 columns apart, which would
+// lie in the same banks.  Each of eight waves computes 16 rows x 32 columns of every product.  What bounds it is the chain: 3 products per
+// step, each a barrier, its operands' LDS reads, MFMAs, the split of its result; two waves on a SIMD fill each other's waits (64 x 64, five
+// steps: 14 us; one wave a SIMD with 32 x 32 quadrants, 17).
+constexpr int kSmall = 512;
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ int small_at(int r, int c) {
+    return ((c >> 4) << 12) + ((r >> 5) << 11) + ((c >> 3 & 1) << 9) + (((r & 31) ^ (c >> 3)) << 4) + ((c & 7) << 1);
+}
+
 template <typename O, bool kMuon>
-__global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, Steps st, double eps, float mu, int nesterov) {
+__global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Steps st, double eps, float mu, int nesterov) {
     __shared__ __align__(16) char xs[2 * kBlockBytes], xts[2 * kBlockBytes], as[2 * kBlockBytes], bs[2 * kBlockBytes];
-    __shared__ double red[kThreads / 64];
-    const int mat = blockIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    __shared__ double red[kSmall / 64];
+    const int mat = blockIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
     const bool skip = a.guard && a.guard->status != 0;
     const O* g = (const O*)a.ptrs.g[mat];
-    // the matrix: thread (tr, tc) holds four rows of four columns (what lies outside is read at the last element and not used)
-    const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4;
-    float v[4][4], old[4][4];
-    for (int i = 0; i < 4; ++i)
+    // the matrix: thread (tr, tc) holds two rows of four columns (what lies outside is read at the last element and not used)
+    const int tr = (threadIdx.x >> 4) * 2, tc = (threadIdx.x & 15) * 4;
+    float v[2][4], old[2][4];
+    for (int i = 0; i < 2; ++i)
         for (int k = 0; k < 4; ++k) {
-            const int r = min(tr * 4 + i, (int)a.rows - 1), c = min(tc + k, (int)a.cols - 1);
+            const int r = min(tr + i, (int)a.rows - 1), c = min(tc + k, (int)a.cols - 1);
             v[i][k] = to_f32(g[r * d.ldg + c]);
             if (kMuon) old[i][k] = a.ptrs.m[mat][r * d.ldm + c];
         }
     double s = 0.;
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
         for (int k = 0; k < 4; ++k) {
-            const int r = tr * 4 + i, c = tc + k;
+            const int r = tr + i, c = tc + k;
             const bool in = r < a.rows && c < a.cols;
             if (kMuon) {
                 const float mv = fmaf(mu, old[i][k], v[i][k]);
@@ -594,81 +603,90 @@ __global__ __launch_bounds__(kThreads) void small_kernel(FinalArgs a, Dims d, St
     if (lane == 0) red[wave] = s;
     __syncthreads();
     float f;
-    const double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
+    const double scale = start_scale(sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]))), eps, f);
     char *straight = d.tall ? xts : xs, *flipped = d.tall ? xs : xts;
-    for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 2; ++i)
         for (int k = 0; k < 4; ++k) v[i][k] = (float)((double)v[i][k] * scale);
-    for (int i = 0; i < 4; ++i) {
-        half4 h, l, ht, lt;
-        split4(v[i], h, l);
-        split4({v[0][i], v[1][i], v[2][i], v[3][i]}, ht, lt);
-        const long at = piece_at(tr * 4 + i, tc, 2), att = piece_at(tc + i, tr * 4, 2);
-        *(half4*)(straight + at) = h;
-        *(half4*)(straight + at + kLo) = l;
-        *(half4*)(flipped + att) = ht;
-        *(half4*)(flipped + att + kLo) = lt;
+    half4 h[2], l[2];
+    for (int i = 0; i < 2; ++i) {
+        split4(v[i], h[i], l[i]);
+        const int at = small_at(tr + i, tc);
+        *(half4*)(straight + at) = h[i];
+        *(half4*)(straight + at + kLo) = l[i];
     }
-    const int wr = (wave >> 1) * 32, wc = (wave & 1) * 32;
-    // quadrant (pr, qr) of sum_k P[r][k] Q[c][k]: a lane holds columns 8 g + 4 (lane / 32) + e of row lane % 32
+    for (int k = 0; k < 4; ++k) {
+        const int at = small_at(tc + k, tr);
+        *(half2*)(flipped + at) = (half2){h[0][k], h[1][k]};
+        *(half2*)(flipped + at + kLo) = (half2){l[0][k], l[1][k]};
+    }
+    const int wr = (wave >> 1) * 16, wc = (wave & 1) * 32;
+    struct Part { float4v t[2]; };
+    // rows pr .. + 15 and columns qr .. + 31 of sum_k P[r][k] Q[c][k]: a lane holds columns 16 t + 4 (lane / 16) + e of row lane % 16
     auto multiply = [&](const char* p, int pr, const char* q, int qr) {
-        float16v acc = {};
+        Part acc = {};
 #pragma unroll
-        for (int kb = 0; kb < 4; ++kb) {
-            const char *pp = p + kb * 4096 + pr * 64 + lane * 16, *qq = q + kb * 4096 + qr * 64 + lane * 16;
-            const half8 ph = *(const half8*)pp, pl = *(const half8*)(pp + kLo);
-            const half8 qh = *(const half8*)qq, ql = *(const half8*)(qq + kLo);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ql, ph, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, pl, acc, 0, 0, 0);
-            acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qh, ph, acc, 0, 0, 0);
+        for (int kb = 0; kb < 2; ++kb) {
+            const int c = kb * 32 + (lane >> 4) * 8, pat = small_at(pr + (lane & 15), c);
+            const half8 ph = *(const half8*)(p + pat), pl = *(const half8*)(p + pat + kLo);
+            half8 qh[2], ql[2];
+            for (int t = 0; t < 2; ++t) {
+                const int qat = small_at(qr + t * 16 + (lane & 15), c);
+                qh[t] = *(const half8*)(q + qat);
+                ql[t] = *(const half8*)(q + qat + kLo);
+            }
+            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[t], ph, acc.t[t], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], pl, acc.t[t], 0, 0, 0);
+            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], ph, acc.t[t], 0, 0, 0);
         }
         return acc;
     };
-    const int row = wr + (lane & 31), col = wc + (lane >> 5) * 4;
-    auto store = [&](char* to, char* flip, const float16v& x) {      // pieces of the quadrant, and of its transpose where flip is given
-        for (int q = 0; q < 4; ++q) {
+    const int row = wr + (lane & 15), col = wc + (lane >> 4) * 4;
+    auto store = [&](char* to, char* flip, const Part& x) {  // pieces of the wave's part, and of its transpose where flip is given
+        for (int t = 0; t < 2; ++t) {
             half4 h, l;
-            split4({x[q * 4], x[q * 4 + 1], x[q * 4 + 2], x[q * 4 + 3]}, h, l);
-            const long at = piece_at(row, col + q * 8, 2);
+            split4({x.t[t][0], x.t[t][1], x.t[t][2], x.t[t][3]}, h, l);
+            const int at = small_at(row, col + t * 16);
             *(half4*)(to + at) = h;
             *(half4*)(to + at + kLo) = l;
             if (flip)
                 for (int e = 0; e < 4; ++e) {
-                    const long t = piece_at(col + q * 8 + e, row, 2);
-                    *(f16*)(flip + t) = h[e];
-                    *(f16*)(flip + t + kLo) = l[e];
+                    const int to = small_at(col + t * 16 + e, row);
+                    *(f16*)(flip + to) = h[e];
+                    *(f16*)(flip + to + kLo) = l[e];
                 }
         }
     };
     for (int k = 0; k < st.n; ++k) {
         __syncthreads();
-        float16v A = multiply(xs, wr, xs, wc);
-        for (int i = 0; i < 16; ++i) A[i] *= kInvScale * f * f;
+        Part A = multiply(xs, wr, xs, wc);
+        for (int t = 0; t < 2; ++t) A.t[t] *= kInvScale * f * f;
         store(as, nullptr, A);
         __syncthreads();
-        float16v B = multiply(as, wr, as, wc);
+        Part B = multiply(as, wr, as, wc);
         const float diag = row < d.m ? st.a[k] * kScale : 0.f;
-        for (int i = 0; i < 16; ++i) {
-            B[i] = fmaf(st.c[k] * kInvScale, B[i], st.b[k] * A[i]);
-            B[i] += row == col + (i >> 2) * 8 + (i & 3) ? diag : 0.f;
-        }
+        for (int t = 0; t < 2; ++t)
+            for (int e = 0; e < 4; ++e) {
+                B.t[t][e] = fmaf(st.c[k] * kInvScale, B.t[t][e], st.b[k] * A.t[t][e]);
+                B.t[t][e] += row == col + t * 16 + e ? diag : 0.f;
+            }
         store(bs, nullptr, B);
         __syncthreads();
         if (k + 1 < st.n) {
-            float16v X = multiply(bs, wr, xts, wc);
+            Part X = multiply(bs, wr, xts, wc);
             const float f1 = fminf(1.f, f * st.grow[k]);
-            for (int i = 0; i < 16; ++i) X[i] *= kInvScale * (f / f1);
+            for (int t = 0; t < 2; ++t) X.t[t] *= kInvScale * (f / f1);
             f = f1;
             __syncthreads();                                 // everybody has read X^T
             store(xs, xts, X);
         }
     }
     if (skip) return;
-    const float16v X = d.tall ? multiply(xts, wr, bs, wc) : multiply(bs, wr, xts, wc);
+    const Part X = d.tall ? multiply(xts, wr, bs, wc) : multiply(bs, wr, xts, wc);
     if (row >= a.rows) return;
-    for (int q = 0; q < 4; ++q) {
+    for (int t = 0; t < 2; ++t) {
         float val[4];
-        for (int e = 0; e < 4; ++e) val[e] = X[q * 4 + e] * (kInvScale * kInvScale * f);
-        if (col + q * 8 < a.cols) put4<O, kMuon>(a, mat, row, col + q * 8, val);
+        for (int e = 0; e < 4; ++e) val[e] = X.t[t][e] * (kInvScale * kInvScale * f);
+        if (col + t * 16 < a.cols) put4<O, kMuon>(a, mat, row, col + t * 16, val);
     }
 }
 
@@ -784,7 +802,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     g.step = kMuon ? (float)(a.opts->lr * a.opts->scale) : 1.f;
     g.vec = vec_out;
     if (pl.small) {
-        small_kernel<O, kMuon><<<dim3(a.count), kThreads, 0, s>>>(g, d, st, a.ns->eps, mu, nesterov);
+        small_kernel<O, kMuon><<<dim3(a.count), kSmall, 0, s>>>(g, d, st, a.ns->eps, mu, nesterov);
         return hipGetLastError();
     }
     const long xb = d.mp * d.np * 4, ab = d.mp * d.mp * 4;
