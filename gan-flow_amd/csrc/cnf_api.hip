@@ -896,6 +896,9 @@ int cnf_orthogonalize(const void* const* g, int64_t ldg, void* const* out, int64
     if (check_ptrs(who, "g", g, count, rows, cols, ldg, elem_bytes(dtype)) ||
         check_ptrs(who, "out", out, count, rows, cols, ldo, elem_bytes(dtype)))
         return 1;
+    for (int64_t i = 0; i < count; ++i)
+        for (int64_t j = 0; j < i; ++j)
+            if (out[i] == out[j]) return fail("%s: matrices %ld and %ld have the same output", who, (long)j, (long)i);
     cnf::MuonArgs a{};
     a.g = g;
     a.ldg = ldg;
@@ -930,6 +933,10 @@ int cnf_muon_step(void* const* params, int64_t ldp, const void* const* grads, in
         for (int64_t j = 0; j < i; ++j)
             if (params[i] == params[j] || momenta[i] == momenta[j])
                 return fail("%s: matrices %ld and %ld are the same parameter or momentum", who, (long)j, (long)i);
+    for (int64_t i = 0; i < count; ++i)                      // (a gradient may be its own parameter: it is read before that is written)
+        for (int64_t j = 0; j < count; ++j)
+            if (grads[i] == momenta[j] || params[i] == momenta[j])
+                return fail("%s: momentum %ld is also a gradient or a parameter", who, (long)j);
     cnf::MuonArgs a{};
     a.g = grads;
     a.ldg = ldg;

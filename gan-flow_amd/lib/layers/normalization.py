@@ -122,7 +122,8 @@ class _LayerNormFn(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis of x: (x - mean) / sqrt(var + eps) * weight + bias, one HIP kernel forward and
     backward (gan-flow_amd/csrc/cnf_norm.hip).  x: fp32, fp16 or bf16 on a HIP device, any leading axes, weight and bias of
-    x's type or fp32, or None.  Statistics and the sums of the weight gradients are fp32.  Differentiable once."""
+    x's type or fp32, or None.  Statistics and the sums of the weight gradients are fp32.  Differentiable once.  Capturable; as with
+    every autograd function, drop the outputs of eager passes over the same leaves before a backward pass is captured."""
     if not torch.is_tensor(x) or x.dim() == 0:
         raise _native.CnfError("x must be a tensor with at least one axis (got %s)" % (getattr(x, "shape", type(x)),))
     x2 = x if x.dim() == 2 else x.reshape(-1 if x.numel() else x[..., 0].numel(), x.shape[-1])

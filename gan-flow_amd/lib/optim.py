@@ -57,7 +57,7 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
     if not len(params) == len(grads) == len(momenta):
         raise _native.CnfError("%d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
     ns = _native.ns_params(steps, coefficients, eps)
-    groups, seen, given = {}, set(), 0
+    groups, seen, given, owned = {}, set(), 0, set()
     for p, g, m in zip(params, grads, momenta):
         for name, t in (("params", p), ("grads", g), ("momenta", m)):
             if not torch.is_tensor(t) or not t.is_cuda or t.dim() != 2:
@@ -70,15 +70,19 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
             g = g.contiguous()
             gs = g.stride()
         seen.update((p.data_ptr(), m.data_ptr()))
+        owned.add(m.data_ptr())
         given += 2
         groups.setdefault((p.shape, p.dtype, p.device, p.stride(), gs, m.stride()), []).append((p, g, m))
     if len(seen) != given:
         raise _native.CnfError("the same parameter or momentum is given twice")
+    if not owned.isdisjoint([g.data_ptr() for g in grads]):
+        raise _native.CnfError("a gradient is also a momentum")
     for key, members in groups.items():
         step = _at_once(len(members), *key[0])
         for lo in range(0, len(members), step):
             ps, gs, ms = zip(*members[lo:lo + step])
             _native.muon_step(ps, gs, ms, ns, lr, momentum, nesterov, weight_decay, scale, guard)
+            torch.autograd.graph.increment_version([t for t in ps + ms if not t.is_inference()])   # (written through raw pointers)
 
 
 def adjusted_scale(how, rows, cols):
@@ -141,7 +145,6 @@ class Muon(torch.optim.Optimizer):
                 muon_step(ps, gs, ms, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
                           weight_decay=group["weight_decay"], scale=adjusted_scale(group["adjust_lr"], *shape), steps=group["ns_steps"],
                           coefficients=group["ns_coefficients"], eps=group["eps"])
-                torch.autograd.graph.increment_version(ps)   # (written through raw pointers: autograd is told)
         return loss
 
 

@@ -372,7 +372,7 @@ int cnf_orthogonalize(const void *const *g, int64_t ldg, void *const *out, int64
 /* One Muon update of `count` matrices of one shape, in place:
  *     M <- momentum M + g;   U = g + momentum M (nesterov) or M;   W <- (1 - lr weight_decay) W - lr scale NS(U)
  *   params, grads: matrices of type dtype;  momenta: fp32 whatever dtype is (a state: never rounded to fewer bits).
- *   workspace as above.  guard (nullable): as in cnf_adam_step, a non-zero status there changes nothing.                */
+ *   No matrix overlaps another (grads[i] may be params[i]).  workspace as above.  guard (nullable): as in cnf_adam_step, a non-zero status there changes nothing.                */
 typedef struct CnfMuonOpts {
     double lr, momentum, weight_decay, scale;
     int32_t nesterov;    /* 0 | 1 */

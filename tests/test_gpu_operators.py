@@ -270,6 +270,21 @@ def test_layer_norm_on_another_stream_and_in_a_graph():
             assert all(torch.equal(p, q) for p, q in zip(want, out))
 
 
+def test_layer_norm_past_two_to_the_31_elements():
+    rows, cols = (1 << 20) + 5, 2051
+    assert rows * cols > 1 << 31
+    g = torch.Generator(device=DEV).manual_seed(31)
+    x, dy = (torch.randn(rows, cols, generator=g, device=DEV, dtype=F16) for _ in range(2))
+    w, b = (torch.randn(cols, generator=g, device=DEV, dtype=F16) for _ in range(2))
+    from gan_flow_amd.lib.layers import layer_norm
+    x.requires_grad_()
+    y = layer_norm(x, w, b)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for part in (slice(0, 3), slice(rows // 2, rows // 2 + 40), slice(rows - 60, rows)):
+        for name, got, (want, tol) in zip(("y", "dx"), (y.detach()[part], dx[part]), norm_reference(x.detach()[part], w, b, 1e-5, dy[part], F16, F16)):
+            check(got, want, tol, "%s, rows %s" % (name, part))
+
+
 # ---- Newton-Schulz orthogonalisation --------------------------------------------------------------------------------------
 
 COEF = (3.4445, -4.7750, 2.0315)
@@ -451,6 +466,37 @@ def test_muon_step_of_strided_blocks_leaves_the_rest():
     for w, w0, g0, m0 in zip(block(bufs[0]), block(before[0]), block(before[1]), block(before[2])):
         want, tol, _ = muon_reference(w0, g0, m0, 0.1, 0.95, True, 0.1, 1.0, F32)
         assert (w.double() - want).norm().item() <= tol
+
+
+def test_muon_step_in_a_buffer_past_two_to_the_31_elements():
+    from gan_flow_amd.lib.optim import muon_step
+    rows, ld, cols = 33100, 65536, 48
+    assert rows * ld > 1 << 31
+    gen = torch.Generator(device=DEV).manual_seed(32)
+    w, g, m = (torch.zeros(rows, ld, dtype=t, device=DEV)[:, 5:5 + cols] for t in (F16, F16, F32))
+    for t in (w, g, m):
+        t.copy_(torch.randn(rows, cols, generator=gen, device=DEV))
+    w0, m0 = w.clone(), m.clone()
+    muon_step([w], [g], [m], lr=0.1, weight_decay=0.05, scale=3.0)
+    want, tol, m1 = muon_reference(w0, g, m0, 0.1, 0.95, True, 0.05, 3.0, F16)
+    check(m, m1, 3 * U * (m0.double().abs() + g.double().abs()), "momentum")
+    assert (w.double() - want).norm().item() <= tol
+
+
+def test_muon_step_tells_autograd_and_refuses_a_momentum_as_gradient():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.optim import muon_step
+    w, m = torch.randn(70, 80, device=DEV), torch.zeros(70, 80, device=DEV)
+    g = torch.randn(70, 80, device=DEV)
+    before = w._version, m._version, g._version
+    muon_step([w], [g], [m])
+    assert w._version > before[0] and m._version > before[1] and g._version == before[2]
+    with pytest.raises(CnfError, match="also a momentum"):
+        muon_step([w], [m], [m])
+    with pytest.raises(CnfError, match="given twice"):
+        muon_step([w], [g], [w])
+    with torch.inference_mode():
+        muon_step([w.clone()], [g.clone()], [m.clone()])
 
 
 def test_muon_step_guard_and_refusals():

@@ -140,6 +140,22 @@ def test_muon_step_refuses_the_same_matrix_twice():
         assert rc != 0 and b"same parameter" in lib.cnf_last_error()
 
 
+def test_muon_step_refuses_a_momentum_that_is_something_else():
+    from gan_flow_amd import _native as nat
+    lib = nat.load_library()
+    o = nat.CnfMuonOpts(1e-3, 0.95, 0.1, 1.0, 1, 0)
+    for p, g, m in ((_ptrs(4096, 8192), _ptrs(1 << 20, 1 << 21), _ptrs(1 << 22, 1 << 20)), (_ptrs(4096, 8192), _ptrs(1 << 20, 1 << 21), _ptrs(8192, 1 << 22))):
+        rc = lib.cnf_muon_step(p, 8, g, 8, m, 8, 0, 2, 4, 8, ctypes.byref(o), ctypes.byref(_ns(nat)), None, ONE, 1 << 30, None)
+        assert rc != 0 and b"also a gradient or a parameter" in lib.cnf_last_error()
+
+
+def test_orthogonalize_refuses_one_output_for_two_matrices():
+    from gan_flow_amd import _native as nat
+    lib = nat.load_library()
+    rc = lib.cnf_orthogonalize(_ptrs(4096, 8192), 8, _ptrs(1 << 20, 1 << 20), 8, 0, 2, 4, 8, ctypes.byref(_ns(nat)), ONE, 1 << 30, None)
+    assert rc != 0 and b"same output" in lib.cnf_last_error()
+
+
 def test_python_entry_points_refuse_host_tensors():
     from gan_flow_amd import CnfError
     from gan_flow_amd.lib.layers import LayerNorm, layer_norm
