@@ -618,3 +618,73 @@ def test_normalised_network_trained_with_muon():
         loss.backward()
         muon.step(), adam.step()
     assert torch.isfinite(loss)
+
+
+def test_calls_on_two_streams_at_once():
+    """Two streams busy with calls of their own, each result the bits of the same call alone."""
+    from gan_flow_amd.lib.layers import layer_norm
+    from gan_flow_amd.lib.optim import muon_step, orthogonalize
+    gen = torch.Generator().manual_seed(77)
+    gs = [torch.randn(c, r, n, generator=gen).to(DEV) for c, r, n in ((3, 300, 200), (2, 64, 40), (1, 700, 900))]
+    x = torch.randn(500, 900, generator=gen).to(DEV)
+    w, m = torch.randn(300, 200, generator=gen).to(DEV), torch.randn(300, 200, generator=gen).to(DEV)
+
+    def work():
+        w1, m1 = w.clone(), m.clone()
+        muon_step([w1], [gs[0][0]], [m1])
+        return [orthogonalize(g) for g in gs] + [layer_norm(x), w1, m1]
+
+    want = work()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(work())
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(torch.equal(p, q) for p, q in zip(want, out))
+
+
+def test_training_step_of_a_normalised_layer_captured_and_replayed():
+    """Forward, backward through autograd and the Muon update of one layer in one captured graph, against the eager steps."""
+    from gan_flow_amd.lib.layers import layer_norm
+    from gan_flow_amd.lib.optim import muon_step
+    gen = torch.Generator().manual_seed(78)
+    w0, s0, b0 = torch.randn(96, 130, generator=gen).to(DEV) / 10, torch.ones(96, device=DEV), torch.zeros(96, device=DEV)
+    xs = [torch.randn(200, 130, generator=gen).to(DEV) for _ in range(4)]
+    dy = torch.randn(200, 96, generator=gen).to(DEV)
+
+    def step(x, w, s, b, m):
+        y = layer_norm(x @ w.t(), s, b)
+        gw, gs, gb = torch.autograd.grad(y, (w, s, b), dy)
+        with torch.no_grad():
+            muon_step([w], [gw], [m], lr=0.02)
+            s.sub_(gs, alpha=0.01), b.sub_(gb, alpha=0.01)
+        return y.detach()
+
+    def leaves():
+        return [t.clone().requires_grad_() for t in (w0, s0, b0)] + [torch.zeros_like(w0)]
+
+    eager = leaves()
+    want = [(step(x, *eager), [t.detach().clone() for t in eager]) for x in xs]
+    mine, x = leaves(), torch.empty_like(xs[0])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(xs[0], *mine)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(x, *mine)
+    with torch.no_grad():
+        for t, v in zip(mine, (w0, s0, b0, torch.zeros_like(w0))):
+            t.copy_(v)
+    for k, xk in enumerate(xs):
+        x.copy_(xk)
+        graph.replay()
+        torch.cuda.synchronize()
+        layer_norm(xk)                                        # eager work between the replays
+        assert torch.equal(out, want[k][0])
+        assert all(torch.equal(t.detach(), v) for t, v in zip(mine, want[k][1]))
