@@ -570,7 +570,7 @@ class _at:
         self.index = device.index
 
     def __enter__(self):
-        self.was = torch.cuda.current_device()
+        self.was = _CURRENT_DEVICE()
         if self.was != self.index:
             torch.cuda.set_device(self.index)
         return torch.cuda.current_stream(self.index).cuda_stream if _RAW_STREAM is None else _RAW_STREAM(self.index)
@@ -582,6 +582,7 @@ class _at:
 
 
 _RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (what torch.cuda.current_stream wraps; 0.1 against 2.7 us)
+_CURRENT_DEVICE = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _rows_of(t):
@@ -596,14 +597,16 @@ def _rows_of(t):
 def _norm_weight(t, name, x):
     if t is None:
         return None
-    _elem(t, name, (torch.float32, x.dtype))
-    if t.shape != x.shape[1:] or t.device != x.device:
+    if not torch.is_tensor(t) or not t.is_cuda or t.dtype not in (torch.float32, x.dtype):
+        _elem(t, name, (torch.float32, x.dtype))
+    if t.dim() != 1 or t.shape[0] != x.shape[1] or t.device != x.device:
         raise CnfError("%s must have shape (%d,) on %s (got %s on %s)" % (name, x.shape[1], x.device, tuple(t.shape), t.device))
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _norm_args(x, weight, bias):
-    _elem(x, "x")
+    if not torch.is_tensor(x) or not x.is_cuda or x.dtype not in DTYPE_IDS:
+        _elem(x, "x")
     if x.dim() != 2 or x.shape[1] == 0:
         raise CnfError("x must be (rows, cols) with cols > 0 (got %s)" % (tuple(x.shape),))
     weight, bias = _norm_weight(weight, "weight", x), _norm_weight(bias, "bias", x)
@@ -626,8 +629,8 @@ def norm_forward(x, weight, bias, eps, want_stats):
     x, stride = _rows_of(x)
     rows, cols = x.shape
     dt, dev = x.dtype, x.device
-    y = torch.empty((rows, cols), dtype=dt, device=dev)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=dev) if want_stats else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    stats = x.new_empty((2, rows), dtype=torch.float32) if want_stats else None
     mean = stats.data_ptr() if want_stats else None
     with _at(dev) as stream:
         rc = lib.cnf_layer_norm_fwd(x.data_ptr(), stride, DTYPE_IDS[dt], _addr(weight), _addr(bias), DTYPE_IDS[wd], rows, cols, float(eps),
@@ -644,13 +647,13 @@ def norm_backward(dy, x, weight, wd, mean_ptr, rstd_ptr, want):
     dy, dy_stride = _rows_of(dy)
     rows, cols = x.shape
     dt, dev = x.dtype, x.device
-    dx = torch.empty((rows, cols), dtype=dt, device=dev) if want[0] else None
-    dw = torch.empty(cols, dtype=wd, device=dev) if want[1] else None
-    db = torch.empty(cols, dtype=wd, device=dev) if want[2] else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if want[0] else None
+    dw = x.new_empty(cols, dtype=wd) if want[1] else None
+    db = x.new_empty(cols, dtype=wd) if want[2] else None
     if dx is None and dw is None and db is None:
         return None, None, None
     need = lib.cnf_layer_norm_workspace_bytes(rows, cols) if want[1] or want[2] else 0
-    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
     with _at(dev) as stream:
         rc = lib.cnf_layer_norm_bwd(dy.data_ptr(), dy_stride, x.data_ptr(), x_stride, DTYPE_IDS[dt], _addr(weight), DTYPE_IDS[wd],
                                     mean_ptr, rstd_ptr, rows, cols, _addr(dx), _addr(dw), _addr(db), _addr(ws), need, stream)
