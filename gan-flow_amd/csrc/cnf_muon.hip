@@ -81,6 +81,14 @@ __device__ __forceinline__ void split4(const float (&v)[4], half4& hi, half4& lo
     lo = __builtin_shufflevector(l0, l1, 0, 1, 2, 3);
 }
 
+__device__ __forceinline__ void split8(const float (&v)[8], half8& hi, half8& lo) {
+    half4 h0, l0, h1, l1;
+    split4({v[0], v[1], v[2], v[3]}, h0, l0);
+    split4({v[4], v[5], v[6], v[7]}, h1, l1);
+    hi = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
+    lo = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+
 // four neighbouring elements of a row, or the last ones of it
 template <typename T, bool kVec>
 __device__ __forceinline__ void load4(const T* p, long left, float (&v)[4]) {
@@ -148,6 +156,30 @@ __device__ __forceinline__ double start_scale(double norm, double eps, float& f)
     return (double)kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
 }
 
+// s before every step
+__device__ __forceinline__ void put_factors(float* to, float f, const Steps& st) {
+    for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
+        to[k] = f;
+        if (k < st.n) f = fminf(1.f, f * st.grow[k]);
+    }
+}
+
+// four neighbouring elements of X0 times 2^10: zeros outside G (what is outside is read at its last row and not used)
+template <typename T, bool kMuon, bool kVec>
+__device__ __forceinline__ void start_values(const Ptrs& p, const Dims& d, int mat, long row, long c, float mu, int nesterov, double scale, float (&v)[4]) {
+    const long r = min(row, d.rows - 1), left = d.cols - c;  // columns from here on
+    float m[4] = {};
+    for (int k = 0; k < 4; ++k) v[k] = 0.f;
+    if (left > 0) {
+        load4<T, kVec>((const T*)p.g[mat] + r * d.ldg + c, left, v);
+        if (kMuon) load4<float, kVec>(p.m[mat] + r * d.ldm + c, left, m);        // the new momentum
+    }
+    for (int k = 0; k < 4; ++k) {
+        const float u = kMuon ? (nesterov ? fmaf(mu, m[k], v[k]) : m[k]) : v[k];
+        v[k] = row < d.rows ? (float)((double)u * scale) : 0.f;
+    }
+}
+
 // X0 = G / (|G| + eps) as the piece matrices X (m x n) and X^T (n x m); one 64 x 64 tile of G per workgroup, through LDS.  Thread (tr, tc)
 // loads columns 4 tc .. of rows tr, tr + 16, ..; what is outside G is read at its last row and not used.
 template <typename T, bool kMuon, bool kVec>
@@ -177,10 +209,7 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
     // (double: the largest and smallest fp32 gradients have a scale outside fp32)
     const double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
-        for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
-            factors[mat * (CNF_NS_MAX_STEPS + 1) + k] = f;
-            if (k < st.n) f = fminf(1.f, f * st.grow[k]);
-        }
+        put_factors(factors + mat * (CNF_NS_MAX_STEPS + 1), f, st);
     for (int i = 0; i < 4; ++i) {
         const bool in = r0 + tr + i * 16 < d.rows;
         for (int k = 0; k < 4; ++k) {
@@ -198,13 +227,12 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
         const int i = e & 63, q = (e >> 6 & 7) * 8;
         float w[8];
         for (int k = 0; k < 8; ++k) w[k] = e < 512 ? tile[i][q + k] : tile[q + k][i];
-        half4 h0, l0, h1, l1;
-        split4({w[0], w[1], w[2], w[3]}, h0, l0);
-        split4({w[4], w[5], w[6], w[7]}, h1, l1);
+        half8 h, l;
+        split8(w, h, l);
         char* base = e < 512 ? straight : flipped;
         const long at = e < 512 ? piece_at(r0 + i, c0 + q, kc_s) : piece_at(c0 + i, r0 + q, kc_f);
-        *(half8*)(base + at) = __builtin_shufflevector(h0, h1, 0, 1, 2, 3, 4, 5, 6, 7);
-        *(half8*)(base + at + kLo) = __builtin_shufflevector(l0, l1, 0, 1, 2, 3, 4, 5, 6, 7);
+        *(half8*)(base + at) = h;
+        *(half8*)(base + at + kLo) = l;
     }
 }
 
@@ -570,6 +598,48 @@ __device__ __forceinline__ int small_at(int r, int c) {
     return ((c >> 4) << 12) + ((r >> 5) << 11) + ((c >> 3 & 1) << 9) + (((r & 31) ^ (c >> 3)) << 4) + ((c & 7) << 1);
 }
 
+// rows pr .. + 15 and columns qr .. + 31 of sum_k P[r][k] Q[c][k], k = 0 .. 63: a lane holds columns 16 t + 4 (lane / 16) + e of row lane % 16
+struct Part { float4v t[2]; };
+
+__device__ __forceinline__ void multiply64(Part& acc, const char* p, int pr, const char* q, int qr, int lane) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        const int c = kb * 32 + (lane >> 4) * 8, pat = small_at(pr + (lane & 15), c);
+        const half8 ph = *(const half8*)(p + pat), pl = *(const half8*)(p + pat + kLo);
+        half8 qh[2], ql[2];
+        for (int t = 0; t < 2; ++t) {
+            const int qat = small_at(qr + t * 16 + (lane & 15), c);
+            qh[t] = *(const half8*)(q + qat);
+            ql[t] = *(const half8*)(q + qat + kLo);
+        }
+        for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[t], ph, acc.t[t], 0, 0, 0);
+        for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], pl, acc.t[t], 0, 0, 0);
+        for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], ph, acc.t[t], 0, 0, 0);
+    }
+}
+
+// pieces of a wave's part, whose lane has columns col + 16 t .. + 3 of `row`: in LDS, or (kMemory) in a piece matrix 64 columns wide
+template <bool kMemory = false>
+__device__ __forceinline__ void store64(char* to, const Part& x, int row, int col) {
+    for (int t = 0; t < 2; ++t) {
+        half4 h, l;
+        split4({x.t[t][0], x.t[t][1], x.t[t][2], x.t[t][3]}, h, l);
+        const long at = kMemory ? piece_at(row, col + t * 16, 2) : small_at(row, col + t * 16);
+        *(half4*)(to + at) = h;
+        *(half4*)(to + at + kLo) = l;
+    }
+}
+
+// a I + b A + c A^2 from A and, in B's place, the accumulator of A A
+__device__ __forceinline__ void poly64(Part& B, const Part& A, float a, float b, float c, int row, int col, long m) {
+    const float diag = row < m ? a * kScale : 0.f;
+    for (int t = 0; t < 2; ++t)
+        for (int e = 0; e < 4; ++e) {
+            B.t[t][e] = fmaf(c * kInvScale, B.t[t][e], b * A.t[t][e]);
+            B.t[t][e] += row == col + t * 16 + e ? diag : 0.f;
+        }
+}
+
 template <typename O, bool kMuon>
 __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Steps st, double eps, float mu, int nesterov) {
     __shared__ __align__(16) char xs[2 * kBlockBytes], xts[2 * kBlockBytes], as[2 * kBlockBytes], bs[2 * kBlockBytes];
@@ -620,56 +690,32 @@ __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Step
         *(half2*)(flipped + at + kLo) = (half2){l[0][k], l[1][k]};
     }
     const int wr = (wave >> 1) * 16, wc = (wave & 1) * 32;
-    struct Part { float4v t[2]; };
-    // rows pr .. + 15 and columns qr .. + 31 of sum_k P[r][k] Q[c][k]: a lane holds columns 16 t + 4 (lane / 16) + e of row lane % 16
     auto multiply = [&](const char* p, int pr, const char* q, int qr) {
         Part acc = {};
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            const int c = kb * 32 + (lane >> 4) * 8, pat = small_at(pr + (lane & 15), c);
-            const half8 ph = *(const half8*)(p + pat), pl = *(const half8*)(p + pat + kLo);
-            half8 qh[2], ql[2];
-            for (int t = 0; t < 2; ++t) {
-                const int qat = small_at(qr + t * 16 + (lane & 15), c);
-                qh[t] = *(const half8*)(q + qat);
-                ql[t] = *(const half8*)(q + qat + kLo);
-            }
-            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql[t], ph, acc.t[t], 0, 0, 0);
-            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], pl, acc.t[t], 0, 0, 0);
-            for (int t = 0; t < 2; ++t) acc.t[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh[t], ph, acc.t[t], 0, 0, 0);
-        }
+        multiply64(acc, p, pr, q, qr, lane);
         return acc;
     };
     const int row = wr + (lane & 15), col = wc + (lane >> 4) * 4;
-    auto store = [&](char* to, char* flip, const Part& x) {  // pieces of the wave's part, and of its transpose where flip is given
+    auto flip = [&](char* to, const Part& x) {               // pieces of the transpose of the wave's part
         for (int t = 0; t < 2; ++t) {
             half4 h, l;
             split4({x.t[t][0], x.t[t][1], x.t[t][2], x.t[t][3]}, h, l);
-            const int at = small_at(row, col + t * 16);
-            *(half4*)(to + at) = h;
-            *(half4*)(to + at + kLo) = l;
-            if (flip)
-                for (int e = 0; e < 4; ++e) {
-                    const int to = small_at(col + t * 16 + e, row);
-                    *(f16*)(flip + to) = h[e];
-                    *(f16*)(flip + to + kLo) = l[e];
-                }
+            for (int e = 0; e < 4; ++e) {
+                const int at = small_at(col + t * 16 + e, row);
+                *(f16*)(to + at) = h[e];
+                *(f16*)(to + at + kLo) = l[e];
+            }
         }
     };
     for (int k = 0; k < st.n; ++k) {
         __syncthreads();
         Part A = multiply(xs, wr, xs, wc);
         for (int t = 0; t < 2; ++t) A.t[t] *= kInvScale * f * f;
-        store(as, nullptr, A);
+        store64(as, A, row, col);
         __syncthreads();
         Part B = multiply(as, wr, as, wc);
-        const float diag = row < d.m ? st.a[k] * kScale : 0.f;
-        for (int t = 0; t < 2; ++t)
-            for (int e = 0; e < 4; ++e) {
-                B.t[t][e] = fmaf(st.c[k] * kInvScale, B.t[t][e], st.b[k] * A.t[t][e]);
-                B.t[t][e] += row == col + t * 16 + e ? diag : 0.f;
-            }
-        store(bs, nullptr, B);
+        poly64(B, A, st.a[k], st.b[k], st.c[k], row, col, d.m);
+        store64(bs, B, row, col);
         __syncthreads();
         if (k + 1 < st.n) {
             Part X = multiply(bs, wr, xts, wc);
@@ -677,7 +723,8 @@ __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Step
             for (int t = 0; t < 2; ++t) X.t[t] *= kInvScale * (f / f1);
             f = f1;
             __syncthreads();                                 // everybody has read X^T
-            store(xs, xts, X);
+            store64(xs, X, row, col);
+            flip(xts, X);
         }
     }
     if (skip) return;
@@ -688,6 +735,142 @@ __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Step
         for (int e = 0; e < 4; ++e) val[e] = X.t[t][e] * (kInvScale * kInvScale * f);
         if (col + t * 16 < a.cols) put4<O, kMuon>(a, mat, row, col + t * 16, val);
     }
+}
+
+// Matrices whose shorter side is at most 64 and whose longer one is not.  A 64 x 64 tile of X is a whole block of columns, so the workgroup that
+// makes it adds its part of X X^T at once, and X itself is never stored (the next product reads X^T).  Five steps are seven launches instead of
+// twenty (64 x 1000: 42 us against 86).  `gram`: per matrix and workgroup the partial sums of X X^T as the waves hold them.  (Three steps at a time as
+// in run() would save two more launches, 33 us, but a step costs little here and the grouping two thirds of the accuracy:
+// 2.7e-6 against 0.9e-6 for 64 x 66, where plain fp32 is 1.2e-6 off.)
+// How many workgroups share the tiles of a matrix: more make shorter loops and longer sums.  A step of 64 x 1000 takes 5.9 us with 16 workgroups
+// and 6.8 with 8; 64 x 4096 14.8 with 8, 9.7 with 23, 13.1 with 64; 64 x 65536 94 with 16, 35 with 91.
+int skinny_parts(long tiles) {
+    const long n = (long)std::fmax(16., std::ceil(std::sqrt(8. * (double)tiles)));
+    return (int)(n < tiles ? n : tiles);
+}
+
+__device__ __forceinline__ void put_gram(float* gram, const Part& x, int wave, int lane) {
+    float4v* to = (float4v*)(gram + ((long)blockIdx.y * gridDim.x + blockIdx.x) * 4096 + wave * 512) + lane * 2;
+    to[0] = x.t[0], to[1] = x.t[1];
+}
+
+// 16 KB of a piece matrix 64 columns wide to LDS, in small_at's order
+__device__ __forceinline__ void fetch64(char* to, const char* from) {
+    for (int i = 0; i < 2; ++i) {
+        const int at = (i * kSmall + threadIdx.x) * 16, c8 = (at >> 12) * 2 + (at >> 9 & 1);
+        *(uint4*)(to + (at ^ c8 << 4)) = *(const uint4*)(from + at);
+    }
+}
+
+template <typename T, bool kMuon, bool kVec>
+__global__ __launch_bounds__(kSmall) void skinny_start_kernel(Ptrs p, Dims d, char* xt, const double* part, int parts, double eps, float mu,
+                                                              int nesterov, Steps st, float* factors, float* gram) {
+    __shared__ float tile[64][68];
+    __shared__ __align__(16) char xs[2 * kBlockBytes];
+    __shared__ double red[kSmall / 64];
+    const int mat = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int tr = threadIdx.x >> 4, tc = (threadIdx.x & 15) * 4, wr = (wave >> 1) * 16, wc = (wave & 1) * 32;
+    double s = 0.;
+    for (int k = threadIdx.x; k < parts; k += kSmall) s += part[mat * kNormBlocks + k];
+    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
+    if (lane == 0) red[wave] = s;
+    __syncthreads();
+    float f;
+    const double scale = start_scale(sqrt(((red[0] + red[1]) + (red[2] + red[3])) + ((red[4] + red[5]) + (red[6] + red[7]))), eps, f);
+    if (threadIdx.x == 0 && blockIdx.x == 0) put_factors(factors + mat * (CNF_NS_MAX_STEPS + 1), f, st);
+    xt += mat * d.np * (64 * 4);
+    Part acc = {};
+    for (long t = blockIdx.x; t * 64 < d.np; t += gridDim.x) {
+        const long r0 = d.tall ? t * 64 : 0, c = (d.tall ? 0 : t * 64) + tc;
+        for (int i = 0; i < 2; ++i) {
+            float v[4];
+            start_values<T, kMuon, kVec>(p, d, mat, r0 + tr + i * 32, c, mu, nesterov, scale, v);
+            *(float4*)&tile[tr + i * 32][tc] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+        __syncthreads();
+        const int i = threadIdx.x & 63, q = wave * 8;
+        for (int out = 0; out < 2; ++out) {                     // X to LDS, X^T to memory
+            float w[8];
+            for (int k = 0; k < 8; ++k) w[k] = (out == 0) != (d.tall != 0) ? tile[i][q + k] : tile[q + k][i];
+            half8 h, l;
+            split8(w, h, l);
+            char* to = out == 0 ? xs + small_at(i, q) : xt + t * (2 * kBlockBytes) + piece_at(i, q, 2);
+            *(half8*)to = h;
+            *(half8*)(to + kLo) = l;
+        }
+        __syncthreads();
+        multiply64(acc, xs, wr, xs, wc, lane);
+    }
+    put_gram(gram, acc, wave, lane);
+}
+
+// One step: every workgroup adds the partial sums of X X^T and makes Q = a I + b A + c A^2 of them; X <- Q X for its tiles: X^T to xt2 and
+// the partial sums of the new X X^T to gram2, or (kLast) X to the output.
+template <bool kLast, typename O, bool kMuon>
+__global__ __launch_bounds__(kSmall) void skinny_step_kernel(FinalArgs a, Dims d, Steps st, int k, const float* factors, const char* xt, char* xt2,
+                                                             const float* gram, float* gram2) {
+    __shared__ __align__(16) char as[2 * kBlockBytes], qs[2 * kBlockBytes], xts[2 * kBlockBytes];
+    char* const xs = as;                                     // (A is not needed once Q is there)
+    const int mat = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const int wr = (wave >> 1) * 16, wc = (wave & 1) * 32, row = wr + (lane & 15), col = wc + (lane >> 4) * 4;
+    const float f = factors[mat * (CNF_NS_MAX_STEPS + 1) + k];
+    const float scale = kInvScale * (kLast ? f * kInvScale : f / factors[mat * (CNF_NS_MAX_STEPS + 1) + k + 1]);
+    const bool skip = kLast && a.guard && a.guard->status != 0;
+    xt += mat * d.np * (64 * 4);
+    xt2 += mat * d.np * (64 * 4);
+    long t = blockIdx.x;
+    fetch64(xts, xt + t * (2 * kBlockBytes));
+    Part A = {};
+    const float4v* from = (const float4v*)(gram + (long)mat * gridDim.x * 4096 + wave * 512) + lane * 2;
+    const int sums = gridDim.x;
+    for (int w = 0; w < sums; w += 8) {                      // eight at a time on their way (past the last one: the last one again)
+        Part x[8];
+        for (int i = 0; i < 8; ++i)
+            for (int u = 0; u < 2; ++u) x[i].t[u] = from[min(w + i, sums - 1) * 1024 + u];
+        for (int i = 0; i < 8; ++i)
+            for (int u = 0; u < 2; ++u)
+                if (w + i < sums) A.t[u] += x[i].t[u];
+    }
+    for (int u = 0; u < 2; ++u) A.t[u] *= kInvScale * f * f;
+    store64(as, A, row, col);
+    __syncthreads();
+    Part Q = {}, acc = {};
+    multiply64(Q, as, wr, as, wc, lane);
+    poly64(Q, A, st.a[k], st.b[k], st.c[k], row, col, d.m);
+    store64(qs, Q, row, col);
+    __syncthreads();
+    while (true) {
+        const long next = t + gridDim.x;
+        Part X = {};
+        if (kLast) {
+            if (d.tall)                                      // the output's rows are X^T's
+                multiply64(X, xts, wr, qs, wc, lane);
+            else
+                multiply64(X, qs, wr, xts, wc, lane);
+            const long r = row + (d.tall ? t * 64 : 0);
+            for (int u = 0; u < 2; ++u) {
+                const long c = col + u * 16 + (d.tall ? 0 : t * 64);
+                float val[4];
+                for (int e = 0; e < 4; ++e) val[e] = X.t[u][e] * scale;
+                if (!skip && r < a.rows && c < a.cols) put4<O, kMuon>(a, mat, r, c, val);
+            }
+        } else {
+            Part Xt = {};
+            multiply64(X, qs, wr, xts, wc, lane);
+            multiply64(Xt, xts, wr, qs, wc, lane);
+            for (int u = 0; u < 2; ++u) X.t[u] *= scale, Xt.t[u] *= scale;
+            store64(xs, X, row, col);
+            store64<true>(xt2 + t * (2 * kBlockBytes), Xt, row, col);
+        }
+        if (kLast && next * 64 >= d.np) return;
+        __syncthreads();                                     // X^T is read, X is there
+        if (next * 64 < d.np) fetch64(xts, xt + next * (2 * kBlockBytes));
+        if (!kLast) multiply64(acc, xs, wr, xs, wc, lane);
+        if (next * 64 >= d.np) break;
+        t = next;
+        __syncthreads();
+    }
+    if (!kLast) put_gram(gram2, acc, wave, lane);
 }
 
 long pad_to(long v, long t) { return (v + t - 1) / t * t; }
@@ -727,6 +910,7 @@ struct Plan {
     long m, n;      // the shorter and the longer side
     int pm, pn;     // in panels of 64
     bool small;     // one workgroup per matrix does everything in LDS
+    bool skinny;    // the shorter side fits a tile: skinny_start_kernel and its like
     bool together;  // several steps at a time on the m x m side (decided for three steps, from the estimated times of the products)
 };
 
@@ -737,6 +921,7 @@ Plan plan_of(long count, long rows, long cols) {
     p.small = p.n <= 64;
     p.pm = (int)((p.m + 63) / 64);
     p.pn = (int)((p.n + 63) / 64);
+    p.skinny = !p.small && p.pm == 1;
     const double gram = choose(count, p.pm, p.pm, true, 2 * p.pn).time, sym = choose(count, p.pm, p.pm, true, 2 * p.pm).time,
                  full = choose(count, p.pm, p.pn, false, 2 * p.pm).time;
     p.together = gram + 9 * sym + full < 3 * (gram + sym + full);
@@ -807,9 +992,6 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
     }
     const long xb = d.mp * d.np * 4, ab = d.mp * d.mp * 4;
     double* part = (double*)a.ws;
-    char *x = (char*)(part + (size_t)a.count * kNormBlocks), *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *sym[5];
-    for (int i = 0; i < 5; ++i) sym[i] = xt2 + a.count * (xb + i * ab);
-    float* factors = (float*)(sym[pl.together ? 4 : 1] + a.count * ab);
     // partial sums: enough workgroups for the device, at least 2 K elements each
     long parts = (d.rows * d.cols + 2047) / 2048, most = (2048 + a.count - 1) / a.count;
     most = most < kNormBlocks ? most : kNormBlocks;
@@ -819,6 +1001,27 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         begin_kernel<O, kMuon, true><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
     else
         begin_kernel<O, kMuon, false><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
+    char* const data = (char*)(part + (size_t)a.count * kNormBlocks);
+    if (pl.skinny) {
+        const int n_parts = skinny_parts(pl.pn);
+        char *xt = data, *xt2 = xt + a.count * xb;
+        float *gram = (float*)(xt2 + a.count * xb), *gram2 = gram + (long)a.count * n_parts * 4096, *factors = gram2 + (long)a.count * n_parts * 4096;
+        const dim3 grid((unsigned)n_parts, a.count);
+        if (vec_in)
+            skinny_start_kernel<O, kMuon, true><<<grid, kSmall, 0, s>>>(p, d, xt, part, (int)parts, a.ns->eps, mu, nesterov, st, factors, gram);
+        else
+            skinny_start_kernel<O, kMuon, false><<<grid, kSmall, 0, s>>>(p, d, xt, part, (int)parts, a.ns->eps, mu, nesterov, st, factors, gram);
+        for (int k = 0; k + 1 < st.n; ++k) {
+            skinny_step_kernel<false, float, false><<<grid, kSmall, 0, s>>>(g, d, st, k, factors, xt, xt2, gram, gram2);
+            std::swap(xt, xt2);
+            std::swap(gram, gram2);
+        }
+        skinny_step_kernel<true, O, kMuon><<<grid, kSmall, 0, s>>>(g, d, st, st.n - 1, factors, xt, xt2, gram, gram2);
+        return hipGetLastError();
+    }
+    char *x = data, *xt = x + a.count * xb, *xt2 = xt + a.count * xb, *sym[5];
+    for (int i = 0; i < 5; ++i) sym[i] = xt2 + a.count * (xb + i * ab);
+    float* factors = (float*)(sym[pl.together ? 4 : 1] + a.count * ab);
     const long rp = d.tall ? d.np : d.mp, cp = d.tall ? d.mp : d.np;
     const dim3 tiles((unsigned)(cp / 64), (unsigned)(rp / 64), a.count);
     if (vec_in)
@@ -836,14 +1039,13 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
             g.c0 = x, g.b0 = xb;
             g.c1 = xt2, g.b1 = xb;
             product<kApply>(g, a.count, s);
-            char* t = xt;
-            xt = xt2;
-            xt2 = t;
+            std::swap(xt, xt2);
             return;
         }
         if (d.tall) {                                        // the output's rows are X^T's
-            g.p = xt, g.bp = xb, g.panels_p = pl.pn;
-            g.q = Q, g.bq = ab, g.panels_q = pl.pm;
+            std::swap(g.p, g.q);
+            std::swap(g.bp, g.bq);
+            std::swap(g.panels_p, g.panels_q);
         }
         product<kFinal, O, kMuon>(g, a.count, s);
     };
@@ -934,6 +1136,9 @@ size_t muon_workspace_bytes(long count, long rows, long cols) {
     const Plan p = plan_of(count, rows, cols);
     if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)
     const size_t m = p.pm * 64, n = p.pn * 64;
+    if (p.skinny)
+        return (size_t)count *
+               (kNormBlocks * sizeof(double) + 2 * m * n * 4 + (size_t)skinny_parts(p.pn) * (2 * 16384) + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
     return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + (p.together ? 5 : 2) * m * m) * 4 + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
 }
 

@@ -347,6 +347,30 @@ def test_orthogonalize_larger_launches(count, rows, cols, dtype):
         check_ns(out[i], g[i], "matrix %d" % i)
 
 
+@pytest.mark.parametrize("count, rows, cols", [(1, 50, 5000), (2, 5001, 64), (3, 64, 2100), (7, 1030, 3), (1, 33, 65536), (64, 20, 130)])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=lambda t: IDS[t])
+def test_orthogonalize_of_short_sides(count, rows, cols, dtype):
+    """One side of at most a tile, the other of many: several tiles a workgroup, workgroups without a full share."""
+    from gan_flow_amd.lib.optim import orthogonalize
+    wide = torch.randn(count, rows, cols + 3, generator=torch.Generator().manual_seed(count + rows)).to(DEV, dtype)
+    for g in (wide[..., :cols].contiguous(), wide[..., 3:]):
+        out = orthogonalize(g)
+        for i in sorted({0, count // 2, count - 1}):
+            check_ns(out[i], g[i], "matrix %d" % i)
+
+
+@pytest.mark.parametrize("rows, cols", [(40, 900), (900, 40), (3, 300)])
+@pytest.mark.parametrize("steps, coefficients", [(1, COEF), (2, COEF), (9, (2.0, -1.5, 0.5))])
+def test_orthogonalize_of_short_sides_in_other_steps(rows, cols, steps, coefficients):
+    from gan_flow_amd.lib.optim import orthogonalize
+    gen = torch.Generator().manual_seed(rows)
+    for scale in (1.0, 1e-12):                                # (the second far below eps)
+        g = (torch.randn(2, rows, cols, generator=gen) * scale).to(DEV)
+        out = orthogonalize(g, steps, coefficients)
+        for i in range(2):
+            check_ns(out[i], g[i], "matrix %d, scale %g" % (i, scale), steps=steps, coefficients=coefficients)
+
+
 @pytest.mark.parametrize("rows, cols", [(64, 64), (33, 50), (200, 90), (320, 320)])
 def test_orthogonalize_batches_and_strides(rows, cols):
     from gan_flow_amd.lib.optim import orthogonalize
