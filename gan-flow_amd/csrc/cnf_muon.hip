@@ -156,6 +156,19 @@ __device__ __forceinline__ double start_scale(double norm, double eps, float& f)
     return (double)kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
 }
 
+// A 16-bit matrix scaled by a power of two has no low pieces (but for what lies below 2^-34), and its first products are fewer by as much: the rest of the scale goes to s, which
+// is then at least 1/2 (4096 x 4096: 3360 us against 3525).  Not in Muon, where what is iterated is the fp32 momentum's.
+template <typename T, bool kMuon>
+constexpr bool kHighPieces = !kMuon && sizeof(T) == 2;
+
+__device__ __forceinline__ double power_of_two(double scale, float& f) {
+    if (scale == 0.) return scale;
+    int e;
+    const double rest = frexp(scale, &e);                    // 1/2 <= rest < 1
+    f = fmaxf((float)(f * rest), 1e-37f);
+    return ldexp(1., e);
+}
+
 // s before every step
 __device__ __forceinline__ void put_factors(float* to, float f, const Steps& st) {
     for (int k = 0; k <= CNF_NS_MAX_STEPS; ++k) {
@@ -207,7 +220,8 @@ __global__ __launch_bounds__(kThreads) void pieces_kernel(Ptrs p, Dims d, char* 
     __syncthreads();
     float f;
     // (double: the largest and smallest fp32 gradients have a scale outside fp32)
-    const double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
+    double scale = start_scale(sqrt((red[0] + red[1]) + (red[2] + red[3])), eps, f);
+    if (kHighPieces<T, kMuon>) scale = power_of_two(scale, f);
     if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0)
         put_factors(factors + mat * (CNF_NS_MAX_STEPS + 1), f, st);
     for (int i = 0; i < 4; ++i) {
@@ -324,24 +338,25 @@ __device__ __forceinline__ void my_tile(int tiles_r, int tiles_c, bool sym, int&
     }
 }
 
-// Operands of the products of 16 k: kNu x kNv tiles of 32 x 32
-template <int kNu, int kNv>
+// Operands of the products of 16 k: kNu x kNv tiles of 32 x 32.  kTerms: 3 products of pieces, or 2 where Q has no low pieces, or 1 where P has none either
+template <int kNu, int kNv, int kTerms>
 struct Frag {
+    static constexpr int kReads = (kTerms > 1 ? 2 : 1) * kNu + (kTerms > 2 ? 2 : 1) * kNv;
     half8 ph[kNu], pl[kNu], qh[kNv], ql[kNv];
     // p, q: the first of the wave's fragments of either operand, in LDS or in memory
     __device__ __forceinline__ void read(const char* p, const char* q, int lane) {
         for (int v = 0; v < kNv; ++v) {
-            ql[v] = *(const half8*)(q + v * 2048 + kLo + lane * 16);
+            if (kTerms > 2) ql[v] = *(const half8*)(q + v * 2048 + kLo + lane * 16);
             qh[v] = *(const half8*)(q + v * 2048 + lane * 16);
         }
         for (int u = 0; u < kNu; ++u) {
             ph[u] = *(const half8*)(p + u * 2048 + lane * 16);
-            pl[u] = *(const half8*)(p + u * 2048 + kLo + lane * 16);
+            if (kTerms > 1) pl[u] = *(const half8*)(p + u * 2048 + kLo + lane * 16);
         }
     }
     // operands exchanged: a lane gets four neighbouring columns of a row of C
     __device__ __forceinline__ void multiply(float16v (&acc)[kNu][kNv]) const {
-        for (int j = 0; j < 3; ++j)                          // lo hi, hi lo, hi hi: the three on one tile as far apart as they can be
+        for (int j = 3 - kTerms; j < 3; ++j)                          // lo hi, hi lo, hi hi: the three on one tile as far apart as they can be
             for (int u = 0; u < kNu; ++u)
                 for (int v = 0; v < kNv; ++v)
                     acc[u][v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(j == 0 ? ql[v] : qh[v], j == 1 ? pl[u] : ph[u], acc[u][v], 0, 0, 0);
@@ -433,7 +448,7 @@ __device__ __forceinline__ float scale_of(const ArgsOf<kMode>& a, int mat) {
 // registers kAhead steps before it needs them, and the partial sums are added at the end, in a fixed order.  The waves share no operands,
 // so LDS would only add its own traffic: four matrices' 1024 x 1024 x 1024 symmetric products take 24 us, and 27 with operands copied to LDS
 // (by one, two or four waves, which then wait for LDS).  What bounds it is the operands' way from L2, 16 TB/s.
-template <int kMode, typename O = float, bool kMuon = false>
+template <int kMode, int kTerms, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__(256) void tile64_kernel(ArgsOf<kMode> a) {
     constexpr int kW = 4, kAhead = 4;
     __shared__ __align__(16) char lds[49152];                // partial sums: [quadrant][other wave][register][lane]; then finish()'s
@@ -444,7 +459,7 @@ __global__ __launch_bounds__(256) void tile64_kernel(ArgsOf<kMode> a) {
     const char* qs = a.q + mat * a.bq + (long)tj * a.kc * kBlockBytes + wave * 4096;
     const int steps = 2 * a.kc / kW;                         // (kc is even)
     float16v acc[2][2] = {};
-    Frag<2, 2> f[kAhead];
+    Frag<2, 2, kTerms> f[kAhead];
     auto load = [&](int d, int s) { f[d].read(ps + (long)s * (kW * 4096), qs + (long)s * (kW * 4096), lane); };
 #pragma unroll
     for (int d = 0; d < kAhead; ++d)
@@ -494,7 +509,7 @@ __global__ __launch_bounds__(256) void tile64_kernel(ArgsOf<kMode> a) {
 // between the products.  4096 x 4096 x 4096 with T = 256: 300 us (1.38 PFLOP/s of piece products; a large library product of fp16 matrices: 1.35),
 // against 374 with reads and products in turn and 335 with the copies under a condition; the products alone, on operands that
 // stay in registers, take 252 us: the device's power limit (177 with zeros for operands).
-template <int T, int kNu, int kNv, int kStages, int kMode, typename O = float, bool kMuon = false>
+template <int T, int kNu, int kNv, int kStages, int kMode, int kTerms, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_kernel(ArgsOf<kMode> a) {
     constexpr int kAcross = T / 32 / kNv, kW = T / 32 / kNu * kAcross, kStage = 2 * T * 128, kLoads = kStage / 1024 / kW;
     constexpr bool kDealt = T < 256;
@@ -517,7 +532,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     };
     const int wr = (wave / kAcross) * kNu * 32, wc = (wave % kAcross) * kNv * 32;
     float16v acc[kNu][kNv] = {};
-    Frag<kNu, kNv> f0, f1;
+    Frag<kNu, kNv, kTerms> f0, f1;
     for (int k = 0; k < kStages && k < a.kc; ++k) load(k);
     if (kStages <= a.kc)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"((kStages - 1) * kLoads) : "memory");
@@ -526,7 +541,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     f0.read(lds[0] + wr * 64, lds[0] + (T + wc) * 64, lane);
-    constexpr int kReads = 2 * (kNu + kNv), kMul = 3 * kNu * kNv;
+    constexpr int kReads = f0.kReads, kMul = kTerms * kNu * kNv;
     int k = 0;
     for (; k < a.kc - kStages; ++k) {
         f1.read(lds[k % kStages] + (2 * T + wr) * 64, lds[k % kStages] + (3 * T + wc) * 64, lane);
@@ -536,7 +551,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
                 __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(kSchedMfma, kMul - kReads, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, kMul, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         // the next stage has landed (the kStages - 2 after it may be on their way), and every wave has read this one
@@ -548,7 +563,7 @@ __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_ker
         load(k + kStages);
         f1.multiply(acc);
         if (kDealt) {
-            for (int i = 0; i < kReads / 2; ++i) {
+            for (int i = 0; i < (kReads + 1) / 2; ++i) {
                 __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 2, 0);
                 __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
             }
@@ -937,20 +952,20 @@ int steps_together(const Plan& p, int steps, const double (&grow)[CNF_NS_MAX_STE
     return n;
 }
 
-template <int kMode, typename O = float, bool kMuon = false>
+template <int kMode, int kTerms = 3, typename O = float, bool kMuon = false>
 void product(const FinalArgs& g, int count, hipStream_t s) {
     const Choice how = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>, g.kc);
     const int t = how.tile / 64;
     const long r = (g.panels_p + t - 1) / t, c = (g.panels_q + t - 1) / t;
     const dim3 grid((unsigned)(count * (kSymmetric<kMode> ? r * (r + 1) / 2 : r * c)));
     if (how.tile == 256)
-        tile_kernel<256, 4, 2, 2, kMode, O, kMuon><<<grid, 512, 0, s>>>(g);
+        tile_kernel<256, 4, 2, 2, kMode, kTerms, O, kMuon><<<grid, 512, 0, s>>>(g);
     else if (how.tile == 192)
-        tile_kernel<192, 3, 3, 3, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+        tile_kernel<192, 3, 3, 3, kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
     else if (how.tile == 128)
-        tile_kernel<128, 2, 2, 2, kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+        tile_kernel<128, 2, 2, 2, kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
     else
-        tile64_kernel<kMode, O, kMuon><<<grid, 256, 0, s>>>(g);
+        tile64_kernel<kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
 }
 
 template <typename O, bool kMuon>
@@ -966,6 +981,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         st.grow[k] = (float)fmax(1., grow[k]);
     }
     const Plan pl = plan_of(a.count, a.rows, a.cols);
+    constexpr bool kHigh = kHighPieces<O, kMuon>;
     Ptrs p{};
     bool vec_in = a.cols % 4 == 0 && a.ldg % 4 == 0 && (!kMuon || a.ldm % 4 == 0), vec_out = a.ldo % 4 == 0;
     for (int i = 0; i < a.count; ++i) {
@@ -1038,7 +1054,10 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         if (k + n < st.n) {
             g.c0 = x, g.b0 = xb;
             g.c1 = xt2, g.b1 = xb;
-            product<kApply>(g, a.count, s);
+            if (kHigh && k == 0)
+                product<kApply, 2>(g, a.count, s);
+            else
+                product<kApply>(g, a.count, s);
             std::swap(xt, xt2);
             return;
         }
@@ -1047,23 +1066,27 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
             std::swap(g.bp, g.bq);
             std::swap(g.panels_p, g.panels_q);
         }
-        product<kFinal, O, kMuon>(g, a.count, s);
+        product<kFinal, 3, O, kMuon>(g, a.count, s);
     };
-    auto symmetric = [&](auto mode, const char* p, const char* q, long bytes, int kc, char* to) {
+    auto symmetric = [&](auto mode, auto terms, const char* p, const char* q, long bytes, int kc, char* to) {
         g.p = p, g.q = q, g.bp = g.bq = bytes, g.kc = kc;
         g.panels_p = g.panels_q = pl.pm;
         g.c0 = to, g.b0 = ab;
-        product<decltype(mode)::value>(g, a.count, s);
+        product<decltype(mode)::value, decltype(terms)::value>(g, a.count, s);
     };
+    constexpr std::integral_constant<int, 3> three{};
     auto gram = [&](int k, char* to) {
         g.factors = factors + k;
-        symmetric(std::integral_constant<int, kGram>{}, x, x, xb, kn, to);
+        if (kHigh && k == 0)
+            symmetric(std::integral_constant<int, kGram>{}, std::integral_constant<int, 1>{}, x, x, xb, kn, to);
+        else
+            symmetric(std::integral_constant<int, kGram>{}, three, x, x, xb, kn, to);
     };
     auto poly = [&](int k, const char* A, char* to) {
         g.ca = st.a[k], g.cb = st.b[k], g.cc = st.c[k], g.m = d.m;
-        symmetric(std::integral_constant<int, kPoly>{}, A, A, ab, km, to);
+        symmetric(std::integral_constant<int, kPoly>{}, three, A, A, ab, km, to);
     };
-    auto times = [&](const char* p, const char* q, char* to) { symmetric(std::integral_constant<int, kSym>{}, p, q, ab, km, to); };
+    auto times = [&](const char* p, const char* q, char* to) { symmetric(std::integral_constant<int, kSym>{}, three, p, q, ab, km, to); };
     for (int k = 0; k < st.n;) {
         const int n = steps_together(pl, st.n, grow, k);
         char *A = sym[0], *B = sym[1], *Q = B;

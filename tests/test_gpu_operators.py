@@ -371,6 +371,17 @@ def test_orthogonalize_of_short_sides_in_other_steps(rows, cols, steps, coeffici
             check_ns(out[i], g[i], "matrix %d, scale %g" % (i, scale), steps=steps, coefficients=coefficients)
 
 
+@pytest.mark.parametrize("rows, cols", [(200, 300), (300, 140), (64, 64), (40, 500)])
+@pytest.mark.parametrize("dtype, scales", [(F16, (1.0, 1e-4, 6000.0)), (BF16, (1.0, 1e-9, 1e-30, 1e30))], ids=["fp16", "bf16"])
+def test_orthogonalize_of_16_bit_matrices_of_any_scale(rows, cols, dtype, scales):
+    from gan_flow_amd.lib.optim import orthogonalize
+    gen = torch.Generator().manual_seed(rows)
+    for scale in scales:
+        g = (torch.randn(rows, cols, generator=gen) * scale).to(DEV, dtype)
+        for steps in (1, 5):
+            check_ns(orthogonalize(g, steps), g, "scale %g, %d steps" % (scale, steps), steps=steps)
+
+
 @pytest.mark.parametrize("rows, cols", [(64, 64), (33, 50), (200, 90), (320, 320)])
 def test_orthogonalize_batches_and_strides(rows, cols):
     from gan_flow_amd.lib.optim import orthogonalize
