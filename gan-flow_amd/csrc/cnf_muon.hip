@@ -33,6 +33,7 @@ namespace cnf {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr long kCus = 256;
 constexpr int kNormBlocks = 512;   // at most, per matrix
 constexpr float kScale = 1024.f, kInvScale = 1.f / 1024.f;
 constexpr long kBlockBytes = 64 * 128;
@@ -758,9 +759,13 @@ __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Step
 // in run() would save two more launches, 33 us, but a step costs little here and the grouping two thirds of the accuracy:
 // 2.7e-6 against 0.9e-6 for 64 x 66, where plain fp32 is 1.2e-6 off.)
 // How many workgroups share the tiles of a matrix: more make shorter loops and longer sums.  A step of 64 x 1000 takes 5.9 us with 16 workgroups
-// and 6.8 with 8; 64 x 4096 14.8 with 8, 9.7 with 23, 13.1 with 64; 64 x 65536 94 with 16, 35 with 91.
-int skinny_parts(long tiles) {
-    const long n = (long)std::fmax(16., std::ceil(std::sqrt(8. * (double)tiles)));
+// and 6.8 with 8; 64 x 4096 14.8 with 8, 9.7 with 23, 13.1 with 64; 64 x 65536 94 with 16, 35 with 91.  Of many matrices no more than
+// one to a CU, or two where there are tiles for long loops: 64 matrices 64 x 1000 88 us a call with 256 in all, 110 with 512, 159 without
+// a limit; 64 x (64 x 20000) 1185 with 256, 966 with 512.
+int skinny_parts(long count, long tiles) {
+    const long most = (count * tiles > 4096 ? 2 : 1) * kCus / count;
+    long n = (long)std::fmax(16., std::ceil(std::sqrt(8. * (double)tiles)));
+    n = n < most ? n : most;
     return (int)(n < tiles ? n : tiles);
 }
 
@@ -894,7 +899,6 @@ long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 // 4096 of k with few of them and `full` us when full, and `fixed` us whatever k is (its first operands, its results).  Where two run on a
 // CU, a round takes `full` as soon as one CU has two; where one does, what lies behind the CUs slows down from half full on.  Fitted
 // to products of 1 .. 1024 tiles and k = 256 .. 4096 (within a tenth for most, a quarter at worst); of those no choice was 5 % behind the best.
-constexpr long kCus = 256;
 struct Choice {
     int tile;
     double time;
@@ -1019,7 +1023,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         begin_kernel<O, kMuon, false><<<grid_in, kThreads, 0, s>>>(p, d, part, mu, nesterov, a.guard);
     char* const data = (char*)(part + (size_t)a.count * kNormBlocks);
     if (pl.skinny) {
-        const int n_parts = skinny_parts(pl.pn);
+        const int n_parts = skinny_parts(a.count, pl.pn);
         char *xt = data, *xt2 = xt + a.count * xb;
         float *gram = (float*)(xt2 + a.count * xb), *gram2 = gram + (long)a.count * n_parts * 4096, *factors = gram2 + (long)a.count * n_parts * 4096;
         const dim3 grid((unsigned)n_parts, a.count);
@@ -1161,7 +1165,7 @@ size_t muon_workspace_bytes(long count, long rows, long cols) {
     const size_t m = p.pm * 64, n = p.pn * 64;
     if (p.skinny)
         return (size_t)count *
-               (kNormBlocks * sizeof(double) + 2 * m * n * 4 + (size_t)skinny_parts(p.pn) * (2 * 16384) + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
+               (kNormBlocks * sizeof(double) + 2 * m * n * 4 + (size_t)skinny_parts(count, p.pn) * (2 * 16384) + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
     return (size_t)count * (kNormBlocks * sizeof(double) + (3 * m * n + (p.together ? 5 : 2) * m * m) * 4 + (CNF_NS_MAX_STEPS + 1) * sizeof(float));
 }
 
