@@ -82,7 +82,11 @@ def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, wei
         for lo in range(0, len(members), step):
             ps, gs, ms = zip(*members[lo:lo + step])
             _native.muon_step(ps, gs, ms, ns, lr, momentum, nesterov, weight_decay, scale, guard)
-            torch.autograd.graph.increment_version([t for t in ps + ms if not t.is_inference()])   # (written through raw pointers)
+            written = ps + ms                                # (through raw pointers: autograd is told)
+            try:
+                torch.autograd.graph.increment_version(written)
+            except RuntimeError:                             # inference tensors have no version
+                torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
 
 
 def adjusted_scale(how, rows, cols):
