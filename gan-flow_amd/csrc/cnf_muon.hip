@@ -14,7 +14,7 @@
 //
 // A gradient far below eps makes X0 = G / eps tiny, below what pieces hold.  X is therefore s Y with a factor s per matrix and
 // step: s = 1 unless |X0|_F < 1/2, then s = |X0|_F, Y = G / |G|_F, and every step takes s to min(1, s max|a + b t + c t^2|), which never lets Y grow
-// before s has reached 1:   A = s^2 Y Y^T,   Y' = (s / s') (a I + b A + c A^2) Y.
+// before s has reached 1:   A = s^2 Y Y^T,   Y' = (s / s') (a I + b A + c A^2) Y.  (A 16-bit matrix starts with s in [1/2, 1]: power_of_two.)
 //
 // LAYOUT ("piece matrix").  R x K, padded with zeros to multiples of 64 and stored in blocks of 64 rows x 32 columns, 8 KB
 // each, block (r / 64, k / 32) after block along k.  A block is eight fragments of 1 KB -- by 16 columns, 32 rows, piece (hi, lo) -- and a
@@ -157,8 +157,9 @@ __device__ __forceinline__ double start_scale(double norm, double eps, float& f)
     return (double)kScale * (small ? (norm > 0. ? 1. / norm : 0.) : 1. / (norm + eps));
 }
 
-// A 16-bit matrix scaled by a power of two has no low pieces (but for what lies below 2^-34), and its first products are fewer by as much: the rest of the scale goes to s, which
-// is then at least 1/2 (4096 x 4096: 3360 us against 3525).  Not in Muon, where what is iterated is the fp32 momentum's.
+// A 16-bit matrix scaled by a power of two has no low pieces (but for what lies below 2^-34), and its first products are fewer by as
+// much: the rest of the scale, at least 1/2, goes to s (4096 x 4096: 3360 us against 3525).  Not in Muon, where what is iterated is made of
+// the fp32 momentum.
 template <typename T, bool kMuon>
 constexpr bool kHighPieces = !kMuon && sizeof(T) == 2;
 
@@ -758,6 +759,7 @@ __global__ __launch_bounds__(kSmall) void small_kernel(FinalArgs a, Dims d, Step
 // twenty (64 x 1000: 42 us against 86).  `gram`: per matrix and workgroup the partial sums of X X^T as the waves hold them.  (Three steps at a time as
 // in run() would save two more launches, 33 us, but a step costs little here and the grouping two thirds of the accuracy:
 // 2.7e-6 against 0.9e-6 for 64 x 66, where plain fp32 is 1.2e-6 off.)
+
 // How many workgroups share the tiles of a matrix: more make shorter loops and longer sums.  A step of 64 x 1000 takes 5.9 us with 16 workgroups
 // and 6.8 with 8; 64 x 4096 14.8 with 8, 9.7 with 23, 13.1 with 64; 64 x 65536 94 with 16, 35 with 91.  Of many matrices no more than
 // one to a CU, or two where there are tiles for long loops: 64 matrices 64 x 1000 88 us a call with 256 in all, 110 with 512, 159 without
@@ -892,8 +894,6 @@ __global__ __launch_bounds__(kSmall) void skinny_step_kernel(FinalArgs a, Dims d
     }
     if (!kLast) put_gram(gram2, acc, wave, lane);
 }
-
-long pad_to(long v, long t) { return (v + t - 1) / t * t; }
 
 // Which kernel computes a product: the one whose estimated time is least.  A round is as many workgroups as run at once; it takes `few` us per
 // 4096 of k with few of them and `full` us when full, and `fixed` us whatever k is (its first operands, its results).  Where two run on a
