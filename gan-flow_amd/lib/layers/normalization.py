@@ -103,6 +103,16 @@ class MovingBatchNorm1d(MovingBatchNormNd):
         return [1, -1]
 
 
+def _layer_norm_backward(ctx, dy):   # (autograd gives dy the output's type, shape and device)
+    x, weight, stats = ctx.saved_tensors
+    mean = stats.data_ptr()
+    dx, dw, db = _native.norm_backward(dy, x, weight, ctx.wdtype, mean, mean + 4 * stats.shape[1], ctx.needs_input_grad)
+    return dx, dw, db, None
+
+
+_layer_norm_backward_once = once_differentiable(_layer_norm_backward)
+
+
 class _LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
@@ -111,12 +121,9 @@ class _LayerNormFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):   # (autograd gives dy the output's type, shape and device)
-        x, weight, stats = ctx.saved_tensors
-        mean = stats.data_ptr()
-        dx, dw, db = _native.norm_backward(dy, x, weight, ctx.wdtype, mean, mean + 4 * stats.shape[1], ctx.needs_input_grad)
-        return dx, dw, db, None
+    def backward(ctx, dy):
+        # (the wrapper matters only where the backward pass itself is recorded)
+        return _layer_norm_backward_once(ctx, dy) if torch.is_grad_enabled() else _layer_norm_backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
