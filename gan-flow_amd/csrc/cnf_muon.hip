@@ -899,19 +899,14 @@ __global__ __launch_bounds__(kSmall) void skinny_step_kernel(FinalArgs a, Dims d
 // 4096 of k with few of them and `full` us when full, and `fixed` us whatever k is (its first operands, its results).  Where two run on a
 // CU, a round takes `full` as soon as one CU has two; where one does, what lies behind the CUs slows down from half full on.  Fitted
 // to products of 1 .. 1024 tiles and k = 256 .. 4096 (within a tenth for most, a quarter at worst); of those no choice was 5 % behind the best.
-struct Choice {
-    int tile;
-    double time;
-};
-
-Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
+int choose(long count, int panels_p, int panels_q, bool sym, int kc) {
     struct Entry {
         int tile;
         long at_once;
         double few, full, fixed;
     };
     static constexpr Entry entries[] = {{64, 512, 22, 50, 4}, {128, 512, 84, 178, 7}, {192, 256, 135, 183, 14}, {256, 256, 196, 298, 20}};
-    Choice best{};
+    int best = 0;
     double least = 1e300;
     for (const Entry& e : entries) {
         const int t = e.tile / 64;
@@ -920,7 +915,7 @@ Choice choose(long count, int panels_p, int panels_q, bool sym, int kc) {
         double last = 0.;
         if (rest) last = e.at_once > kCus ? (rest > kCus ? e.full : e.few) : e.few + (e.full - e.few) * std::fmax(0., 2. * rest / kCus - 1.);
         const double time = (whole * e.full + last) * kc / 128. + (whole + (rest > 0)) * e.fixed;
-        if (time < least) least = time, best = {e.tile, time};
+        if (time < least) least = time, best = e.tile;
     }
     return best;
 }
@@ -930,10 +925,16 @@ struct Plan {
     int pm, pn;     // in panels of 64
     bool small;     // one workgroup per matrix does everything in LDS
     bool skinny;    // the shorter side fits a tile: skinny_start_kernel and its like
-    bool together;  // several steps at a time on the m x m side (decided for three steps, from the estimated times of the products)
+    bool together;  // several steps at a time on the m x m side
 };
 
-Plan plan_of(long count, long rows, long cols) {
+// Several steps at a time need fewer operations where n is larger than m, and round the matrix of squared singular values, whose small ones the
+// steps lift most.  Error of fp32 results against plain fp32's (normal matrices, gradient-like ones, and singular values over one, two and four
+// decades): at most 1.45 times for m > 192 and n >= 2 m, where step by step it is 0.3 .. 1.1 times (1.5 at n >= 4096), but 3.5 times for 80 x 5000 and 2.2 for
+// 100 x 4000, whose plain sums are no longer while their operands weigh more: those go step by step.  Time, step by step and together:
+// 200 x 800 114 and 118 us, 200 x 1600 137 and 128, 400 x 800 138 and 148, 400 x 1600 166 and 158, 512 x 1024 147 and 151 (eight of them 256 and 242),
+// 1024 x 4096 363 and 291 (four of them in a Muon update 1097 and 777).  A rule on the shape alone: what a matrix's neighbours are does not change its error.
+Plan plan_of(long rows, long cols) {
     Plan p{};
     p.m = rows < cols ? rows : cols;
     p.n = rows < cols ? cols : rows;
@@ -941,9 +942,7 @@ Plan plan_of(long count, long rows, long cols) {
     p.pm = (int)((p.m + 63) / 64);
     p.pn = (int)((p.n + 63) / 64);
     p.skinny = !p.small && p.pm == 1;
-    const double gram = choose(count, p.pm, p.pm, true, 2 * p.pn).time, sym = choose(count, p.pm, p.pm, true, 2 * p.pm).time,
-                 full = choose(count, p.pm, p.pn, false, 2 * p.pm).time;
-    p.together = gram + 9 * sym + full < 3 * (gram + sym + full);
+    p.together = p.m > 192 && p.n >= (p.m < 512 ? 4 : 2) * p.m;
     return p;
 }
 
@@ -958,15 +957,15 @@ int steps_together(const Plan& p, int steps, const double (&grow)[CNF_NS_MAX_STE
 
 template <int kMode, int kTerms = 3, typename O = float, bool kMuon = false>
 void product(const FinalArgs& g, int count, hipStream_t s) {
-    const Choice how = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>, g.kc);
-    const int t = how.tile / 64;
+    const int tile = choose(count, g.panels_p, g.panels_q, kSymmetric<kMode>, g.kc);
+    const int t = tile / 64;
     const long r = (g.panels_p + t - 1) / t, c = (g.panels_q + t - 1) / t;
     const dim3 grid((unsigned)(count * (kSymmetric<kMode> ? r * (r + 1) / 2 : r * c)));
-    if (how.tile == 256)
+    if (tile == 256)
         tile_kernel<256, 4, 2, 2, kMode, kTerms, O, kMuon><<<grid, 512, 0, s>>>(g);
-    else if (how.tile == 192)
+    else if (tile == 192)
         tile_kernel<192, 3, 3, 3, kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
-    else if (how.tile == 128)
+    else if (tile == 128)
         tile_kernel<128, 2, 2, 2, kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
     else
         tile64_kernel<kMode, kTerms, O, kMuon><<<grid, 256, 0, s>>>(g);
@@ -984,7 +983,7 @@ hipError_t run(const MuonArgs& a, hipStream_t s) {
         st.c[k] = (float)a.ns->c[k];
         st.grow[k] = (float)fmax(1., grow[k]);
     }
-    const Plan pl = plan_of(a.count, a.rows, a.cols);
+    const Plan pl = plan_of(a.rows, a.cols);
     constexpr bool kHigh = kHighPieces<O, kMuon>;
     Ptrs p{};
     bool vec_in = a.cols % 4 == 0 && a.ldg % 4 == 0 && (!kMuon || a.ldm % 4 == 0), vec_out = a.ldo % 4 == 0;
@@ -1160,7 +1159,7 @@ int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
 }
 
 size_t muon_workspace_bytes(long count, long rows, long cols) {
-    const Plan p = plan_of(count, rows, cols);
+    const Plan p = plan_of(rows, cols);
     if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)
     const size_t m = p.pm * 64, n = p.pn * 64;
     if (p.skinny)

@@ -723,3 +723,43 @@ def test_training_step_of_a_normalised_layer_captured_and_replayed():
         layer_norm(xk)                                        # eager work between the replays
         assert torch.equal(out, want[k][0])
         assert all(torch.equal(t.detach(), v) for t, v in zip(mine, want[k][1]))
+
+
+# ---- no less exact than plain fp32 ----------------------------------------------------------------------------------------
+
+def _spectrum(kind, count, rows, cols):
+    """Normal matrices, gradients (a decaying spectrum over noise), or singular values over `kind` decades; 64 bits."""
+    gen = torch.Generator(device=DEV).manual_seed(rows + cols)
+    randn = lambda *s: torch.randn(*s, generator=gen, device=DEV, dtype=torch.float64)  # noqa: E731
+    m = min(rows, cols)
+    if kind == "normal":
+        g = randn(count, m, max(rows, cols))
+    elif kind == "gradient":
+        g = (randn(count, m, m) * torch.logspace(0, -3, m, device=DEV)) @ randn(count, m, max(rows, cols)) / m ** 0.5 + 0.1 * randn(count, m, max(rows, cols))
+    else:
+        u, v = torch.linalg.qr(randn(count, m, m))[0], torch.linalg.qr(randn(count, max(rows, cols), m))[0]
+        g = (u * torch.logspace(0, -kind, m, device=DEV)) @ v.transpose(1, 2).contiguous()
+    return (g if rows <= cols else g.transpose(1, 2)).contiguous()
+
+
+def _plain(g, steps=5):
+    x = g.transpose(1, 2).contiguous() if g.shape[1] > g.shape[2] else g
+    x = x / (x.double().square().sum((1, 2), keepdim=True).sqrt() + 1e-7).to(x.dtype)
+    a, b, c = COEF
+    for _ in range(steps):
+        s = x @ x.transpose(1, 2).contiguous()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.transpose(1, 2) if g.shape[1] > g.shape[2] else x
+
+
+@pytest.mark.parametrize("kind", ["normal", "gradient", 2, 3])
+@pytest.mark.parametrize("count, rows, cols", [(4, 80, 5000), (4, 4000, 100), (40, 130, 260), (2, 300, 9000), (8, 200, 800), (2, 512, 1100), (2, 900, 260)])
+def test_orthogonalize_is_as_exact_as_plain_fp32(count, rows, cols, kind):
+    """Operands of 23 bits round at most twice what those of 24 do, and everything else is fp32 in both: twice the error of the same
+    iteration in fp32 tensor operations is allowed."""
+    from gan_flow_amd.lib.optim import orthogonalize
+    g = _spectrum(kind, count, rows, cols).float()
+    want = _plain(g.double())
+    err = lambda x: ((x.double() - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).mean().item()  # noqa: E731
+    mine, plain = err(orthogonalize(g)), err(_plain(g))
+    assert mine <= 2 * plain, "%g, and %g of the plain form" % (mine, plain)

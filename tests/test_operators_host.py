@@ -201,3 +201,11 @@ def test_layer_norm_module_mirrors_its_arguments():
     m.reset_parameters()
     assert m.weight.eq(1).all() and m.bias.eq(0).all()
     assert not list(LayerNorm(12, affine=False).parameters())
+
+
+@pytest.mark.parametrize("rows, cols", [(130, 260), (260, 130), (512, 640), (700, 500), (1000, 500), (256, 1024), (1024, 4096)])
+def test_a_matrix_is_iterated_the_same_way_in_every_stack(rows, cols):
+    """Whether steps are taken together (which needs more workspace) is decided by the shape, not by the number of matrices."""
+    from gan_flow_amd import _native as nat
+    one = nat.matrix_workspace_bytes(1, rows, cols)
+    assert [nat.matrix_workspace_bytes(n, rows, cols) for n in (2, 8, 40, 64)] == [n * one for n in (2, 8, 40, 64)]
