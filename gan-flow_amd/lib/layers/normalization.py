@@ -5,6 +5,7 @@ parity unpinned.  An elementwise map over (rows, d) with d <= 16: ordinary tenso
 integrators; it is a flow layer like CNF (same call signature, contributes its log-determinant)."""
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ... import _native
@@ -129,12 +130,15 @@ class _LayerNormFn(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """Layer normalisation over the last axis of x: (x - mean) / sqrt(var + eps) * weight + bias, one HIP kernel forward and
     backward (gan-flow_amd/csrc/cnf_norm.hip).  x: fp32, fp16 or bf16 on a HIP device, any leading axes, weight and bias of
-    x's type or fp32, or None.  Statistics and the sums of the weight gradients are fp32.  Differentiable once.  Capturable; as with
-    every autograd function, drop the outputs of eager passes over the same leaves before a backward pass is captured."""
+    x's type or fp32, or None.  Statistics and the sums of the weight gradients are fp32.  Differentiable once, in reverse mode (dual
+    tensors of forward mode are refused).  Capturable; as with every autograd function, drop the outputs of eager passes over the same
+    leaves before a backward pass is captured."""
     if not torch.is_tensor(x) or x.dim() == 0:
         raise _native.CnfError("x must be a tensor with at least one axis (got %s)" % (getattr(x, "shape", type(x)),))
     x2 = x if x.dim() == 2 else x.reshape(-1 if x.numel() else x[..., 0].numel(), x.shape[-1])
-    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+    # (inside a forward-mode level an input may carry a tangent without requiring a gradient: the autograd function refuses it)
+    if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
+            x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         y = _LayerNormFn.apply(x2, weight, bias, eps)
     else:
         y = _native.norm_forward(x2, weight, bias, eps, False)[0]

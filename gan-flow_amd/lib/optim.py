@@ -4,6 +4,7 @@ cnf_adam_step); vectors, and whatever else is not a matrix, stay with it."""
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 
@@ -23,8 +24,10 @@ def _at_once(n, rows, cols):
 def orthogonalize(g, steps=5, coefficients=DEFAULT_COEFFICIENTS, eps=1e-7):
     """X = g / (|g|_F + eps), then `steps` times X <- a X + (b X X^T + c (X X^T)^2) X, for every matrix of g (..., rows, cols);
     fp32, fp16 or bf16, returned in g's type.  coefficients: (a, b, c), or one such triple per step.  Matrices of zeros
-    stay zero.  Not differentiable."""
+    stay zero.  Not differentiable (dual tensors of forward mode are refused)."""
     _native._elem(g, "g")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(g).tangent is not None:
+        raise _native.CnfError("orthogonalize is not differentiable: g carries a forward-mode tangent")
     if g.dim() < 2:
         raise _native.CnfError("g must be a matrix or a stack of matrices (got shape %s)" % (tuple(g.shape),))
     ns = _native.ns_params(steps, coefficients, eps)

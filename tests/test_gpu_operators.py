@@ -763,3 +763,21 @@ def test_orthogonalize_is_as_exact_as_plain_fp32(count, rows, cols, kind):
     err = lambda x: ((x.double() - want).norm(dim=(1, 2)) / want.norm(dim=(1, 2))).mean().item()  # noqa: E731
     mine, plain = err(orthogonalize(g)), err(_plain(g))
     assert mine <= 2 * plain, "%g, and %g of the plain form" % (mine, plain)
+
+
+def test_operators_refuse_forward_mode():
+    from torch.autograd import forward_ad
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.layers import layer_norm
+    from gan_flow_amd.lib.optim import orthogonalize
+    x = torch.randn(70, 80, generator=torch.Generator().manual_seed(1)).to(DEV)
+    want = layer_norm(x), orthogonalize(x)
+    with forward_ad.dual_level():
+        assert torch.equal(layer_norm(x), want[0]) and torch.equal(orthogonalize(x), want[1])
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            layer_norm(dual)
+        with torch.no_grad(), pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            layer_norm(x, dual[0])
+        with pytest.raises(CnfError, match="tangent"):
+            orthogonalize(dual)

@@ -209,3 +209,31 @@ def test_a_matrix_is_iterated_the_same_way_in_every_stack(rows, cols):
     from gan_flow_amd import _native as nat
     one = nat.matrix_workspace_bytes(1, rows, cols)
     assert [nat.matrix_workspace_bytes(n, rows, cols) for n in (2, 8, 40, 64)] == [n * one for n in (2, 8, 40, 64)]
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias"])
+@pytest.mark.parametrize("grad", [True, False])
+def test_layer_norm_refuses_dual_tensors(monkeypatch, which, grad):
+    """A tangent is not dropped without a word (the kernel's call is replaced: the refusal comes from autograd)."""
+    from torch.autograd import forward_ad
+    from gan_flow_amd.lib.layers import layer_norm, normalization
+    monkeypatch.setattr(normalization._native, "norm_forward", lambda x, w, b, eps, stats: (x.clone(), x.new_zeros(2, len(x)), x, w, x.dtype))
+    args = dict(x=torch.randn(3, 8), weight=torch.ones(8), bias=torch.zeros(8))
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        layer_norm(**args)                                     # no tangent: nothing to refuse
+        args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises((RuntimeError, NotImplementedError), match="forward"):
+            layer_norm(**args)
+
+
+def test_orthogonalize_refuses_dual_tensors(monkeypatch):
+    from torch.autograd import forward_ad
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib import optim
+    monkeypatch.setattr(optim._native, "_elem", lambda t, name, dtypes=None: t)
+    monkeypatch.setattr(optim._native, "orthogonalize", lambda g, out, ns: out.copy_(g))
+    g = torch.randn(3, 8)
+    with forward_ad.dual_level():
+        optim.orthogonalize(g)
+        with pytest.raises(CnfError, match="tangent"):
+            optim.orthogonalize(forward_ad.make_dual(g, torch.ones_like(g)))
