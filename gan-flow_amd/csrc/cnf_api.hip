@@ -827,6 +827,7 @@ int cnf_layer_norm_bwd(const void* dy, int64_t dy_stride, const void* x, int64_t
     if (misaligned(dy, e) || misaligned(dx, e) || misaligned(dweight, we) || misaligned(dbias, we) || misaligned(mean, 4) ||
         misaligned(rstd, 4))
         return fail("%s: every pointer must be aligned to its element type", who);
+    if (rows == 0 && !dweight && !dbias) return 0;           // (dx has no elements, and no address where it is an empty tensor's)
     if (!dx && !dweight && !dbias) return fail("%s: nothing to compute (dx, dweight and dbias are all NULL)", who);
     if (rows > 0 && (dweight || dbias) &&
         (!workspace || misaligned(workspace, 16) || workspace_bytes < cnf::layer_norm_workspace_bytes(rows, cols)))

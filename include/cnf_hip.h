@@ -338,8 +338,8 @@ int cnf_layer_norm_fwd(const void *x, int64_t x_stride, int32_t dtype, const voi
 /* Its gradients: with h = dy * weight and xh = (x - mean) * rstd,
  *     dx = rstd * (h - mean(h) - xh * mean(h * xh)) per row,   dweight = sum over rows of dy * xh,   dbias = sum of dy.
  * dx (rows x cols, contiguous, not overlapping x or dy), dweight, dbias (cols elements of type wdtype): each nullable, then not
- * computed.  rows = 0 writes zeros to dweight and dbias.  workspace: cnf_layer_norm_workspace_bytes() bytes, 16-byte aligned,
- * any content.  Deterministic: column sums in a fixed order, no atomics.                                                 */
+ * computed (at least one, unless rows = 0, which writes zeros to dweight and dbias).  workspace:
+ * cnf_layer_norm_workspace_bytes() bytes, 16-byte aligned, any content.  Deterministic: column sums in a fixed order, no atomics.                                                 */
 size_t cnf_layer_norm_workspace_bytes(int64_t rows, int64_t cols);
 int cnf_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t x_stride, int32_t dtype, const void *weight,
                        int32_t wdtype, const float *mean, const float *rstd, int64_t rows, int64_t cols, void *dx,

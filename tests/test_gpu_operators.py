@@ -781,3 +781,18 @@ def test_operators_refuse_forward_mode():
             layer_norm(x, dual[0])
         with pytest.raises(CnfError, match="tangent"):
             orthogonalize(dual)
+
+
+def test_layer_norm_of_an_empty_batch_without_weight_gradients():
+    from gan_flow_amd.lib.layers import layer_norm
+    w, b = torch.ones(12, device=DEV), torch.zeros(12, device=DEV)
+    for shape in ((0, 12), (2, 0, 12)):
+        for args in ((None, None), (w, b)):
+            x = torch.empty(shape, device=DEV, requires_grad=True)
+            y = layer_norm(x, *args)
+            y.sum().backward()
+            assert y.shape == shape and x.grad.shape == shape
+    x = torch.empty(0, 12, device=DEV)
+    for lw, lb in ((w.clone().requires_grad_(), b), (w, b.clone().requires_grad_())):
+        layer_norm(x, lw, lb).sum().backward()
+        assert all(t.grad.eq(0).all() for t in (lw, lb) if t.requires_grad)

@@ -237,3 +237,10 @@ def test_orthogonalize_refuses_dual_tensors(monkeypatch):
         optim.orthogonalize(g)
         with pytest.raises(CnfError, match="tangent"):
             optim.orthogonalize(forward_ad.make_dual(g, torch.ones_like(g)))
+
+
+def test_layer_norm_bwd_of_no_rows_without_weight_gradients_enqueues_nothing():
+    from gan_flow_amd import _native as nat
+    lib = nat.load_library()
+    for dx in (None, ONE):
+        assert _norm_bwd(lib, rows=0, dx=dx, dw=None, db=None, dy=None, x=None, mean=None, rstd=None, ws=None, bytes_=0) == 0
