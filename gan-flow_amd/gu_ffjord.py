@@ -122,7 +122,8 @@ class GraphedTrainStep:
     as the kernels themselves early in training.  Capturing the iteration removes it: replay = one graph launch.
     Requirements: fixed batch shape, an optimizer built with capturable=True, no host sync inside (the solver status
     is left in device memory and checked by .check()).  `warmup` eager iterations run first on a side stream (they
-    are real training steps)."""
+    are real training steps); at least one is needed by an optimizer that has no state yet, which would otherwise create it inside
+    the capture, anew at every replay (Muon refuses that)."""
 
     def __init__(self, model, optimizer, example_batch, warmup_batches=()):
         self.model, self.optimizer = model, optimizer

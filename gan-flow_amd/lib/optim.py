@@ -104,10 +104,14 @@ def adjusted_scale(how, rows, cols):
     return float(how)
 
 
+def _capturing(t):
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class Muon(torch.optim.Optimizer):
     """Muon for a model's matrices (2-d parameters on a HIP device); every parameter of one shape is updated in one set of
     launches.  State per parameter: `momentum_buffer`, fp32.  step() synchronises nothing and can be captured into a graph
-    once the momenta exist (after the first step); a captured step keeps the learning rate it was captured with."""
+    once the momenta exist (after the first step; refused before); a captured step keeps the learning rate it was captured with."""
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_steps=5,
                  ns_coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, adjust_lr="original"):
@@ -145,6 +149,8 @@ class Muon(torch.optim.Optimizer):
                     raise _native.CnfError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if _capturing(p):                              # (its zeros would be written again at every replay)
+                        raise _native.CnfError("Muon's momenta do not exist yet: take a step before the first one that is captured")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 by_shape.setdefault(p.shape, []).append((p, p.grad, state["momentum_buffer"]))
             for shape, members in by_shape.items():

@@ -136,3 +136,14 @@ def test_graphed_loop_with_muon_replays_the_eager_steps():
         step(x)
     step.check()
     assert (_flat(ref) - _flat(model)).abs().max().item() <= 1e-4
+
+
+def test_graphed_loop_without_a_warm_up_is_refused_for_muon():
+    from gan_flow_amd import CnfError, gu_ffjord
+    from gan_flow_amd.lib.optim import MuonWithAdam
+    batches = _batches(1)
+    model = _model()
+    with torch.no_grad():                                      # (what the solves themselves read back once is there)
+        gu_ffjord.compute_loss(model, batches[0])
+    with pytest.raises(CnfError, match="before the first one that is captured"):
+        gu_ffjord.GraphedTrainStep(model, MuonWithAdam(model, MUON, dict(lr=1e-3, capturable=True)), batches[0])

@@ -244,3 +244,22 @@ def test_layer_norm_bwd_of_no_rows_without_weight_gradients_enqueues_nothing():
     lib = nat.load_library()
     for dx in (None, ONE):
         assert _norm_bwd(lib, rows=0, dx=dx, dw=None, db=None, dy=None, x=None, mean=None, rstd=None, ws=None, bytes_=0) == 0
+
+
+def test_muon_refuses_to_create_its_momenta_inside_a_capture(monkeypatch):
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib import optim
+    p = torch.nn.Parameter(torch.zeros(4, 8))
+    p.grad = torch.ones(4, 8)
+    taken = []
+    monkeypatch.setattr(optim, "muon_step", lambda *a, **kw: taken.append(a))
+    monkeypatch.setattr(optim, "_capturing", lambda t: True)
+    opt = optim.Muon([p])
+    with pytest.raises(CnfError, match="before the first one that is captured"):
+        opt.step()
+    assert not taken
+    monkeypatch.setattr(optim, "_capturing", lambda t: False)
+    opt.step()
+    monkeypatch.setattr(optim, "_capturing", lambda t: True)
+    opt.step()                                                 # the momenta exist
+    assert len(taken) == 2
