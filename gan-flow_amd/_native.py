@@ -776,7 +776,6 @@ def orthogonalize(gs, outs, ns):
 def muon_step(params, grads, momenta, ns, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, guard=None):
     """cnf_muon_step: one Muon update, in place, of the matrices `params` (as in orthogonalize) from `grads` (of their type) with the fp32
     momenta.  guard: stats words as in adam_step."""
-    lib = load_library()
     dt = _dtype_of(params)
     if dt not in DTYPE_IDS:
         raise CnfError("params must be %s (got %s)" % (" or ".join(str(d) for d in DTYPE_IDS), dt))
@@ -786,12 +785,18 @@ def muon_step(params, grads, momenta, ns, lr=1e-3, momentum=0.95, nesterov=True,
     if gshape != shape or mshape != shape or gdev != dev or mdev != dev:
         raise CnfError("grads and momenta must have the parameters' shape %s and device (got %s on %s, %s on %s)"
                        % (shape, gshape, gdev, mshape, mdev))
+    muon_launch(p, ldp, g, ldg, m, ldm, dt, shape, dev, ns, lr, momentum, nesterov, weight_decay, scale, guard)
+
+
+def muon_launch(p, ldp, g, ldg, m, ldm, dtype, shape, device, ns, lr, momentum, nesterov, weight_decay, scale, guard):
+    """muon_step on matrices that are checked: arrays of pointers and row strides of `shape` = (count, rows, cols)."""
+    lib = load_library()
     count, rows, cols = shape
     o = CnfMuonOpts(lr, momentum, weight_decay, scale, 1 if nesterov else 0, 0)
     need = lib.cnf_orthogonalize_workspace_bytes(count, rows, cols)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _at(dev) as stream:
-        rc = lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[dt], count, rows, cols, ctypes.byref(o), ctypes.byref(ns),
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
+    with _at(device) as stream:
+        rc = lib.cnf_muon_step(p, ldp, g, ldg, m, ldm, DTYPE_IDS[dtype], count, rows, cols, ctypes.byref(o), ctypes.byref(ns),
                                _stats_ptr(guard), ws.data_ptr(), need, stream)
     if rc:
         _check(rc, lib)

@@ -1,6 +1,7 @@
 """The Muon optimiser for the matrices of a network: each update is the momentum with its singular values driven to one
 by Newton-Schulz products (gan-flow_amd/csrc/cnf_muon.hip).  The reference trains with Adam only (the library's
 cnf_adam_step); vectors, and whatever else is not a matrix, stay with it."""
+import ctypes
 import math
 
 import torch
@@ -51,45 +52,78 @@ def orthogonalize(g, steps=5, coefficients=DEFAULT_COEFFICIENTS, eps=1e-7):
     return out
 
 
-def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, steps=5,
-              coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, guard=None):
-    """One Muon update, in place, of a list of matrices:
-        m <- momentum m + g;   u = g + momentum m (nesterov) or m;   p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)
-    grads: of the parameters' types; momenta: fp32.  Matrices of one shape, type and stride are updated side by side.  The
-    matrices must not overlap.  guard: the stats words of the solve that made the gradients (a failed one changes nothing)."""
+def _loose(rows, cols, strides):
+    """Whether the rows of a matrix are not contiguous, or overlap."""
+    return cols > 1 and strides[1] != 1 or rows > 1 and strides[0] < cols
+
+
+def _side_by_side(params, grads, momenta):
+    """Lists of (param, gradient, momentum) for one call of the library each: matrices of one shape, type and stride.  Everything is
+    checked here, before any of them is updated."""
     if not len(params) == len(grads) == len(momenta):
         raise _native.CnfError("%d params, %d grads, %d momenta" % (len(params), len(grads), len(momenta)))
-    ns = _native.ns_params(steps, coefficients, eps)
-    groups, seen, given, owned = {}, set(), 0, set()
+    groups, seen, given, owned, read = {}, set(), 0, set(), []
     for p, g, m in zip(params, grads, momenta):
         for name, t in (("params", p), ("grads", g), ("momenta", m)):
             if not torch.is_tensor(t) or not t.is_cuda or t.dim() != 2:
                 _native._elem(t, name)
                 raise _native.CnfError("%s: Muon updates matrices (got shape %s)" % (name, tuple(t.shape)))
-        if p.numel() == 0:
+        shape, dtype, dev = p.shape, p.dtype, p.device
+        if dtype not in _native.DTYPE_IDS or g.dtype != dtype or m.dtype != torch.float32:
+            _native._elem(p, "params"), _native._elem(g, "grads", (dtype,)), _native._elem(m, "momenta", (torch.float32,))
+        if g.shape != shape or m.shape != shape or g.device != dev or m.device != dev:
+            raise _native.CnfError("grads and momenta must have the parameters' shape %s and device %s (got %s on %s, %s on %s)"
+                                   % (tuple(shape), dev, tuple(g.shape), g.device, tuple(m.shape), m.device))
+        rows, cols = shape
+        if not rows or not cols:
             continue
-        gs, (rows, cols) = g.stride(), g.shape
-        if cols > 1 and gs[1] != 1 or rows > 1 and gs[0] < cols:
+        ps, gs, ms = p.stride(), g.stride(), m.stride()
+        if _loose(rows, cols, ps) or _loose(rows, cols, ms):
+            raise _native.CnfError("params and momenta: rows must be contiguous and must not overlap (strides %s, %s)" % (ps, ms))
+        pp, gp, mp = p.data_ptr(), g.data_ptr(), m.data_ptr()
+        read.append(gp)
+        if _loose(rows, cols, gs):
             g = g.contiguous()
-            gs = g.stride()
-        seen.update((p.data_ptr(), m.data_ptr()))
-        owned.add(m.data_ptr())
+            gs, gp = g.stride(), g.data_ptr()
+        seen.update((pp, mp))
+        owned.add(mp)
         given += 2
-        groups.setdefault((p.shape, p.dtype, p.device, p.stride(), gs, m.stride()), []).append((p, g, m))
+        groups.setdefault((shape, dtype, dev, ps[0], gs[0], ms[0]), []).append((p, g, m, pp, gp, mp))
     if len(seen) != given:
         raise _native.CnfError("the same parameter or momentum is given twice")
-    if not owned.isdisjoint([g.data_ptr() for g in grads]):
+    if not owned.isdisjoint(read):
         raise _native.CnfError("a gradient is also a momentum")
+    out = []
     for key, members in groups.items():
         step = _at_once(len(members), *key[0])
-        for lo in range(0, len(members), step):
-            ps, gs, ms = zip(*members[lo:lo + step])
-            _native.muon_step(ps, gs, ms, ns, lr, momentum, nesterov, weight_decay, scale, guard)
-            written = ps + ms                                # (through raw pointers: autograd is told)
-            try:
-                torch.autograd.graph.increment_version(written)
-            except RuntimeError:                             # inference tensors have no version
-                torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+        out += [(key, members[lo:lo + step]) for lo in range(0, len(members), step)]
+    return out
+
+
+def _update(calls, ns, lr, momentum, nesterov, weight_decay, scale, guard=None):
+    for ((rows, cols), dtype, dev, ldp, ldg, ldm), members in calls:
+        n = len(members)
+        ps, _, ms, pp, gp, mp = zip(*members)
+        array = ctypes.c_void_p * n
+        if rows == 1:
+            ldp = ldg = ldm = cols
+        _native.muon_launch(array(*pp), ldp, array(*gp), ldg, array(*mp), ldm, dtype, (n, rows, cols), dev, ns, lr, momentum, nesterov, weight_decay,
+                            scale, guard)
+        written = ps + ms                                    # (through raw pointers: autograd is told)
+        try:
+            torch.autograd.graph.increment_version(written)
+        except RuntimeError:                                 # inference tensors have no version
+            torch.autograd.graph.increment_version([t for t in written if not t.is_inference()])
+
+
+def muon_step(params, grads, momenta, lr=1e-3, momentum=0.95, nesterov=True, weight_decay=0.1, scale=1.0, steps=5,
+              coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, guard=None):
+    """One Muon update, in place, of a list of matrices:
+        m <- momentum m + g;   u = g + momentum m (nesterov) or m;   p <- (1 - lr weight_decay) p - lr scale orthogonalize(u)
+    grads: of the parameters' types; momenta: fp32.  Matrices of one shape, type and stride are updated side by side.  The
+    matrices must not overlap.  guard: the stats words of the solve that made the gradients (a failed one changes nothing).  A call that is
+    refused changes nothing either."""
+    _update(_side_by_side(params, grads, momenta), _native.ns_params(steps, coefficients, eps), lr, momentum, nesterov, weight_decay, scale, guard)
 
 
 def adjusted_scale(how, rows, cols):
@@ -115,16 +149,30 @@ class Muon(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, weight_decay=0.1, momentum=0.95, nesterov=True, ns_steps=5,
                  ns_coefficients=DEFAULT_COEFFICIENTS, eps=1e-7, adjust_lr="original"):
-        if not (lr >= 0.0 and 0.0 <= momentum < 1.0 and weight_decay >= 0.0 and eps > 0.0):
-            raise ValueError("invalid hyper-parameters (lr %r, momentum %r, weight_decay %r, eps %r)" % (lr, momentum, weight_decay, eps))
-        adjusted_scale(adjust_lr, 1, 1)
-        _native.ns_params(ns_steps, ns_coefficients, eps)
         super().__init__(params, dict(lr=lr, weight_decay=weight_decay, momentum=momentum, nesterov=nesterov, ns_steps=ns_steps,
                                       ns_coefficients=ns_coefficients, eps=eps, adjust_lr=adjust_lr))
-        for group in self.param_groups:
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            self._check(group)
             for p in group["params"]:
                 if p.dim() != 2:
                     raise ValueError("Muon updates matrices; give parameters of shape %s to another optimizer" % (tuple(p.shape),))
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check(group):
+        """CnfNewtonSchulz of a group whose hyper-parameters are valid."""
+        lr, momentum, weight_decay, eps = (group[k] for k in ("lr", "momentum", "weight_decay", "eps"))
+        scale = adjusted_scale(group["adjust_lr"], 1, 1)
+        if not (0.0 <= lr < math.inf and 0.0 <= momentum < 1.0 and 0.0 <= weight_decay < math.inf and 0.0 < eps < math.inf and 0.0 <= scale < math.inf):
+            raise ValueError("invalid hyper-parameters (lr %r, momentum %r, weight_decay %r, eps %r, adjust_lr %r)"
+                             % (lr, momentum, weight_decay, eps, group["adjust_lr"]))
+        return _native.ns_params(group["ns_steps"], group["ns_coefficients"], eps)
 
     def load_state_dict(self, state_dict):
         super().load_state_dict(state_dict)   # (casts state to the parameter's type: the momentum is fp32 whatever that is)
@@ -140,8 +188,9 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        updates = []                                         # (everything is checked before anything is updated)
         for group in self.param_groups:
-            by_shape = {}
+            ns, by_shape = self._check(group), {}
             for p in group["params"]:
                 if p.grad is None:
                     continue
@@ -149,15 +198,15 @@ class Muon(torch.optim.Optimizer):
                     raise _native.CnfError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
-                    if _capturing(p):                              # (its zeros would be written again at every replay)
+                    if _capturing(p):                        # (its zeros would be written again at every replay)
                         raise _native.CnfError("Muon's momenta do not exist yet: take a step before the first one that is captured")
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 by_shape.setdefault(p.shape, []).append((p, p.grad, state["momentum_buffer"]))
-            for shape, members in by_shape.items():
-                ps, gs, ms = zip(*members)
-                muon_step(ps, gs, ms, lr=group["lr"], momentum=group["momentum"], nesterov=group["nesterov"],
-                          weight_decay=group["weight_decay"], scale=adjusted_scale(group["adjust_lr"], *shape), steps=group["ns_steps"],
-                          coefficients=group["ns_coefficients"], eps=group["eps"])
+            hyper = {k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay")}
+            updates += [(_side_by_side(*zip(*members)), ns, dict(hyper, scale=adjusted_scale(group["adjust_lr"], *shape)))
+                        for shape, members in by_shape.items()]
+        for calls, ns, hyper in updates:
+            _update(calls, ns, **hyper)
         return loss
 
 

@@ -796,3 +796,47 @@ def test_layer_norm_of_an_empty_batch_without_weight_gradients():
     for lw, lb in ((w.clone().requires_grad_(), b), (w, b.clone().requires_grad_())):
         layer_norm(x, lw, lb).sum().backward()
         assert all(t.grad.eq(0).all() for t in (lw, lb) if t.requires_grad)
+
+
+def test_a_refused_muon_update_changes_nothing():
+    """One matrix among several that cannot be updated, whatever its place: the others are left as they were."""
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.optim import Muon, muon_step
+    gen = torch.Generator().manual_seed(41)
+    make = lambda *s: torch.randn(*s, generator=gen).to(DEV)  # noqa: E731
+    good = [(make(64, 64), make(64, 64), make(64, 64)), (make(70, 90), make(70, 90), make(70, 90))]
+    before = [[t.clone() for t in three] for three in good]
+    w, g, m = make(48, 32), make(48, 32), make(48, 32)
+    turned = lambda t: t.t().contiguous().t()  # noqa: E731
+    for bad in ((turned(w), g, m), (w, g, turned(m)), (w, g.half(), m), (w, g, m.half()), (w.double(), g.double(), m), (w, g[:-1], m), (w, g, m[:-1]),
+                (w, g, good[0][2]), (w, m, m), (torch.zeros(1, 65537, device=DEV),) * 3):
+        for at in range(3):
+            lists = [list(t) for t in zip(*(good[:at] + [bad] + good[at:]))]
+            with pytest.raises(CnfError):
+                muon_step(*lists)
+    assert all(torch.equal(t, s) for three, saved in zip(good, before) for t, s in zip(three, saved))
+    params = [torch.nn.Parameter(t) for t in (make(64, 64), turned(make(48, 32)), make(70, 90))]
+    opt = Muon(params[:1])
+    opt.add_param_group(dict(params=params[1:]))
+    for p in params:
+        p.grad = make(*p.shape)
+    saved = [p.detach().clone() for p in params]
+    with pytest.raises(CnfError, match="contiguous"):
+        opt.step()
+    assert all(torch.equal(p, s) for p, s in zip(params, saved))
+    assert all(opt.state[p]["momentum_buffer"].eq(0).all() for p in params)
+    params[1].grad = None
+    opt.step()
+    assert [torch.equal(p, s) for p, s in zip(params, saved)] == [False, True, False]
+
+
+def test_the_binding_and_the_optimizer_take_the_same_step():
+    from gan_flow_amd import _native as nat
+    from gan_flow_amd.lib.optim import muon_step
+    gen = torch.Generator().manual_seed(42)
+    for shape in ((3, 64, 64), (2, 1, 9), (2, 100, 300)):
+        w, g, m = (torch.randn(shape, generator=gen).to(DEV) for _ in range(3))
+        w2, m2 = w.clone(), m.clone()
+        muon_step(list(w), list(g), list(m), lr=0.1, scale=0.5)
+        nat.muon_step(w2, g, m2, nat.newton_schulz(), lr=0.1, scale=0.5)
+        assert torch.equal(w, w2) and torch.equal(m, m2)

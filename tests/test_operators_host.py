@@ -252,7 +252,8 @@ def test_muon_refuses_to_create_its_momenta_inside_a_capture(monkeypatch):
     p = torch.nn.Parameter(torch.zeros(4, 8))
     p.grad = torch.ones(4, 8)
     taken = []
-    monkeypatch.setattr(optim, "muon_step", lambda *a, **kw: taken.append(a))
+    monkeypatch.setattr(optim, "_side_by_side", lambda *lists: lists)
+    monkeypatch.setattr(optim, "_update", lambda *a, **kw: taken.append(a))
     monkeypatch.setattr(optim, "_capturing", lambda t: True)
     opt = optim.Muon([p])
     with pytest.raises(CnfError, match="before the first one that is captured"):
@@ -263,3 +264,20 @@ def test_muon_refuses_to_create_its_momenta_inside_a_capture(monkeypatch):
     monkeypatch.setattr(optim, "_capturing", lambda t: True)
     opt.step()                                                 # the momenta exist
     assert len(taken) == 2
+
+
+def test_every_group_of_muon_is_checked():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.optim import Muon
+    opt = Muon([torch.nn.Parameter(torch.zeros(4, 8))])
+    for bad, error in ((dict(lr=-1.0), ValueError), (dict(lr=float("inf")), ValueError), (dict(momentum=1.0), ValueError), (dict(eps=0.0), ValueError),
+                       (dict(adjust_lr=-0.5), ValueError), (dict(adjust_lr="other"), CnfError), (dict(ns_steps=0), CnfError),
+                       (dict(weight_decay=float("nan")), ValueError)):
+        with pytest.raises(error):
+            opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(4, 8))], **bad))
+    with pytest.raises(ValueError, match="another optimizer"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(4))]))
+    assert len(opt.param_groups) == 1
+    opt.param_groups[0]["lr"] = -1.0
+    with pytest.raises(ValueError):
+        opt.step()
