@@ -1131,14 +1131,11 @@ hipError_t run_op(const MuonArgs& a, hipStream_t s) {
 static double quintic_max(double a, double b, double c, double s) {
     auto f = [&](double u) { return std::fabs(u * (a + u * u * (b + u * u * c))); };
     double best = f(s);
-    double roots[2] = {-1., -1.};
+    // the roots in u^2, from the sum of two numbers of one sign: a difference loses the smaller root where c is small
     const double A = 5. * c, B = 3. * b, D = B * B - 4. * A * a;
-    if (A != 0. && D >= 0.) {
-        roots[0] = (-B + std::sqrt(D)) / (2. * A);
-        roots[1] = (-B - std::sqrt(D)) / (2. * A);
-    } else if (A == 0. && B != 0.) {
-        roots[0] = -a / B;
-    }
+    if (!(D >= 0.)) return best;
+    const double q = -0.5 * (B + std::copysign(std::sqrt(D), B));
+    const double roots[2] = {q / A, a / q};                  // (infinite or NaN where there is none)
     for (double r : roots)
         if (r > 0. && std::sqrt(r) < s) best = std::fmax(best, f(std::sqrt(r)));
     return best;

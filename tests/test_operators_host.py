@@ -281,3 +281,12 @@ def test_every_group_of_muon_is_checked():
     opt.param_groups[0]["lr"] = -1.0
     with pytest.raises(ValueError):
         opt.step()
+
+
+@pytest.mark.parametrize("c", [0.0, 1e-300, -1e-300, 1e-18, -1e-18, 1e-16, 1e-15, -1e-14, 1e-9])
+def test_a_hump_inside_the_interval_is_found_whatever_the_highest_coefficient(c):
+    """50 u - 50 u^3 + c u^5 is 0 at both ends of [0, 1] and 19 between: it diverges."""
+    from gan_flow_amd import _native as nat
+    lib = nat.load_library()
+    assert _orth(nat, lib, ns=_ns(nat, steps=1, coefficients=(50.0, -50.0, c)), bytes_=16) != 0 and b"diverge" in lib.cnf_last_error()
+    assert _orth(nat, lib, ns=_ns(nat, steps=1, coefficients=(5.0, -5.0, c)), bytes_=16) != 0 and b"workspace" in lib.cnf_last_error()
