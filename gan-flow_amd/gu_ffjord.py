@@ -240,8 +240,8 @@ class FusedTrainStep:
         # the stretches of each flat vector that Adam updates, each with its step count: one, or what lies between the hidden matrices
         self.stretches = [[(0, f.numel())] for f in self.flats]
         if optimizer == "muon":
-            from .lib.optim import Muon, adjusted_scale
-            groups = Muon([p for net in self.nets for p in self._hidden(net)], **dict(muon or {})).param_groups[0]   # (checks the arguments)
+            from .lib.optim import Muon, adjusted_scale, some_matrices
+            groups = Muon(some_matrices([p for net in self.nets for p in self._hidden(net)]), **dict(muon or {})).param_groups[0]   # (checks the arguments)
             self.muon = {k: groups[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "eps")}
             self.muon.update(steps=groups["ns_steps"], coefficients=groups["ns_coefficients"])
             self.muon_params, self.muon_views, self.muon_scales = [], [], []

@@ -216,7 +216,7 @@ class MuonWithAdam:
     optimizer where gu_ffjord's training loops need one (zero_grad, step, state_dict, load_state_dict)."""
 
     def __init__(self, model, muon=None, adam=None):
-        hidden = hidden_matrices(model)
+        hidden = some_matrices(hidden_matrices(model))
         taken = {id(p) for p in hidden}
         self.muon = Muon(hidden, **dict(muon or {}))
         self.adam = torch.optim.Adam([p for p in model.parameters() if id(p) not in taken], **dict(adam or {}))
@@ -245,3 +245,9 @@ def hidden_matrices(model):
         if isinstance(blk, CNF):
             out += [layer._layer.weight for layer in list(_inner(blk.odefunc).diffeq.layers)[1:-1]]
     return out
+
+
+def some_matrices(hidden):
+    if not hidden:
+        raise ValueError("Muon updates the weights from hidden to hidden layers, and this flow has none: its nets need at least two hidden layers")
+    return hidden

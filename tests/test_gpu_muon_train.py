@@ -147,3 +147,9 @@ def test_graphed_loop_without_a_warm_up_is_refused_for_muon():
         gu_ffjord.compute_loss(model, batches[0])
     with pytest.raises(CnfError, match="before the first one that is captured"):
         gu_ffjord.GraphedTrainStep(model, MuonWithAdam(model, MUON, dict(lr=1e-3, capturable=True)), batches[0])
+
+
+def test_fused_muon_step_says_that_a_flow_has_no_hidden_matrices():
+    from gan_flow_amd import gu_ffjord
+    with pytest.raises(ValueError, match="at least two hidden layers"):
+        gu_ffjord.FusedTrainStep(_model(dims=(64,)), _batches(1)[0], optimizer="muon", muon=MUON)

@@ -290,3 +290,11 @@ def test_a_hump_inside_the_interval_is_found_whatever_the_highest_coefficient(c)
     lib = nat.load_library()
     assert _orth(nat, lib, ns=_ns(nat, steps=1, coefficients=(50.0, -50.0, c)), bytes_=16) != 0 and b"diverge" in lib.cnf_last_error()
     assert _orth(nat, lib, ns=_ns(nat, steps=1, coefficients=(5.0, -5.0, c)), bytes_=16) != 0 and b"workspace" in lib.cnf_last_error()
+
+
+def test_muon_says_that_a_flow_has_no_hidden_matrices():
+    from gan_flow_amd import gu_ffjord
+    from gan_flow_amd.lib.optim import MuonWithAdam
+    with pytest.raises(ValueError, match="at least two hidden layers"):
+        MuonWithAdam(gu_ffjord.build_model(2, (64,)))
+    assert len(MuonWithAdam(gu_ffjord.build_model(2, (64, 64))).muon.param_groups[0]["params"]) == 1
