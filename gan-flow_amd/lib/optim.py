@@ -175,6 +175,10 @@ class Muon(torch.optim.Optimizer):
         return _native.ns_params(group["ns_steps"], group["ns_coefficients"], eps)
 
     def load_state_dict(self, state_dict):
+        """A state of this class only: other optimizers keep a `momentum_buffer` too (torch.optim.Muon an average of the gradients, 1 - momentum
+        times this sum of them)."""
+        if any("adjust_lr" not in g for g in state_dict["param_groups"]) or any("momentum_buffer" not in s for s in state_dict["state"].values()):
+            raise ValueError("the state is another optimizer's")
         super().load_state_dict(state_dict)   # (casts state to the parameter's type: the momentum is fp32 whatever that is)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [p for g in self.param_groups for p in g["params"]]
@@ -233,6 +237,8 @@ class MuonWithAdam:
         return {"muon": self.muon.state_dict(), "adam": self.adam.state_dict()}
 
     def load_state_dict(self, state):
+        if "muon" not in state or "adam" not in state:
+            raise ValueError("the state is another optimizer's (Muon's and Adam's are wanted, got %s)" % sorted(state))
         self.muon.load_state_dict(state["muon"])
         self.adam.load_state_dict(state["adam"])
 

@@ -298,3 +298,30 @@ def test_muon_says_that_a_flow_has_no_hidden_matrices():
     with pytest.raises(ValueError, match="at least two hidden layers"):
         MuonWithAdam(gu_ffjord.build_model(2, (64,)))
     assert len(MuonWithAdam(gu_ffjord.build_model(2, (64, 64))).muon.param_groups[0]["params"]) == 1
+
+
+def test_muon_loads_no_other_optimizers_state():
+    from gan_flow_amd import gu_ffjord
+    from gan_flow_amd.lib.optim import Muon, MuonWithAdam
+    p = torch.nn.Parameter(torch.zeros(4, 8))
+    mine = Muon([p], lr=0.03)
+    mine.state[p]["momentum_buffer"] = torch.ones(4, 8)
+    fresh = Muon([p])
+    others = [torch.optim.SGD([p], lr=0.1, momentum=0.9), torch.optim.Adam([p])]
+    if hasattr(torch.optim, "Muon"):
+        others.append(torch.optim.Muon([p]))
+    for other in others:
+        if isinstance(other, torch.optim.Adam):
+            other.state[p].update(exp_avg=torch.ones(4, 8), exp_avg_sq=torch.ones(4, 8), step=torch.tensor(1.0))
+        else:
+            other.state[p]["momentum_buffer"] = torch.ones(4, 8)
+        with pytest.raises(ValueError, match="another optimizer"):
+            fresh.load_state_dict(other.state_dict())
+        assert not fresh.state
+    fresh.load_state_dict(mine.state_dict())
+    assert fresh.param_groups[0]["lr"] == 0.03 and fresh.state[p]["momentum_buffer"].eq(1).all()
+    model = gu_ffjord.build_model(2, (64, 64))
+    both = MuonWithAdam(model)
+    with pytest.raises(ValueError, match="another optimizer"):
+        both.load_state_dict(torch.optim.Adam(model.parameters()).state_dict())
+    both.load_state_dict(both.state_dict())
