@@ -900,6 +900,9 @@ int cnf_orthogonalize(const void* const* g, int64_t ldg, void* const* out, int64
     for (int64_t i = 0; i < count; ++i)
         for (int64_t j = 0; j < i; ++j)
             if (out[i] == out[j]) return fail("%s: matrices %ld and %ld have the same output", who, (long)j, (long)i);
+    for (int64_t i = 0; i < count; ++i)                      // (written while the other matrix may still be read)
+        for (int64_t j = 0; j < count; ++j)
+            if (i != j && out[i] == g[j]) return fail("%s: the output of matrix %ld is matrix %ld", who, (long)i, (long)j);
     cnf::MuonArgs a{};
     a.g = g;
     a.ldg = ldg;
@@ -938,6 +941,9 @@ int cnf_muon_step(void* const* params, int64_t ldp, const void* const* grads, in
         for (int64_t j = 0; j < count; ++j)
             if (grads[i] == momenta[j] || params[i] == momenta[j])
                 return fail("%s: momentum %ld is also a gradient or a parameter", who, (long)j);
+    for (int64_t i = 0; i < count; ++i)                      // (another matrix's parameter may be written by then)
+        for (int64_t j = 0; j < count; ++j)
+            if (i != j && grads[i] == params[j]) return fail("%s: gradient %ld is parameter %ld", who, (long)i, (long)j);
     cnf::MuonArgs a{};
     a.g = grads;
     a.ldg = ldg;

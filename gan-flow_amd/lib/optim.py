@@ -81,7 +81,8 @@ def _side_by_side(params, grads, momenta):
         if _loose(rows, cols, ps) or _loose(rows, cols, ms):
             raise _native.CnfError("params and momenta: rows must be contiguous and must not overlap (strides %s, %s)" % (ps, ms))
         pp, gp, mp = p.data_ptr(), g.data_ptr(), m.data_ptr()
-        read.append(gp)
+        if gp != pp:
+            read.append(gp)
         if _loose(rows, cols, gs):
             g = g.contiguous()
             gs, gp = g.stride(), g.data_ptr()
@@ -91,8 +92,8 @@ def _side_by_side(params, grads, momenta):
         groups.setdefault((shape, dtype, dev, ps[0], gs[0], ms[0]), []).append((p, g, m, pp, gp, mp))
     if len(seen) != given:
         raise _native.CnfError("the same parameter or momentum is given twice")
-    if not owned.isdisjoint(read):
-        raise _native.CnfError("a gradient is also a momentum")
+    if not seen.isdisjoint(read):
+        raise _native.CnfError("a gradient is also a momentum" if not owned.isdisjoint(read) else "a gradient is another matrix's parameter")
     out = []
     for key, members in groups.items():
         step = _at_once(len(members), *key[0])

@@ -840,3 +840,20 @@ def test_the_binding_and_the_optimizer_take_the_same_step():
         muon_step(list(w), list(g), list(m), lr=0.1, scale=0.5)
         nat.muon_step(w2, g, m2, nat.newton_schulz(), lr=0.1, scale=0.5)
         assert torch.equal(w, w2) and torch.equal(m, m2)
+
+
+def test_muon_step_refuses_another_matrixs_parameter_as_gradient():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.optim import muon_step
+    gen = torch.Generator().manual_seed(43)
+    for a, b in (((64, 64), (64, 64)), ((100, 80), (100, 80))):
+        w, v = (torch.randn(s, generator=gen).to(DEV) for s in (a, b))
+        m = [torch.zeros_like(w), torch.zeros_like(v)]
+        for g in ([v, v.clone()], [w.clone(), w], [v, w]):
+            with pytest.raises(CnfError, match="another matrix's parameter"):
+                muon_step([w, v], g, m)
+        w0, v0 = w.clone(), v.clone()
+        muon_step([w, v], [w, v], m)                           # its own: decay along the parameter itself
+        want = [t.clone() for t in (w0, v0)]
+        muon_step(want, [w0, v0], [torch.zeros_like(w), torch.zeros_like(v)])
+        assert torch.equal(w, want[0]) and torch.equal(v, want[1])

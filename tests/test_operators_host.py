@@ -325,3 +325,16 @@ def test_muon_loads_no_other_optimizers_state():
     with pytest.raises(ValueError, match="another optimizer"):
         both.load_state_dict(torch.optim.Adam(model.parameters()).state_dict())
     both.load_state_dict(both.state_dict())
+
+
+def test_matrices_that_are_read_and_written_by_different_workgroups_are_refused():
+    from gan_flow_amd import _native as nat
+    lib = nat.load_library()
+    A, B, C, D, E, F = (4096 * (i + 1) for i in range(6))
+    o, ns = nat.CnfMuonOpts(1e-3, 0.95, 0.1, 1.0, 1, 0), ctypes.byref(_ns(nat))
+    for g, words in (((B, C), b"gradient 0 is parameter 1"), ((C, A), b"gradient 1 is parameter 0"), ((B, A), b"is parameter")):
+        rc = lib.cnf_muon_step(_ptrs(A, B), 8, _ptrs(*g), 8, _ptrs(E, F), 8, 0, 2, 4, 8, ctypes.byref(o), ns, None, ONE, 1 << 30, None)
+        assert rc != 0 and words in lib.cnf_last_error()
+    for g, out, words in (((A, B), (B, C), b"output of matrix 0 is matrix 1"), ((A, B), (B, A), b"is matrix"), ((A, B), (D, A), b"output of matrix 1 is matrix 0")):
+        rc = lib.cnf_orthogonalize(_ptrs(*g), 8, _ptrs(*out), 8, 0, 2, 4, 8, ns, ONE, 1 << 30, None)
+        assert rc != 0 and words in lib.cnf_last_error()
