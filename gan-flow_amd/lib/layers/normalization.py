@@ -3,6 +3,8 @@
 and no checkpoint of the reference uses it, so names and arithmetic follow the published FFJORD code as recalled --
 parity unpinned.  An elementwise map over (rows, d) with d <= 16: ordinary tensor ops on the device, outside the
 integrators; it is a flow layer like CNF (same call signature, contributes its log-determinant)."""
+import math
+
 import torch
 import torch.nn as nn
 from torch.autograd import forward_ad
@@ -135,10 +137,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     leaves before a backward pass is captured."""
     if not torch.is_tensor(x) or x.dim() == 0:
         raise _native.CnfError("x must be a tensor with at least one axis (got %s)" % (getattr(x, "shape", type(x)),))
-    x2 = x if x.dim() == 2 else x.reshape(-1 if x.numel() else x[..., 0].numel(), x.shape[-1])
+    x2 = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     # (inside a forward-mode level an input may carry a tangent without requiring a gradient: the autograd function refuses it)
     if forward_ad._current_level >= 0 or torch.is_grad_enabled() and (
-            x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+            x.requires_grad or getattr(weight, "requires_grad", False) or getattr(bias, "requires_grad", False)):
         y = _LayerNormFn.apply(x2, weight, bias, eps)
     else:
         y = _native.norm_forward(x2, weight, bias, eps, False)[0]
@@ -166,8 +168,8 @@ class LayerNorm(nn.Module):
             nn.init.zeros_(self.bias)
 
     def forward(self, x):
-        if x.shape[-1] != self.num_features:
-            raise _native.CnfError("LayerNorm(%d) got %d features" % (self.num_features, x.shape[-1]))
+        if x.dim() == 0 or x.shape[-1] != self.num_features:
+            raise _native.CnfError("LayerNorm(%d) got %d features" % (self.num_features, x.shape[-1] if x.dim() else 0))
         return layer_norm(x, self.weight, self.bias, self.eps)
 
     def extra_repr(self):

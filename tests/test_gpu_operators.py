@@ -857,3 +857,17 @@ def test_muon_step_refuses_another_matrixs_parameter_as_gradient():
         want = [t.clone() for t in (w0, v0)]
         muon_step(want, [w0, v0], [torch.zeros_like(w), torch.zeros_like(v)])
         assert torch.equal(w, want[0]) and torch.equal(v, want[1])
+
+
+def test_layer_norm_refuses_what_has_no_features_or_no_tensors():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.layers import layer_norm
+    for x in (torch.empty(2, 3, 0), torch.empty(0), torch.empty(0, 0)):
+        with pytest.raises(CnfError, match="cols > 0"):
+            layer_norm(x.to(DEV))
+    x = torch.randn(4, 8, device=DEV, requires_grad=True)
+    for args in (([1.0] * 8, None), (None, 1.0), (2.0, None)):
+        with pytest.raises(CnfError, match="HIP device"):
+            layer_norm(x, *args)
+    for shape in ((3, 0, 8), (0, 3, 8), (0, 8), (2, 0, 0, 8)):
+        assert layer_norm(torch.empty(shape, device=DEV)).shape == shape

@@ -338,3 +338,16 @@ def test_matrices_that_are_read_and_written_by_different_workgroups_are_refused(
     for g, out, words in (((A, B), (B, C), b"output of matrix 0 is matrix 1"), ((A, B), (B, A), b"is matrix"), ((A, B), (D, A), b"output of matrix 1 is matrix 0")):
         rc = lib.cnf_orthogonalize(_ptrs(*g), 8, _ptrs(*out), 8, 0, 2, 4, 8, ns, ONE, 1 << 30, None)
         assert rc != 0 and words in lib.cnf_last_error()
+
+
+def test_layer_norm_refuses_what_has_no_features_or_no_tensors(monkeypatch):
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.layers import LayerNorm, layer_norm
+    for x in (torch.empty(2, 3, 0), torch.empty(0), torch.empty(0, 0), torch.empty(2, 0, 3, 0)):
+        with pytest.raises(CnfError):
+            layer_norm(x)
+    with pytest.raises(CnfError):
+        LayerNorm(8)(torch.tensor(1.0))
+    for args in (([1.0] * 8, None), (None, 1.0), (2.0, None)):
+        with pytest.raises(CnfError):
+            layer_norm(torch.randn(4, 8, requires_grad=True), *args)
