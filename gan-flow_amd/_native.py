@@ -92,7 +92,8 @@ EXPORTS = ("cnf_param_count", "cnf_workspace_bytes", "cnf_last_error", "cnf_eval
            "cnf_debug_kernel_timing", "cnf_debug_last_kernel_ms", "cnf_activation", "cnf_debug_eval_field_b16",
            "cnf_solve_fwd_static", "cnf_static_scratch_bytes", "cnf_gu_sample", "cnf_gu_sample_rows", "cnf_solve_fwd_times",
            "cnf_solve_fwd_reg", "cnf_solve_bwd_reg", "cnf_layer_norm_fwd", "cnf_layer_norm_workspace_bytes",
-           "cnf_layer_norm_bwd", "cnf_orthogonalize_workspace_bytes", "cnf_orthogonalize", "cnf_muon_step")
+           "cnf_layer_norm_bwd", "cnf_orthogonalize_workspace_bytes", "cnf_orthogonalize", "cnf_muon_step",
+           "cnf_debug_matrix_plan")
 
 
 def library_path(act="tanh"):
@@ -169,6 +170,8 @@ def load_library(act="tanh"):
     lib.cnf_orthogonalize.argtypes = [PP, I64, PP, I64, I32, I64, I64, I64, NS, P, SZ, VP]
     lib.cnf_muon_step.restype = ctypes.c_int
     lib.cnf_muon_step.argtypes = [PP, I64, PP, I64, PP, I64, I32, I64, I64, I64, MO, NS, P, P, SZ, VP]
+    lib.cnf_debug_matrix_plan.restype = ctypes.c_int
+    lib.cnf_debug_matrix_plan.argtypes = [I64, I64, I64, ctypes.POINTER(I32)]
     lib.cnf_debug_kernel_timing.restype = ctypes.c_int
     lib.cnf_debug_kernel_timing.argtypes = [ctypes.c_int]
     lib.cnf_debug_last_kernel_ms.restype = ctypes.c_int
@@ -750,6 +753,13 @@ def _dtype_of(ts):
 def matrix_workspace_bytes(count, rows, cols):
     """Bytes cnf_orthogonalize and cnf_muon_step need; 0 where the sizes are not supported."""
     return load_library().cnf_orthogonalize_workspace_bytes(count, rows, cols)
+
+
+def matrix_plan(count, rows, cols):
+    """cnf_debug_matrix_plan: (path, steps together, tiles of the three kinds of product)."""
+    lib, plan = load_library(), (ctypes.c_int32 * 5)()
+    _check(lib.cnf_debug_matrix_plan(count, rows, cols, plan), lib)
+    return tuple(plan)
 
 
 def orthogonalize(gs, outs, ns):

@@ -963,6 +963,15 @@ int cnf_muon_step(void* const* params, int64_t ldp, const void* const* grads, in
     return 0;
 }
 
+int cnf_debug_matrix_plan(int64_t count, int64_t rows, int64_t cols, int32_t plan[5]) {
+    if (!plan || !cnf_orthogonalize_workspace_bytes(count, rows, cols))
+        return fail("cnf_debug_matrix_plan: NULL pointer or unsupported sizes (%ld, %ld, %ld)", (long)count, (long)rows, (long)cols);
+    int32_t p[5];
+    cnf::muon_plan(count, rows, cols, p);
+    for (int i = 0; i < 5; ++i) plan[i] = p[i];
+    return 0;
+}
+
 int cnf_debug_fill_lds(uint32_t pattern, uint32_t* scratch_word, void* stream) {
     if (!scratch_word) return fail("cnf_debug_fill_lds: NULL pointer");
     hipError_t err = cnf::launch_fill_lds(pattern, scratch_word, (hipStream_t)stream);

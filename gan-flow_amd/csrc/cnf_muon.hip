@@ -1155,6 +1155,17 @@ int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]) {
     return 0;
 }
 
+void muon_plan(long count, long rows, long cols, int32_t (&plan)[5]) {
+    const Plan p = plan_of(rows, cols);
+    plan[0] = p.small ? 0 : p.skinny ? 1 : 2;
+    plan[1] = plan[0] == 2 && p.together;
+    plan[2] = plan[3] = plan[4] = 64;
+    if (plan[0] != 2) return;
+    plan[2] = choose(count, p.pm, p.pm, true, 2 * p.pn);
+    plan[3] = choose(count, p.pm, p.pm, true, 2 * p.pm);
+    plan[4] = choose(count, p.pm, p.pn, false, 2 * p.pm);
+}
+
 size_t muon_workspace_bytes(long count, long rows, long cols) {
     const Plan p = plan_of(rows, cols);
     if (p.small) return 256;   // (uses none; 0 stands for a call that is not supported)

@@ -56,6 +56,7 @@ struct MuonArgs {
 // bounds the iteration over singular values in [0, 1]: 0, or the number of the first step that lets them leave the range the
 // kernels hold; grow[k]: the largest |a + b t + c t^2| of step k
 int ns_bounds(const CnfNewtonSchulz& ns, double (&grow)[CNF_NS_MAX_STEPS]);
+void muon_plan(long count, long rows, long cols, int32_t (&plan)[5]);   // cnf_debug_matrix_plan
 size_t muon_workspace_bytes(long count, long rows, long cols);
 hipError_t launch_muon(int dtype, const MuonArgs& a, hipStream_t s);
 

@@ -403,6 +403,11 @@ int cnf_debug_eval_field_b16(const CnfNetDesc *net, const float *params, float t
 int cnf_debug_kernel_timing(int enable);
 int cnf_debug_last_kernel_ms(float *ms_out);
 
+/* Diagnostics (no counterpart in the reference): how cnf_orthogonalize and cnf_muon_step iterate matrices of these sizes, so that the
+ * tests can tell that they reach every kernel: plan[0]: 0 one workgroup per matrix, 1 the shorter side within a tile, 2 products;
+ * plan[1]: several steps are taken together; plan[2 .. 4]: side of the tiles of X X^T, of the other symmetric products, of the products with X. */
+int cnf_debug_matrix_plan(int64_t count, int64_t rows, int64_t cols, int32_t plan[5]);
+
 #ifdef __cplusplus
 }
 #endif

@@ -871,3 +871,96 @@ def test_layer_norm_refuses_what_has_no_features_or_no_tensors():
             layer_norm(x, *args)
     for shape in ((3, 0, 8), (0, 3, 8), (0, 8), (2, 0, 0, 8)):
         assert layer_norm(torch.empty(shape, device=DEV)).shape == shape
+
+
+# ---- every kernel of the larger products ----------------------------------------------------------------------------------
+
+# (count, rows, cols): (steps together, tiles of X X^T, of the other symmetric products, of the products with X)
+PLANS = {(12, 768, 768): (0, 128, 128, 128), (40, 515, 523): (0, 192, 192, 128), (16, 1000, 1000): (0, 256, 256, 256), (40, 370, 555): (0, 128, 128, 192),
+         (8, 1010, 500): (0, 64, 64, 128), (6, 460, 2760): (1, 64, 64, 256), (40, 1120, 280): (1, 64, 128, 128), (1, 4000, 4030): (0, 192, 192, 256),
+         (12, 310, 1860): (1, 64, 64, 192)}
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=lambda t: IDS[t])
+@pytest.mark.parametrize("shape", PLANS)
+def test_orthogonalize_through_every_tile(shape, dtype):
+    """16-bit matrices take the kernels of one and two products of pieces in their first step."""
+    from gan_flow_amd import _native as nat
+    from gan_flow_amd.lib.optim import orthogonalize
+    count, rows, cols = shape
+    assert nat.matrix_plan(*shape) == (2,) + PLANS[shape]
+    gen = torch.Generator(device=DEV).manual_seed(rows)
+    wide = torch.randn(count, rows, cols + 2, generator=gen, device=DEV)
+    wide[..., 0] *= 30.0                                       # one direction far above the others
+    wide = wide.to(dtype)
+    for g in (wide[..., :cols].contiguous(), wide[..., 1:cols + 1]) if count * rows * cols < 1 << 23 else (wide[..., :cols].contiguous(),):
+        out = orthogonalize(g)
+        for i in sorted({0, count - 1}):
+            check_ns(out[i], g[i], "matrix %d" % i)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=lambda t: IDS[t])
+@pytest.mark.parametrize("shape", [s for s in PLANS if s[0] > 1])
+def test_muon_step_through_every_tile(shape, dtype):
+    """Parameters in rows of wider buffers, under a guard: a failed solve changes nothing, the next one everything it should."""
+    from gan_flow_amd import _native as nat
+    from gan_flow_amd.lib.optim import muon_step
+    count, rows, cols = shape
+    assert nat.matrix_plan(*shape) == (2,) + PLANS[shape]
+    gen = torch.Generator(device=DEV).manual_seed(cols)
+    wide = torch.randn(count, rows, cols + 5, generator=gen, device=DEV).to(dtype)
+    g, m = torch.randn(count, rows, cols, generator=gen, device=DEV).to(dtype), torch.randn(count, rows, cols, generator=gen, device=DEV)
+    w = wide[..., 2:cols + 2]
+    wide0, m0 = wide.clone(), m.clone()
+    w0 = wide0[..., 2:cols + 2]
+    words = torch.zeros(8, dtype=torch.int32, device=DEV)
+    words[0] = 2
+    kw = dict(lr=0.02, momentum=0.9, weight_decay=0.05, scale=0.7, guard=words)
+    muon_step(list(w), list(g), list(m), **kw)
+    assert torch.equal(wide, wide0) and torch.equal(m, m0)
+    words.zero_()
+    muon_step(list(w), list(g), list(m), **kw)
+    assert torch.equal(wide[..., :2], wide0[..., :2]) and torch.equal(wide[..., cols + 2:], wide0[..., cols + 2:])
+    for i in (0, count - 1):
+        want, tol, m1 = muon_reference(w0[i], g[i], m0[i], 0.02, 0.9, True, 0.05, 0.7, dtype)
+        check(m[i], m1, 3 * U * (m0[i].double().abs() + g[i].double().abs()), "momentum")
+        err = (w[i].double() - want).norm().item()
+        assert err <= tol, "matrix %d: |error|_F %g, %g allowed" % (i, err, tol)
+
+
+@pytest.mark.parametrize("shape", [(3, 40, 900), (2, 900, 40), (2, 7, 65)])
+def test_muon_step_of_short_sides_under_a_guard(shape):
+    from gan_flow_amd.lib.optim import muon_step
+    gen = torch.Generator().manual_seed(44)
+    for dtype in (F32, F16, BF16):
+        w, g, m = (torch.randn(shape, generator=gen).to(DEV) for _ in range(3))
+        w, g = w.to(dtype), g.to(dtype)
+        w0, m0 = w.clone(), m.clone()
+        words = torch.ones(8, dtype=torch.int32, device=DEV)
+        muon_step(list(w), list(g), list(m), lr=0.1, guard=words)
+        assert torch.equal(w, w0) and torch.equal(m, m0)
+        words.zero_()
+        muon_step(list(w), list(g), list(m), lr=0.1, guard=words)
+        for i in range(shape[0]):
+            want, tol, m1 = muon_reference(w0[i], g[i], m0[i], 0.1, 0.95, True, 0.1, 1.0, dtype)
+            check(m[i], m1, 3 * U * (m0[i].double().abs() + g[i].double().abs()), "momentum")
+            assert (w[i].double() - want).norm().item() <= tol
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=lambda t: IDS[t])
+@pytest.mark.parametrize("rows, cols", [(64, 64), (40, 500), (500, 40), (150, 90), (1, 300), (220, 900)])
+def test_orthogonalize_keeps_matrices_apart(rows, cols, dtype):
+    """A NaN or an infinity makes its matrix NaN throughout and leaves the others in the call their bits."""
+    from gan_flow_amd.lib.optim import muon_step, orthogonalize
+    gen = torch.Generator().manual_seed(45)
+    g = torch.randn(4, rows, cols, generator=gen).to(DEV, dtype)
+    clean = orthogonalize(g)
+    for bad in (float("nan"), float("inf"), float("-inf")):
+        g2 = g.clone()
+        g2[1, rows - 1, cols - 1] = bad
+        g2[2, 0, cols // 2] = bad
+        out = orthogonalize(g2)
+        assert out[1:3].isnan().all() and torch.equal(out[[0, 3]], clean[[0, 3]])
+        w, m = torch.zeros_like(g2), torch.zeros(g2.shape, device=DEV)
+        muon_step(list(w), list(g2), list(m))
+        assert w[1:3].isnan().all() and torch.isfinite(w[[0, 3]]).all() and torch.isfinite(m).sum() == m.numel() - 2

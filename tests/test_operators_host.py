@@ -351,3 +351,14 @@ def test_layer_norm_refuses_what_has_no_features_or_no_tensors(monkeypatch):
     for args in (([1.0] * 8, None), (None, 1.0), (2.0, None)):
         with pytest.raises(CnfError):
             layer_norm(torch.randn(4, 8, requires_grad=True), *args)
+
+
+def test_matrix_plan():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd import _native as nat
+    assert nat.matrix_plan(1, 64, 64) == (0, 0, 64, 64, 64) and nat.matrix_plan(3, 64, 5000)[:2] == (1, 0)
+    for shape in ((1, 200, 300), (8, 1024, 512), (16, 1000, 1000)):
+        assert nat.matrix_plan(*shape) == nat.matrix_plan(shape[0], shape[2], shape[1]) and nat.matrix_plan(*shape)[0] == 2
+    for bad in ((0, 8, 8), (65, 8, 8), (1, 0, 8), (1, 8, 65537)):
+        with pytest.raises(CnfError):
+            nat.matrix_plan(*bad)
