@@ -964,3 +964,18 @@ def test_orthogonalize_keeps_matrices_apart(rows, cols, dtype):
         w, m = torch.zeros_like(g2), torch.zeros(g2.shape, device=DEV)
         muon_step(list(w), list(g2), list(m))
         assert w[1:3].isnan().all() and torch.isfinite(w[[0, 3]]).all() and torch.isfinite(m).sum() == m.numel() - 2
+
+
+# ---- weight gradients over many rows --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows, cols, dtype, wdtype", [
+    (4099, 1001, F16, F32), (4097, 320, BF16, F32), (70001, 16, F32, F32), (20011, 64, BF16, BF16),   # a wave's lanes a row, more row groups than workgroups
+    (1500, 2048, F32, F32), (1500, 2048, BF16, BF16), (2100, 1999, BF16, F32), (1300, 3001, F16, F16),
+    (700, 8192, F32, F32), (700, 8192, F16, F16), (1100, 4100, F32, F32),                              # a workgroup a row, more rows than workgroups
+    (300, 9000, F32, F32), (300, 9000, BF16, BF16), (20000, 8200, F16, F32)], ids=str)                 # long rows: several parts, the most parts
+def test_layer_norm_weight_gradients_over_many_rows(rows, cols, dtype, wdtype):
+    x, w, b, dy = norm_inputs(rows, cols, dtype, wdtype, 12)
+    first = norm_both(x, w, b, dy)
+    for name, got, (want, tol) in zip(("y", "dx", "dw", "db"), first, norm_reference(x, w, b, 1e-5, dy, dtype, wdtype)):
+        check(got, want, tol, name)
+    assert all(torch.equal(p, q) for p, q in zip(first, norm_both(x, w, b, dy)))
