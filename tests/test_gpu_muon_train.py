@@ -153,3 +153,57 @@ def test_fused_muon_step_says_that_a_flow_has_no_hidden_matrices():
     from gan_flow_amd import gu_ffjord
     with pytest.raises(ValueError, match="at least two hidden layers"):
         gu_ffjord.FusedTrainStep(_model(dims=(64,)), _batches(1)[0], optimizer="muon", muon=MUON)
+
+
+def _compare(model_kw, muon, batches, coeffs=None, **step_kw):
+    """The captured iteration against the autograd loop on the same batches, as above."""
+    from gan_flow_amd import gu_ffjord
+    from gan_flow_amd.lib.optim import MuonWithAdam
+    ref = _model(**model_kw)
+    opt = MuonWithAdam(ref, muon, dict(lr=1e-3, weight_decay=1e-5))
+    want = []
+    for x in batches:
+        opt.zero_grad(set_to_none=True)
+        loss = gu_ffjord.compute_loss(ref, x)
+        if coeffs:
+            loss = loss + gu_ffjord.get_regularization(ref, coeffs)
+        loss.backward()
+        opt.step()
+        want.append(loss.item())
+    model = _model(**model_kw)
+    step = gu_ffjord.FusedTrainStep(model, batches[0], lr=1e-3, weight_decay=1e-5, optimizer="muon", muon=muon, reg_coeffs=coeffs, **step_kw)
+    got = [step(x).item() for x in batches]
+    step.check()
+    assert all(abs(a - b) <= 1e-4 * abs(a) for a, b in zip(want, got)), (want, got)
+    assert (_flat(ref) - _flat(model)).abs().max().item() <= 1e-4
+
+
+@pytest.mark.parametrize("layer_type", ["concat_v2", "squash"])
+def test_fused_muon_step_of_other_layer_types(layer_type):
+    _compare(dict(layer_type=layer_type, dims=(64, 48, 64)), MUON, _batches())
+
+
+@pytest.mark.parametrize("kw", [dict(nesterov=False), dict(adjust_lr="match_rms_adamw", lr=0.005), dict(ns_steps=3, ns_coefficients=[(4.0, -6.0, 2.5), (3.0, -3.5, 1.4),
+                                (1.5, -0.5, 0.0)]), dict(adjust_lr=0.5, eps=1e-3)], ids=str)
+def test_fused_muon_step_takes_muons_arguments(kw):
+    _compare(dict(), dict(MUON, **kw), _batches(), spread=False)
+
+
+def test_fused_muon_step_with_kinetic_regularisers():
+    from gan_flow_amd.lib.layers.wrappers import cnf_regularization as creg
+    _compare(dict(blocks=2, regularization_fns=(creg.l1_regularzation_fn, creg.l2_regularzation_fn)), MUON, _batches(), coeffs=[0.5, 0.25])
+
+
+def test_fused_muon_step_with_a_device_sampler():
+    from gan_flow_amd import gu_ffjord
+    from gan_flow_amd.gu import make_gu
+    runs = []
+    for _ in range(2):
+        model = _model()
+        sampler = make_gu(8, seed=3, extend_dim=True).device_sampler(torch.device(DEV))
+        step = gu_ffjord.FusedTrainStep(model, torch.zeros(512, 2, device=DEV), sampler=sampler, warmup=2, optimizer="muon", muon=MUON)
+        losses = [step().item() for _ in range(5)]
+        step.check()
+        runs.append((losses, _flat(model)))
+        assert step.step_count == 7
+    assert runs[0][0] == runs[1][0] and torch.equal(runs[0][1], runs[1][1]) and torch.isfinite(runs[0][1]).all()

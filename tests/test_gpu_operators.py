@@ -979,3 +979,27 @@ def test_layer_norm_weight_gradients_over_many_rows(rows, cols, dtype, wdtype):
     for name, got, (want, tol) in zip(("y", "dx", "dw", "db"), first, norm_reference(x, w, b, 1e-5, dy, dtype, wdtype)):
         check(got, want, tol, name)
     assert all(torch.equal(p, q) for p, q in zip(first, norm_both(x, w, b, dy)))
+
+
+@pytest.mark.parametrize("shape", [(2, 40, 900), (2, 900, 230), (12, 700, 760)])
+def test_matrix_products_captured_and_replayed(shape):
+    """Orthogonalisation and update of every path in one captured graph, replayed with eager work between."""
+    from gan_flow_amd.lib.optim import muon_step, orthogonalize
+    gen = torch.Generator(device=DEV).manual_seed(46)
+    new = lambda: torch.randn(shape, generator=gen, device=DEV)  # noqa: E731
+    w, g, m = new(), new(), new()
+    we, me = w.clone(), m.clone()
+    muon_step(list(we), list(g), list(me)), orthogonalize(g)   # (before the capture, on copies that are put back)
+    we.copy_(w), me.copy_(m)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        muon_step(list(w), list(g), list(m))
+        out = orthogonalize(g)
+    for _ in range(3):
+        g.copy_(new())
+        graph.replay()
+        muon_step(list(we), list(g), list(me))
+        want = orthogonalize(g)
+        torch.cuda.synchronize()
+        assert torch.equal(w, we) and torch.equal(m, me) and torch.equal(out, want)
