@@ -508,9 +508,10 @@ __global__ __launch_bounds__(256) void tile64_kernel(ArgsOf<kMode> a) {
 // T x T tiles for larger products: waves of kNu x kNv MFMA tiles share kStages stages of one block column each.  The operands of each 16 k are
 // read while the products of the 16 before are computed, and the stage's one barrier falls between the two halves, with products on
 // either side; the loop holds no branch, so that the compiler (T = 256) or the group barriers (kDealt) can place the reads and copies
-// between the products.  4096 x 4096 x 4096 with T = 256: 300 us (1.38 PFLOP/s of piece products; a large library product of fp16 matrices: 1.35),
-// against 374 with reads and products in turn and 335 with the copies under a condition; the products alone, on operands that
-// stay in registers, take 252 us: the device's power limit (177 with zeros for operands).
+// between the products.  4096 x 4096 x 4096 with T = 256, the loop timed by itself: 300 us (1.38 PFLOP/s of piece products; a large library product of
+// fp16 matrices: 1.35), against 374 with reads and products in turn and 335 with the copies under a condition; the products alone, on operands that
+// stay in registers, take 252 us: the device's power limit (177 with zeros for operands).  The kernel among the others of a call, its results stored: 347
+// us (1.19 PFLOP/s).
 template <int T, int kNu, int kNv, int kStages, int kMode, int kTerms, typename O = float, bool kMuon = false>
 __global__ __launch_bounds__((T / 32 / kNu) * (T / 32 / kNv) * 64) void tile_kernel(ArgsOf<kMode> a) {
     constexpr int kAcross = T / 32 / kNv, kW = T / 32 / kNu * kAcross, kStage = 2 * T * 128, kLoads = kStage / 1024 / kW;

@@ -148,9 +148,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 
 class LayerNorm(nn.Module):
-    """Per-row normalisation of the hidden features of a network trained beside a flow (a conditioner, a critic, an encoder):
-    unlike MovingBatchNorm1d it keeps rows apart -- log-likelihoods of single rows, gradient penalties -- and has no running
-    state.  Not a flow layer (it is not invertible): y = layer_norm(x, weight, bias, eps).  The reference has no such layer."""
+    """Per-row normalisation of the hidden features of a network trained beside a flow (a conditioner, an encoder): unlike
+    MovingBatchNorm1d it keeps rows apart -- log-likelihoods of single rows -- and has no running state.  Differentiable once: not for a
+    gradient penalty, which differentiates the backward pass.  Not a flow layer (it is not invertible): y = layer_norm(x, weight, bias, eps).
+    The reference has no such layer."""
 
     def __init__(self, num_features, eps=1e-5, affine=True):
         super().__init__()

@@ -325,7 +325,7 @@ int cnf_gu_sample_rows(const CnfGuDesc *gu, uint64_t seed, uint32_t call, int64_
 /* Element types of the operators below: tensors are fp32, fp16 or bf16; every sum, statistic and state is fp32 or wider. */
 enum { CNF_F32 = 0, CNF_F16 = 1, CNF_BF16 = 2 };
 
-/* Layer normalisation of the rows of a (rows x cols) matrix, for the networks trained beside a flow (conditioners, critics,
+/* Layer normalisation of the rows of a (rows x cols) matrix, for the networks trained beside a flow (conditioners,
  * encoders), whose rows must not mix as they do in a batch norm.  NO COUNTERPART IN THE REFERENCE'S PATH.
  *     y = (x - mean) * rstd * weight + bias,   mean = sum(x) / cols,   rstd = (sum((x - mean)^2) / cols + eps)^(-1/2)
  *   x: rows of `cols` contiguous elements, x_stride elements apart (0: one row repeated; rows may overlap);
@@ -349,7 +349,7 @@ int cnf_layer_norm_bwd(const void *dy, int64_t dy_stride, const void *x, int64_t
  * COUNTERPART IN THE REFERENCE, which trains with Adam.
  *     X = G / (|G|_F + eps);   for every step k:   A = X X^T,   X <- a[k] X + (b[k] A + c[k] A^2) X        (fewer rows than
  * columns; a matrix with more rows than columns is iterated transposed), i.e. an odd polynomial of the singular values.
- * fp32 accuracy whatever the type.  Refused: coefficients whose polynomial leaves [-7.5, 7.5] on the
+ * fp32 accuracy whatever the type: operands of 23 bits, at most twice the error of plain fp32 products.  Refused: coefficients whose polynomial leaves [-7.5, 7.5] on the
  * singular values it is applied to (it would diverge).  */
 #define CNF_NS_MAX_STEPS 16
 #define CNF_MAX_MATRICES 64
