@@ -93,7 +93,7 @@ EXPORTS = ("cnf_param_count", "cnf_workspace_bytes", "cnf_last_error", "cnf_eval
            "cnf_solve_fwd_static", "cnf_static_scratch_bytes", "cnf_gu_sample", "cnf_gu_sample_rows", "cnf_solve_fwd_times",
            "cnf_solve_fwd_reg", "cnf_solve_bwd_reg", "cnf_layer_norm_fwd", "cnf_layer_norm_workspace_bytes",
            "cnf_layer_norm_bwd", "cnf_orthogonalize_workspace_bytes", "cnf_orthogonalize", "cnf_muon_step",
-           "cnf_debug_matrix_plan")
+           "cnf_newton_schulz_check", "cnf_debug_matrix_plan")
 
 
 def library_path(act="tanh"):
@@ -164,6 +164,8 @@ def load_library(act="tanh"):
     lib.cnf_layer_norm_bwd.restype = ctypes.c_int
     lib.cnf_layer_norm_bwd.argtypes = [P, I64, P, I64, I32, P, I32, P, P, I64, I64, P, P, P, P, SZ, VP]
     NS, MO, PP = ctypes.POINTER(CnfNewtonSchulz), ctypes.POINTER(CnfMuonOpts), ctypes.POINTER(ctypes.c_void_p)
+    lib.cnf_newton_schulz_check.restype = ctypes.c_int
+    lib.cnf_newton_schulz_check.argtypes = [NS]
     lib.cnf_orthogonalize_workspace_bytes.restype = SZ
     lib.cnf_orthogonalize_workspace_bytes.argtypes = [I64, I64, I64]
     lib.cnf_orthogonalize.restype = ctypes.c_int
@@ -716,6 +718,16 @@ def ns_params(steps, coefficients, eps):
     if type(coefficients) is not tuple or any(hasattr(c, "__len__") for c in coefficients):
         coefficients = tuple(tuple(c) if hasattr(c, "__len__") else c for c in coefficients)
     return _newton_schulz(int(steps), coefficients, float(eps))
+
+
+def checked_ns_params(steps, coefficients, eps):
+    """ns_params, refused here where a call would refuse it."""
+    ns = ns_params(steps, coefficients, eps)
+    if not getattr(ns, "checked", False):
+        lib = load_library()
+        _check(lib.cnf_newton_schulz_check(ctypes.byref(ns)), lib)
+        ns.checked = True
+    return ns
 
 
 def _stack(t, name, dtype):

@@ -885,6 +885,12 @@ static int check_ptrs(const char* who, const char* name, const void* const* p, i
     return 0;
 }
 
+int cnf_newton_schulz_check(const CnfNewtonSchulz* ns) {
+    const char* who = "cnf_newton_schulz_check";
+    if (!ns) return fail("%s: NULL pointer", who);
+    return check_ns(who, ns);
+}
+
 size_t cnf_orthogonalize_workspace_bytes(int64_t count, int64_t rows, int64_t cols) {
     if (count < 1 || count > CNF_MAX_MATRICES || rows < 1 || cols < 1 || rows > CNF_MAX_MATRIX_DIM || cols > CNF_MAX_MATRIX_DIM) return 0;
     return cnf::muon_workspace_bytes(count, rows, cols);

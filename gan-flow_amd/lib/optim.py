@@ -173,7 +173,7 @@ class Muon(torch.optim.Optimizer):
         if not (0.0 <= lr < math.inf and 0.0 <= momentum < 1.0 and 0.0 <= weight_decay < math.inf and 0.0 < eps < math.inf and 0.0 <= scale < math.inf):
             raise ValueError("invalid hyper-parameters (lr %r, momentum %r, weight_decay %r, eps %r, adjust_lr %r)"
                              % (lr, momentum, weight_decay, eps, group["adjust_lr"]))
-        return _native.ns_params(group["ns_steps"], group["ns_coefficients"], eps)
+        return _native.checked_ns_params(group["ns_steps"], group["ns_coefficients"], eps)
 
     def load_state_dict(self, state_dict):
         """A state of this class only: other optimizers keep a `momentum_buffer` too (torch.optim.Muon an average of the gradients, 1 - momentum
@@ -208,8 +208,11 @@ class Muon(torch.optim.Optimizer):
                     state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
                 by_shape.setdefault(p.shape, []).append((p, p.grad, state["momentum_buffer"]))
             hyper = {k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay")}
-            updates += [(_side_by_side(*zip(*members)), ns, dict(hyper, scale=adjusted_scale(group["adjust_lr"], *shape)))
-                        for shape, members in by_shape.items()]
+            for shape, members in by_shape.items():
+                scale = adjusted_scale(group["adjust_lr"], *shape)
+                if not math.isfinite(hyper["lr"] * scale) or not math.isfinite(hyper["lr"] * hyper["weight_decay"]):
+                    raise ValueError("invalid hyper-parameters (lr %r, weight_decay %r, scale %r)" % (hyper["lr"], hyper["weight_decay"], scale))
+                updates.append((_side_by_side(*zip(*members)), ns, dict(hyper, scale=scale)))
         for calls, ns, hyper in updates:
             _update(calls, ns, **hyper)
         return loss

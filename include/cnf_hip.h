@@ -360,6 +360,7 @@ typedef struct CnfNewtonSchulz {
     double eps;          /* > 0 */
     double a[CNF_NS_MAX_STEPS], b[CNF_NS_MAX_STEPS], c[CNF_NS_MAX_STEPS];
 } CnfNewtonSchulz;
+int cnf_newton_schulz_check(const CnfNewtonSchulz *ns);   /* 0, or refused as the calls below would refuse it */
 
 /*   g, out: HOST arrays of `count` (1 .. CNF_MAX_MATRICES) device pointers to rows x cols (each 1 .. CNF_MAX_MATRIX_DIM) matrices of type dtype with
  *   contiguous rows, ldg / ldo elements apart; copied into the kernels' arguments (capturable).  out[i] may be g[i] (with the

@@ -1003,3 +1003,24 @@ def test_matrix_products_captured_and_replayed(shape):
         want = orthogonalize(g)
         torch.cuda.synchronize()
         assert torch.equal(w, we) and torch.equal(m, me) and torch.equal(out, want)
+
+
+def test_a_later_group_of_muon_that_would_diverge_leaves_the_first_alone():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd.lib.optim import Muon
+    gen = torch.Generator().manual_seed(47)
+    params = [torch.nn.Parameter(torch.randn(s, generator=gen).to(DEV)) for s in ((64, 64), (70, 90))]
+    opt = Muon(params[:1])
+    opt.add_param_group(dict(params=params[1:]))
+    for p in params:
+        p.grad = torch.randn(p.shape, generator=gen).to(DEV)
+    saved = [p.detach().clone() for p in params]
+    for bad, error in ((dict(ns_coefficients=(9.0, 0.0, 0.0)), CnfError), (dict(lr=1e300, adjust_lr=1e300), ValueError), (dict(momentum=1.0), ValueError)):
+        keep = dict(opt.param_groups[1])
+        opt.param_groups[1].update(bad)
+        with pytest.raises(error):
+            opt.step()
+        opt.param_groups[1].update(keep)
+        assert all(torch.equal(p, s) for p, s in zip(params, saved))
+    opt.step()
+    assert not any(torch.equal(p, s) for p, s in zip(params, saved))

@@ -362,3 +362,24 @@ def test_matrix_plan():
     for bad in ((0, 8, 8), (65, 8, 8), (1, 0, 8), (1, 8, 65537)):
         with pytest.raises(CnfError):
             nat.matrix_plan(*bad)
+
+
+def test_newton_schulz_check_refuses_what_a_call_would():
+    from gan_flow_amd import CnfError
+    from gan_flow_amd import _native as nat
+    from gan_flow_amd.lib.optim import Muon
+    lib = nat.load_library()
+    assert lib.cnf_newton_schulz_check(None) != 0 and b"NULL" in lib.cnf_last_error()
+    assert lib.cnf_newton_schulz_check(ctypes.byref(_ns(nat))) == 0
+    for kw, words in ((dict(coefficients=(9.0, 0.0, 0.0)), b"diverge"), (dict(eps=0.0), b"eps")):
+        assert lib.cnf_newton_schulz_check(ctypes.byref(_ns(nat, **kw))) != 0 and words in lib.cnf_last_error()
+    p = torch.nn.Parameter(torch.zeros(4, 8))
+    opt = Muon([p])
+    with pytest.raises(CnfError, match="diverge"):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(4, 8))], ns_coefficients=(9.0, 0.0, 0.0)))
+    with pytest.raises(CnfError, match="diverge"):
+        Muon([p], ns_coefficients=(9.0, 0.0, 0.0))
+    p.grad = torch.ones(4, 8)
+    opt.param_groups[0].update(lr=1e300, adjust_lr=1e300)
+    with pytest.raises(ValueError, match="hyper-parameters"):
+        opt.step()
